@@ -39,6 +39,7 @@ GA_BOOL, GA_BYTE, GA_UBYTE, GA_SHORT, GA_USHORT = 0, 1, 2, 3, 4
 GA_INT, GA_UINT, GA_LONG, GA_ULONG = 5, 6, 7, 8
 GA_FLOAT, GA_DOUBLE, GA_CFLOAT, GA_CDOUBLE = 11, 12, 14, 15
 GA_HALF, GA_SIZE, GA_SSIZE = 23, 24, 25
+GA_BFLOAT16 = 511
 
 GA_C_CONTIGUOUS = 0x0001
 GA_F_CONTIGUOUS = 0x0002
@@ -232,6 +233,13 @@ SIGNATURES = {
                                     C.c_int]),
     "GpuReduction_call_noalloc": (C.c_int, [C.c_void_p, PA, PA, PA, C.c_uint, C.POINTER(C.c_int),
                                             C.c_int]),
+    # language.h
+    "GpuArray_embedding": (C.c_int, [PA, PA, PA, C.c_double, c_ssize_t, C.c_int]),
+    "GpuArray_embedding_grad": (C.c_int, [PA, PA, PA, C.c_double, c_ssize_t, C.c_int, C.c_int]),
+    "GpuArray_token_logprobs": (C.c_int, [PA] * 7 + [C.c_double, c_ssize_t, C.c_int]),
+    "GpuArray_token_logprobs_grad": (C.c_int, [PA] * 7 + [C.c_double, c_ssize_t, C.c_int]),
+    "GpuArray_global_norm": (C.c_int, [PA, C.POINTER(PA), C.c_size_t]),
+    "GpuArray_clip_global_norm": (C.c_int, [C.POINTER(PA), C.POINTER(PA), C.c_size_t, C.c_double, PA]),
 }
 
 for _name, (_res, _args) in SIGNATURES.items():

@@ -250,8 +250,17 @@ def main():
         check("take1 chunks=%d types=%d,%d,%d nd=%d" % (chunks, a_tc, v_tc, i_tc, tnd),
               gen_t(chunks, a_tc, v_tc, i_tc, tnd))
         t += 1
+    # operators of language models: (operator, operand, result, ids) as the library packs them
+    gen_l = ext(b"hip_language_source", C.c_void_p, [C.c_ulonglong])
+    GA_BFLOAT16 = 511
+    lm = 0
+    for kind in range(6):
+        for x, o in [(GA_FLOAT, GA_FLOAT), (GA_BFLOAT16, GA_FLOAT), (GA_HALF, GA_BFLOAT16)]:
+            check("language operator %d types %d, %d" % (kind, x, o),
+                  gen_l(kind | x << 8 | o << 20 | (GA_LONG if o == GA_FLOAT else GA_INT) << 32))
+            lm += 1
     print("device sources compile for gfx950 (%d reduction variants, %d map-reduce, %d take1, "
-          "50 elementwise)" % (n + 20, m, t))
+          "50 elementwise, %d of language operators)" % (n + 20, m, t, lm))
 
 
 if __name__ == "__main__":

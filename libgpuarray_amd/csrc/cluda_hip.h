@@ -96,6 +96,15 @@ static __device__ inline ga_half ga_float2half(float f) {
   return r;
 }
 
+/* bfloat16, the upper half of a float: converts to float exactly, and from
+ * float to nearest even with the hardware converter. */
+struct ga_bfloat16 {
+  ga_ushort data;
+  ga_bfloat16() = default;
+  __device__ ga_bfloat16(float f) : data(__builtin_bit_cast(ga_ushort, (__bf16)f)) {}
+  __device__ operator float() const { return __builtin_bit_cast(float, (ga_uint)data << 16); }
+};
+
 /* atom_{add,xchg}_<type><space>: type i/I/l/L/f/d/e = int/uint/long/ulong/
  * float/double/half, space g/l = global/local.  Flat addressing makes the
  * two spaces one implementation. */

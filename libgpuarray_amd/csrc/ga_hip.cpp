@@ -320,6 +320,7 @@ struct hip_context : _gpucontext {
   uint64_t last_launch_hash = 0;   // text_hash of the kernel launched last
   void *redux_cache = nullptr;
   void *take1_cache = nullptr;
+  void *language_cache = nullptr;
   mem_cache mem;
   std::string disk_cache;   // directory of the on-disk kernel cache, empty = off
   void *stage = nullptr;    // pinned host memory that small reads and writes go through
@@ -658,6 +659,7 @@ void hip_deinit(gpucontext *c) {
   ga_extcopy_cache_free(c);
   ga_redux_cache_free(c);
   ga_take1_cache_free(c);
+  ga_language_cache_free(c);
   if (ctx->fill_kernel) {
     hip_freekernel(ctx->fill_kernel);
     ctx->fill_kernel = nullptr;
@@ -1719,6 +1721,7 @@ extern "C" char *ga_elemwise_gen_source(const char *preamble, const char *expr, 
                                         unsigned int nd, int idx64, unsigned int tmask);
 extern "C" char *ga_reduction_gen_source(int op, int src_tc, int d0_tc, int d1_tc, unsigned int G,
                                          unsigned int V, unsigned int U);
+char *ga_language_gen_source(unsigned long long variant);
 extern "C" char *ga_take1_gen_source(int chunks, int a_tc, int v_tc, int i_tc, unsigned int tnd);
 extern "C" char *ga_mapreduce_gen_source(int op, const char *reduce_expr, const char *neutral,
                                          int acc_tc, const char *preamble, const char *map_expr,
@@ -1832,6 +1835,7 @@ const ext_entry k_exts[] = {
     {"hip_mapreduce_source", (void *)ga_mapreduce_gen_source},
     {"hip_module_cache_stats", (void *)ext_module_cache_stats},
     {"hip_take1_source", (void *)ga_take1_gen_source},
+    {"hip_language_source", (void *)ga_language_gen_source},
     {"hip_reload_tuning", (void *)ext_reload_tuning},
 };
 
@@ -1862,6 +1866,8 @@ gpudata *ga_hip_scratch(gpucontext *c, size_t bytes) {
   ctx->scratch_sz = want;
   return ctx->scratch;
 }
+
+size_t ga_hip_scratch_size(gpucontext *c) { return HC(c)->scratch_sz; }
 
 gpudata *ga_hip_static_scratch_buf(gpucontext *c, const char **why) {
   hip_context *ctx = HC(c);
@@ -1957,6 +1963,7 @@ void ga_tuning_read(ga_tuning *t) {
 }
 void **ga_hip_redux_cache_slot(gpucontext *c) { return &HC(c)->redux_cache; }
 void **ga_hip_take1_cache_slot(gpucontext *c) { return &HC(c)->take1_cache; }
+void **ga_hip_language_cache_slot(gpucontext *c) { return &HC(c)->language_cache; }
 
 const ga_buffer_ops ga_hip_ops = {
     hip_get_platform_count, hip_get_device_count, hip_init,        hip_deinit,

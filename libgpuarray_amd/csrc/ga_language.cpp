@@ -1,0 +1,655 @@
+// Operators of language models: embedding rows and their gradient, log
+// probabilities of tokens and their gradient, the global norm of many arrays
+// and clipping by it.  The rules are those of gpuarray/language.h; the kernels
+// are in language_kernels.h and are compiled per operator and set of types,
+// kept for the life of the context like those of GpuArray_take1.
+#include "private.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <unordered_map>
+#include <vector>
+
+namespace {
+
+// ---- kernels of a context ------------------------------------------------------
+
+enum lm_kind { LM_EMBED, LM_EMBED_GRAD, LM_LOGPROBS, LM_LOGPROBS_GRAD, LM_NORM, LM_CLIP };
+
+// What a kernel text is specialised on; packed into the key it is kept under.
+struct lm_variant {
+  unsigned kind, x, o, id;   // operator; typecodes of operand, result, ids
+  unsigned extra;            // the operator's own
+  unsigned long long key() const {
+    return (unsigned long long)kind | (unsigned long long)x << 8 | (unsigned long long)o << 20 |
+           (unsigned long long)id << 32 | (unsigned long long)extra << 44;
+  }
+  explicit lm_variant(unsigned long long k)
+      : kind(k & 0xff), x(k >> 8 & 0xfff), o(k >> 20 & 0xfff), id(k >> 32 & 0xfff), extra((unsigned)(k >> 44)) {}
+  lm_variant(unsigned kind_, int x_, int o_, int id_, unsigned extra_)
+      : kind(kind_), x((unsigned)x_), o((unsigned)o_), id((unsigned)id_), extra(extra_) {}
+};
+
+const unsigned LM_TENSORS = 112;   // arrays per launch of the norm and clip kernels
+
+// Arguments of the kernels, as language_kernels.h declares them.
+struct embed_args {
+  void *out;
+  const void *table, *ids;
+  void *err;
+  int64_t out_row, table_row, id_step;
+  int64_t n, v, d, ignore;
+  float scale;
+};
+struct embed_grad_args {
+  void *grad;
+  const void *dout, *ids;
+  void *err;
+  int64_t grad_row, dout_row, id_step;
+  int64_t n, v, d, ignore;
+  float scale;
+  int32_t accumulate;
+};
+struct logprobs_args {
+  const void *logits, *ids;
+  void *logp, *entropy, *stats, *top_logp, *top_ids;
+  void *err;
+  int64_t row, id_step, logp_step, entropy_step, stats_row, stats_col;
+  int64_t topl_row, topl_col, topi_row, topi_col;
+  int64_t t, v, ignore;
+  float scale;
+  int32_t top, top_long;
+};
+struct logprobs_grad_args {
+  void *out;
+  const void *logits, *ids, *stats, *dlogp, *entropy, *dentropy;
+  void *err;
+  int64_t out_row, row, id_step, stats_row, stats_col, dlogp_step, entropy_step, dentropy_step;
+  int64_t t, v, ignore;
+  float scale;
+};
+const int64_t LM_PIECE = 8192;
+struct tensors_args {
+  void *partials, *result, *norm;
+  double max_norm;
+  int64_t partial0, npartials;
+  int32_t n, norm_double, clip, pad;
+  const void *in[LM_TENSORS];
+  void *out[LM_TENSORS];
+  int64_t count[LM_TENSORS];
+  uint32_t first[LM_TENSORS + 1];
+  unsigned char type[LM_TENSORS];
+};
+
+std::string lm_source(const lm_variant &v) {
+  std::string s = "#define LM_KIND " + std::to_string(v.kind) + "\n#define LM_TENSORS " + std::to_string(LM_TENSORS) + "\n";
+  auto name = [&](const char *what, unsigned tc) {
+    const char *c = gpuarray_get_type((int)tc)->cluda_name;
+    s += std::string("#define ") + what + " " + (c ? c : "ga_float") + "\n";
+  };
+  name("LM_X", v.x);
+  name("LM_O", v.o);
+  name("LM_ID", v.id);
+  return s + ga_language_kernels_src;
+}
+
+typedef std::unordered_map<std::string, GpuKernel> lm_cache;
+
+// The kernel `name` of a variant, from the context's cache or built.  Building
+// loads a code object, which a stream that records a graph does not allow.
+int lm_kernel(gpucontext *ctx, const lm_variant &v, const char *name, size_t args_size, GpuKernel **out) {
+  void **slot = ga_hip_language_cache_slot(ctx);
+  if (*slot == nullptr) *slot = new lm_cache();
+  lm_cache &cache = *(lm_cache *)*slot;
+  const unsigned long long k = v.key();
+  std::string key((const char *)&k, sizeof(k));
+  key += name;
+  auto it = cache.find(key);
+  if (it != cache.end()) {
+    *out = &it->second;
+    return GA_NO_ERROR;
+  }
+  if (ga_hip_capturing(ctx))
+    return ga_err_fmt(ctx->err, GA_UNSUPPORTED_ERROR,
+                      "%s is not built yet and the stream records a graph: call once before recording", name);
+  const std::string s = lm_source(v);
+  const char *strs[1] = {s.c_str()};
+  size_t lens[1] = {s.size()};
+  const int types[1] = {ga_plan_typecode(args_size)};
+  GpuKernel nk = {nullptr, nullptr};
+  const int err = GpuKernel_init(&nk, ctx, 1, strs, lens, name, 1, types, 0, nullptr);
+  if (err != GA_NO_ERROR) return err;
+  *out = &cache.emplace(key, nk).first->second;
+  return GA_NO_ERROR;
+}
+
+int lm_launch(GpuKernel *k, size_t groups, size_t lanes, void *args) {
+  void *argv[1] = {args};
+  return GpuKernel_call(k, 1, &groups, &lanes, 0, argv);
+}
+
+// `bytes` of the context's scratch.
+int lm_scratch(gpucontext *ctx, size_t bytes, char **out) {
+  if (bytes > ga_hip_scratch_size(ctx) && ga_hip_capturing(ctx))
+    return ga_err_set(ctx->err, GA_UNSUPPORTED_ERROR,
+                      "The scratch has to grow and the stream records a graph: call once before recording");
+  gpudata *b = ga_hip_scratch(ctx, bytes);
+  if (b == nullptr) return ctx->err->code;
+  *out = (char *)b->devptr;
+  return GA_NO_ERROR;
+}
+
+// ---- checks of arguments -------------------------------------------------------
+
+inline char *at(const GpuArray *a) { return (char *)a->data->devptr + a->offset; }
+inline bool is_value(int tc) { return tc == GA_FLOAT || tc == GA_HALF || tc == GA_BFLOAT16; }
+
+// Lowest and one past the highest byte of an array; lo == hi: no element.
+void span_of(const GpuArray *a, uintptr_t *lo, uintptr_t *hi) {
+  uintptr_t l = (uintptr_t)at(a), h = l + GpuArray_ITEMSIZE(a);
+  for (unsigned i = 0; i < a->nd; i++) {
+    if (a->dimensions[i] == 0) {
+      *lo = *hi = 0;
+      return;
+    }
+    const ssize_t far = (ssize_t)(a->dimensions[i] - 1) * a->strides[i];
+    if (far < 0) l += (uintptr_t)far;
+    else h += (uintptr_t)far;
+  }
+  *lo = l;
+  *hi = h;
+}
+
+bool overlap(const GpuArray *a, const GpuArray *b) {
+  uintptr_t al, ah, bl, bh;
+  span_of(a, &al, &ah);
+  span_of(b, &bl, &bh);
+  return al < bh && bl < ah;
+}
+
+bool same_place(const GpuArray *a, const GpuArray *b) {
+  if (a->nd != b->nd || at(a) != at(b) || a->typecode != b->typecode) return false;
+  for (unsigned i = 0; i < a->nd; i++)
+    if (a->dimensions[i] != b->dimensions[i] || (a->dimensions[i] > 1 && a->strides[i] != b->strides[i])) return false;
+  return true;
+}
+
+// Whether two indices may reach one byte (dims nested by their steps never do).
+bool overlaps_itself(const GpuArray *a) {
+  std::vector<std::pair<size_t, size_t>> d;   // step, extent
+  for (unsigned i = 0; i < a->nd; i++) {
+    if (a->dimensions[i] == 0) return false;
+    if (a->dimensions[i] > 1) d.emplace_back((size_t)std::llabs((long long)a->strides[i]), a->dimensions[i]);
+  }
+  std::sort(d.begin(), d.end());
+  size_t run = GpuArray_ITEMSIZE(a);
+  for (auto &e : d) {
+    if (e.first < run) return true;
+    run += e.first * (e.second - 1);
+  }
+  return false;
+}
+
+// Checks of one operator's arguments; the first failure stays.
+struct checker {
+  gpucontext *ctx;
+  const char *who;
+  int err = GA_NO_ERROR;
+  checker(gpucontext *c, const char *w) : ctx(c), who(w) {}
+  int fail(int code, const char *what) {
+    if (err == GA_NO_ERROR) err = ga_err_fmt(ctx->err, code, "%s: %s", who, what);
+    return err;
+  }
+  int fail(int code, const char *what, const char *arg) {
+    if (err == GA_NO_ERROR) err = ga_err_fmt(ctx->err, code, "%s: %s: %s", who, arg, what);
+    return err;
+  }
+  // what every array has to be
+  void array(const GpuArray *a, const char *arg, unsigned nd) {
+    if (err != GA_NO_ERROR) return;
+    if (GpuArray_context(a) != ctx) fail(GA_INVALID_ERROR, "belongs to another context", arg);
+    else if (a->nd != nd) fail(GA_INVALID_ERROR, nd == 1 ? "must have one dim" : "must have two dims", arg);
+    else aligned(a, arg);
+  }
+  void aligned(const GpuArray *a, const char *arg) {
+    if (err != GA_NO_ERROR) return;
+    if (!GpuArray_ISALIGNED(a) || (uintptr_t)at(a) % gpuarray_get_type(a->typecode)->align != 0)
+      fail(GA_UNALIGNED_ERROR, "not aligned", arg);
+  }
+  void shape(const GpuArray *a, const char *arg, size_t d0) {
+    if (err == GA_NO_ERROR && a->dimensions[0] != d0) fail(GA_INVALID_ERROR, "length does not fit the others", arg);
+  }
+  void shape(const GpuArray *a, const char *arg, size_t d0, size_t d1) {
+    if (err == GA_NO_ERROR && (a->dimensions[0] != d0 || a->dimensions[1] != d1))
+      fail(GA_INVALID_ERROR, "shape does not fit the others", arg);
+  }
+  void rows(const GpuArray *a, const char *arg) {
+    if (err == GA_NO_ERROR && a->dimensions[1] > 1 && a->strides[1] != (ssize_t)GpuArray_ITEMSIZE(a))
+      fail(GA_INVALID_ERROR, "the last dim must have unit stride", arg);
+  }
+  void value_type(const GpuArray *a, const char *arg) {
+    if (err == GA_NO_ERROR && !is_value(a->typecode))
+      fail(GA_UNSUPPORTED_ERROR, "must be float, half or bfloat16", arg);
+  }
+  void type(const GpuArray *a, const char *arg, int tc) {
+    if (err == GA_NO_ERROR && a->typecode != tc) fail(GA_VALUE_ERROR, "must be float", arg);
+  }
+  void id_type(const GpuArray *a, const char *arg) {
+    if (err == GA_NO_ERROR && (a->typecode < GA_BYTE || a->typecode > GA_ULONG))
+      fail(GA_VALUE_ERROR, "must have an integer type", arg);
+  }
+  // a result: writeable, nothing written twice
+  void result(const GpuArray *a, const char *arg) {
+    if (err != GA_NO_ERROR) return;
+    if (!GpuArray_ISWRITEABLE(a)) fail(GA_VALUE_ERROR, "not writeable", arg);
+    else if (overlaps_itself(a)) fail(GA_VALUE_ERROR, "overlaps itself", arg);
+  }
+  void apart(const GpuArray *a, const GpuArray *b, const char *arg) {
+    if (err == GA_NO_ERROR && a != nullptr && b != nullptr && overlap(a, b))
+      fail(GA_VALUE_ERROR, "overlaps another argument", arg);
+  }
+  // a scale that a float holds
+  void scale(double s, bool positive) {
+    if (err == GA_NO_ERROR && (!std::isfinite((float)s) || (positive && !((float)s > 0.0f))))
+      fail(GA_VALUE_ERROR, positive ? "scale must be finite and above 0" : "scale must be finite");
+  }
+};
+
+// One-word errors of a kernel: the context's sticky error word, as GpuArray_take1 has it.
+int lm_errbuf(gpucontext *ctx, const GpuArray *any, gpudata **errbuf) {
+  (void)ctx;
+  return gpudata_property(any->data, GA_CTX_PROP_ERRBUF, errbuf);
+}
+int lm_check_error(gpucontext *ctx, gpudata *errbuf) {
+  int kerr = 0;
+  int err = gpudata_read(&kerr, errbuf, 0, sizeof(int));
+  if (err == GA_NO_ERROR && kerr != 0) {
+    err = ga_err_set(ctx->err, GA_VALUE_ERROR, "Index out of bounds");
+    kerr = 0;
+    gpudata_write(errbuf, 0, &kerr, sizeof(int));
+  }
+  return err;
+}
+
+int no_memory(gpucontext *ctx) { return ga_err_set(ctx->err, GA_MEMORY_ERROR, "Out of memory"); }
+
+const size_t MAX_GROUPS = 0x7fffffff;
+
+}  // namespace
+
+void ga_language_cache_free(gpucontext *ctx) {
+  void **slot = ga_hip_language_cache_slot(ctx);
+  if (*slot == nullptr) return;
+  lm_cache *cache = (lm_cache *)*slot;
+  *slot = nullptr;
+  for (auto &kv : *cache) GpuKernel_clear(&kv.second);
+  delete cache;
+}
+
+// The kernel text of a variant (packed as lm_variant::key packs it), as a
+// malloc'd string; behind the "hip_language_source" hook.
+char *ga_language_gen_source(unsigned long long variant) { return strdup(lm_source(lm_variant(variant)).c_str()); }
+
+// ---- embedding -----------------------------------------------------------------
+
+static int embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, double scale, ssize_t ignore,
+                     int check_error) {
+  gpucontext *ctx = GpuArray_context(out);
+  checker c(ctx, "embedding");
+  c.array(out, "out", 2);
+  c.array(table, "table", 2);
+  c.array(ids, "ids", 1);
+  if (c.err != GA_NO_ERROR) return c.err;
+  const size_t n = ids->dimensions[0], v = table->dimensions[0], d = table->dimensions[1];
+  c.shape(out, "out", n, d);
+  c.value_type(out, "out");
+  c.value_type(table, "table");
+  c.id_type(ids, "ids");
+  c.rows(out, "out");
+  c.rows(table, "table");
+  c.result(out, "out");
+  c.apart(out, table, "out");
+  c.apart(out, ids, "out");
+  c.scale(scale, false);
+  if (c.err != GA_NO_ERROR) return c.err;
+  if (n == 0 || d == 0) return GA_NO_ERROR;
+  if (n > MAX_GROUPS) return c.fail(GA_XLARGE_ERROR, "too many rows");
+  GpuKernel *k;
+  gpudata *errbuf = nullptr;
+  int err = lm_kernel(ctx, lm_variant(LM_EMBED, table->typecode, out->typecode, ids->typecode, 0), "lm_embed_rows",
+                      sizeof(embed_args), &k);
+  if (err == GA_NO_ERROR) err = lm_errbuf(ctx, out, &errbuf);
+  if (err != GA_NO_ERROR) return err;
+  embed_args a = {at(out), at(table), at(ids), errbuf->devptr, out->strides[0], table->strides[0], ids->strides[0],
+                  (int64_t)n, (int64_t)v, (int64_t)d, ignore, (float)scale};
+  err = lm_launch(k, n, 256, &a);
+  return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
+}
+
+static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *ids, double scale, ssize_t ignore,
+                          int accumulate, int check_error) {
+  gpucontext *ctx = GpuArray_context(grad);
+  checker c(ctx, "embedding_grad");
+  c.array(grad, "grad", 2);
+  c.array(dout, "dout", 2);
+  c.array(ids, "ids", 1);
+  if (c.err != GA_NO_ERROR) return c.err;
+  const size_t n = ids->dimensions[0], v = grad->dimensions[0], d = grad->dimensions[1];
+  c.shape(dout, "dout", n, d);
+  c.value_type(grad, "grad");
+  c.value_type(dout, "dout");
+  c.id_type(ids, "ids");
+  c.rows(grad, "grad");
+  c.rows(dout, "dout");
+  c.result(grad, "grad");
+  c.apart(grad, dout, "grad");
+  c.apart(grad, ids, "grad");
+  c.scale(scale, false);
+  if (c.err != GA_NO_ERROR) return c.err;
+  if (d == 0 || (v == 0 && n == 0)) return GA_NO_ERROR;
+  if (v > MAX_GROUPS || n > MAX_GROUPS) return c.fail(GA_XLARGE_ERROR, "too many rows");
+  GpuKernel *k;
+  gpudata *errbuf = nullptr;
+  int err = lm_kernel(ctx, lm_variant(LM_EMBED_GRAD, dout->typecode, grad->typecode, ids->typecode, 0),
+                      "lm_embed_grad_rows", sizeof(embed_grad_args), &k);
+  if (err == GA_NO_ERROR) err = lm_errbuf(ctx, grad, &errbuf);
+  if (err != GA_NO_ERROR) return err;
+  embed_grad_args a = {at(grad), at(dout), at(ids), errbuf->devptr, grad->strides[0], dout->strides[0],
+                       ids->strides[0], (int64_t)n, (int64_t)v, (int64_t)d, ignore, (float)scale, accumulate != 0};
+  err = lm_launch(k, v ? (v + 3) / 4 : 1, 256, &a);
+  return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
+}
+
+// ---- log probabilities -----------------------------------------------------------
+
+static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, GpuArray *top_logp, GpuArray *top_ids,
+                          const GpuArray *logits, const GpuArray *ids, double scale, ssize_t ignore, int check_error) {
+  gpucontext *ctx = GpuArray_context(logits);
+  checker c(ctx, "token_logprobs");
+  c.array(logits, "logits", 2);
+  if (c.err != GA_NO_ERROR) return c.err;
+  const size_t t = logits->dimensions[0], v = logits->dimensions[1];
+  c.value_type(logits, "logits");
+  c.rows(logits, "logits");
+  if ((logp == nullptr) != (ids == nullptr)) return c.fail(GA_VALUE_ERROR, "logp and ids go together");
+  if ((top_logp == nullptr) != (top_ids == nullptr)) return c.fail(GA_VALUE_ERROR, "top_logp and top_ids go together");
+  if (ids != nullptr) {
+    c.array(ids, "ids", 1);
+    c.id_type(ids, "ids");
+    c.shape(ids, "ids", t);
+  }
+  GpuArray *const results[5] = {logp, entropy, stats, top_logp, top_ids};
+  const char *const names[5] = {"logp", "entropy", "stats", "top_logp", "top_ids"};
+  for (int i = 0; i < 5; i++) {
+    if (results[i] == nullptr) continue;
+    c.array(results[i], names[i], i < 2 ? 1 : 2);
+    if (c.err != GA_NO_ERROR) return c.err;
+    if (i < 2) c.shape(results[i], names[i], t);
+    else if (i == 2) c.shape(stats, names[i], t, 2);
+    else c.shape(results[i], names[i], t, top_ids->nd == 2 ? top_ids->dimensions[1] : 0);
+    if (i < 4) c.type(results[i], names[i], GA_FLOAT);
+    else if (top_ids->typecode != GA_INT && top_ids->typecode != GA_LONG)
+      c.fail(GA_VALUE_ERROR, "must be int or long", names[i]);
+    c.result(results[i], names[i]);
+    c.apart(results[i], logits, names[i]);
+    c.apart(results[i], ids, names[i]);
+    for (int j = 0; j < i; j++) c.apart(results[i], results[j], names[i]);
+  }
+  c.scale(scale, true);
+  if (c.err != GA_NO_ERROR) return c.err;
+  const size_t top = top_ids ? top_ids->dimensions[1] : 0;
+  if (top > GA_TOKEN_LOGPROBS_MAX_TOP || top > v)
+    return c.fail(GA_VALUE_ERROR, "more alternatives than the vocabulary or GA_TOKEN_LOGPROBS_MAX_TOP has");
+  if (t == 0 || (logp == nullptr && entropy == nullptr && stats == nullptr && top == 0)) return GA_NO_ERROR;
+  if (v == 0) return c.fail(GA_VALUE_ERROR, "empty vocabulary");
+  if (t > MAX_GROUPS || v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many rows or columns");
+  GpuKernel *k;
+  gpudata *errbuf = nullptr;
+  int err = lm_kernel(ctx, lm_variant(LM_LOGPROBS, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT, 0),
+                      "lm_logprobs_rows", sizeof(logprobs_args), &k);
+  if (err == GA_NO_ERROR) err = lm_errbuf(ctx, logits, &errbuf);
+  if (err != GA_NO_ERROR) return err;
+  auto ptr = [](const GpuArray *x) -> void * { return x ? at(x) : nullptr; };
+  auto step = [](const GpuArray *x, unsigned i) -> int64_t { return x ? x->strides[i] : 0; };
+  logprobs_args a = {at(logits), ptr(ids), ptr(logp), ptr(entropy), ptr(stats), ptr(top_logp), ptr(top_ids),
+                     errbuf->devptr, logits->strides[0], step(ids, 0), step(logp, 0), step(entropy, 0), step(stats, 0),
+                     step(stats, 1), step(top_logp, 0), step(top_logp, 1), step(top_ids, 0), step(top_ids, 1),
+                     (int64_t)t, (int64_t)v, ignore, (float)scale, (int32_t)top,
+                     top_ids != nullptr && top_ids->typecode == GA_LONG};
+  err = lm_launch(k, t, 64, &a);
+  return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
+}
+
+static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const GpuArray *ids, const GpuArray *stats,
+                               const GpuArray *dlogp, const GpuArray *entropy, const GpuArray *dentropy, double scale,
+                               ssize_t ignore, int check_error) {
+  gpucontext *ctx = GpuArray_context(dlogits);
+  checker c(ctx, "token_logprobs_grad");
+  c.array(dlogits, "dlogits", 2);
+  c.array(logits, "logits", 2);
+  c.array(stats, "stats", 2);
+  if (c.err != GA_NO_ERROR) return c.err;
+  const size_t t = logits->dimensions[0], v = logits->dimensions[1];
+  c.shape(dlogits, "dlogits", t, v);
+  c.shape(stats, "stats", t, 2);
+  c.value_type(logits, "logits");
+  if (c.err == GA_NO_ERROR && dlogits->typecode != logits->typecode)
+    c.fail(GA_VALUE_ERROR, "must have the type of logits", "dlogits");
+  c.type(stats, "stats", GA_FLOAT);
+  c.rows(dlogits, "dlogits");
+  c.rows(logits, "logits");
+  c.result(dlogits, "dlogits");
+  if ((ids == nullptr) != (dlogp == nullptr)) return c.fail(GA_VALUE_ERROR, "ids and dlogp go together");
+  if ((entropy == nullptr) != (dentropy == nullptr)) return c.fail(GA_VALUE_ERROR, "entropy and dentropy go together");
+  const GpuArray *const vectors[4] = {ids, dlogp, entropy, dentropy};
+  const char *const names[4] = {"ids", "dlogp", "entropy", "dentropy"};
+  for (int i = 0; i < 4; i++) {
+    if (vectors[i] == nullptr) continue;
+    c.array(vectors[i], names[i], 1);
+    if (c.err != GA_NO_ERROR) return c.err;
+    c.shape(vectors[i], names[i], t);
+    if (i == 0) c.id_type(ids, names[i]);
+    else c.type(vectors[i], names[i], GA_FLOAT);
+    c.apart(dlogits, vectors[i], "dlogits");
+  }
+  c.apart(dlogits, stats, "dlogits");
+  if (c.err == GA_NO_ERROR && !same_place(dlogits, logits)) c.apart(dlogits, logits, "dlogits");
+  c.scale(scale, true);
+  if (c.err != GA_NO_ERROR) return c.err;
+  if (t == 0 || v == 0) return GA_NO_ERROR;
+  if (t > MAX_GROUPS || v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many rows or columns");
+  GpuKernel *k;
+  gpudata *errbuf = nullptr;
+  int err = lm_kernel(ctx, lm_variant(LM_LOGPROBS_GRAD, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT, 0),
+                      "lm_logprobs_grad_rows", sizeof(logprobs_grad_args), &k);
+  if (err == GA_NO_ERROR) err = lm_errbuf(ctx, logits, &errbuf);
+  if (err != GA_NO_ERROR) return err;
+  auto ptr = [](const GpuArray *x) -> void * { return x ? at(x) : nullptr; };
+  auto step = [](const GpuArray *x, unsigned i) -> int64_t { return x ? x->strides[i] : 0; };
+  logprobs_grad_args a = {at(dlogits), at(logits), ptr(ids), at(stats), ptr(dlogp), ptr(entropy), ptr(dentropy),
+                          errbuf->devptr, dlogits->strides[0], logits->strides[0], step(ids, 0), stats->strides[0],
+                          stats->strides[1], step(dlogp, 0), step(entropy, 0), step(dentropy, 0), (int64_t)t,
+                          (int64_t)v, ignore, (float)scale};
+  err = lm_launch(k, t, 256, &a);
+  return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
+}
+
+// ---- global norm -------------------------------------------------------------------
+
+// Norm of the n arrays `as` into `norm` (may be NULL) and, if rs is not NULL, their clipping into rs.
+static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double max_norm, GpuArray *norm, const char *who) {
+  if (n == 0 && norm == nullptr) return GA_NO_ERROR;
+  gpucontext *ctx = GpuArray_context(norm != nullptr ? norm : as[0]);
+  checker c(ctx, who);
+  if (norm != nullptr) {
+    if (norm->nd > 1 || (norm->nd == 1 && norm->dimensions[0] != 1))
+      return c.fail(GA_INVALID_ERROR, "must be 0-d or have one element", "norm");
+    if (norm->typecode != GA_FLOAT && norm->typecode != GA_DOUBLE)
+      return c.fail(GA_VALUE_ERROR, "must be float or double", "norm");
+    c.aligned(norm, "norm");
+    c.result(norm, "norm");
+  }
+  if (std::isnan(max_norm) || max_norm < 0) return c.fail(GA_VALUE_ERROR, "max_norm must be 0 or above");
+  if (c.err != GA_NO_ERROR) return c.err;
+  size_t pieces = 0;
+  std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
+  for (size_t i = 0; i < n; i++) {
+    const GpuArray *a = as[i];
+    if (GpuArray_context(a) != ctx) return c.fail(GA_INVALID_ERROR, "the arrays belong to different contexts");
+    if (!is_value(a->typecode) && a->typecode != GA_DOUBLE)
+      return c.fail(GA_UNSUPPORTED_ERROR, "arrays must be float, half, bfloat16 or double");
+    if (!GpuArray_ISONESEGMENT(a)) return c.fail(GA_INVALID_ERROR, "arrays must be contiguous");
+    c.aligned(a, "arrays");
+    if (c.err != GA_NO_ERROR) return c.err;
+    size_t count = 1;
+    for (unsigned j = 0; j < a->nd; j++) count *= a->dimensions[j];
+    pieces += (count + LM_PIECE - 1) / LM_PIECE;
+    if (norm != nullptr && overlap(norm, a)) return c.fail(GA_VALUE_ERROR, "overlaps an array", "norm");
+    if (rs == nullptr) continue;
+    const GpuArray *r = rs[i];
+    if (r != a && !same_place(r, a)) {
+      if (GpuArray_context(r) != ctx) return c.fail(GA_INVALID_ERROR, "the arrays belong to different contexts");
+      if (r->nd != a->nd || r->typecode != a->typecode)
+        return c.fail(GA_INVALID_ERROR, "a result differs from its array in shape or type");
+      for (unsigned j = 0; j < a->nd; j++)
+        if (r->dimensions[j] != a->dimensions[j] || (a->dimensions[j] > 1 && count > 0 && r->strides[j] != a->strides[j]))
+          return c.fail(GA_INVALID_ERROR, "a result differs from its array in shape or strides");
+      c.aligned(r, "results");
+      if (norm != nullptr) c.apart(norm, r, "norm");
+      uintptr_t lo, hi;
+      span_of(a, &lo, &hi);
+      if (lo < hi) read.emplace_back(lo, hi);
+    }
+    if (!GpuArray_ISWRITEABLE(r)) return c.fail(GA_VALUE_ERROR, "a result is not writeable");
+    if (c.err != GA_NO_ERROR) return c.err;
+    uintptr_t lo, hi;
+    span_of(r, &lo, &hi);
+    if (lo < hi) written.emplace_back(lo, hi);
+  }
+  if (rs != nullptr) {
+    // no two results overlap, and none overlaps an operand that is not itself
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); i++)
+      if (written[i].first < written[i - 1].second) return c.fail(GA_VALUE_ERROR, "results overlap");
+    for (auto &x : read) {
+      auto it = std::lower_bound(written.begin(), written.end(), std::make_pair(x.second, (uintptr_t)0));
+      if (it != written.begin() && (it - 1)->second > x.first)
+        return c.fail(GA_VALUE_ERROR, "a result overlaps another array");
+    }
+  }
+
+  char *scratch = nullptr;
+  GpuKernel *kpieces = nullptr, *kfinal = nullptr, *kclip = nullptr;
+  const lm_variant vn(LM_NORM, GA_FLOAT, GA_FLOAT, GA_INT, 0), vc(LM_CLIP, GA_FLOAT, GA_FLOAT, GA_INT, 0);
+  int err = lm_kernel(ctx, vn, "lm_norm_pieces", sizeof(tensors_args), &kpieces);
+  if (err == GA_NO_ERROR) err = lm_kernel(ctx, vn, "lm_norm_final", sizeof(tensors_args), &kfinal);
+  if (err == GA_NO_ERROR && rs != nullptr) err = lm_kernel(ctx, vc, "lm_clip_pieces", sizeof(tensors_args), &kclip);
+  if (err == GA_NO_ERROR) err = lm_scratch(ctx, 256 + pieces * sizeof(double), &scratch);
+  if (err != GA_NO_ERROR) return err;
+
+  tensors_args a;
+  memset(&a, 0, sizeof(a));
+  a.result = scratch;
+  a.partials = scratch + 256;
+  a.norm = norm ? at(norm) : nullptr;
+  a.norm_double = norm != nullptr && norm->typecode == GA_DOUBLE;
+  a.max_norm = max_norm;
+  a.npartials = (int64_t)pieces;
+  // the arrays in tables of up to LM_TENSORS, each with fewer than 2^31 pieces
+  auto for_tables = [&](auto &&launch) -> int {
+    size_t i = 0;
+    int64_t done = 0;
+    while (i < n) {
+      a.n = 0;
+      a.first[0] = 0;
+      for (; i < n && a.n < (int)LM_TENSORS; i++) {
+        const GpuArray *x = as[i];
+        int64_t count = 1;
+        for (unsigned j = 0; j < x->nd; j++) count *= (int64_t)x->dimensions[j];
+        const int64_t p = (count + LM_PIECE - 1) / LM_PIECE;
+        if (p == 0) continue;
+        if (a.first[a.n] + p > 0x7fffffff) {
+          if (a.n == 0) return c.fail(GA_XLARGE_ERROR, "an array is too large");
+          break;
+        }
+        a.in[a.n] = at(x);
+        a.out[a.n] = rs != nullptr ? at(rs[i]) : nullptr;
+        a.count[a.n] = count;
+        a.type[a.n] = x->typecode == GA_FLOAT ? 0 : x->typecode == GA_HALF ? 1 : x->typecode == GA_BFLOAT16 ? 2 : 3;
+        a.first[a.n + 1] = a.first[a.n] + (uint32_t)p;
+        a.n++;
+      }
+      if (a.n == 0) break;
+      a.partial0 = done;
+      int e = launch();
+      if (e != GA_NO_ERROR) return e;
+      done += a.first[a.n];
+    }
+    return GA_NO_ERROR;
+  };
+  err = for_tables([&] { return lm_launch(kpieces, a.first[a.n], 256, &a); });
+  if (err == GA_NO_ERROR) err = lm_launch(kfinal, 1, 256, &a);
+  if (err == GA_NO_ERROR && rs != nullptr) err = for_tables([&] { return lm_launch(kclip, a.first[a.n], 256, &a); });
+  return err;
+}
+
+// ---- the C entry points: nothing thrown leaves them ----------------------------------
+
+extern "C" {
+
+int GpuArray_embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, double scale, ssize_t ignore,
+                       int check_error) {
+  try {
+    return embedding(out, table, ids, scale, ignore, check_error);
+  } catch (const std::bad_alloc &) {
+    return no_memory(GpuArray_context(out));
+  }
+}
+
+int GpuArray_embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *ids, double scale, ssize_t ignore,
+                            int accumulate, int check_error) {
+  try {
+    return embedding_grad(grad, dout, ids, scale, ignore, accumulate, check_error);
+  } catch (const std::bad_alloc &) {
+    return no_memory(GpuArray_context(grad));
+  }
+}
+
+int GpuArray_token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, GpuArray *top_logp, GpuArray *top_ids,
+                            const GpuArray *logits, const GpuArray *ids, double scale, ssize_t ignore,
+                            int check_error) {
+  try {
+    return token_logprobs(logp, entropy, stats, top_logp, top_ids, logits, ids, scale, ignore, check_error);
+  } catch (const std::bad_alloc &) {
+    return no_memory(GpuArray_context(logits));
+  }
+}
+
+int GpuArray_token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const GpuArray *ids, const GpuArray *stats,
+                                 const GpuArray *dlogp, const GpuArray *entropy, const GpuArray *dentropy,
+                                 double scale, ssize_t ignore, int check_error) {
+  try {
+    return token_logprobs_grad(dlogits, logits, ids, stats, dlogp, entropy, dentropy, scale, ignore, check_error);
+  } catch (const std::bad_alloc &) {
+    return no_memory(GpuArray_context(logits));
+  }
+}
+
+int GpuArray_global_norm(GpuArray *norm, const GpuArray **as, size_t n) {
+  try {
+    return norm_and_clip(nullptr, as, n, 0.0, norm, "global_norm");
+  } catch (const std::bad_alloc &) {
+    return no_memory(GpuArray_context(norm));
+  }
+}
+
+int GpuArray_clip_global_norm(GpuArray **rs, const GpuArray **as, size_t n, double max_norm, GpuArray *norm) {
+  try {
+    return norm_and_clip(rs != nullptr ? rs : (GpuArray **)as, as, n, max_norm, norm, "clip_global_norm");
+  } catch (const std::bad_alloc &) {
+    return n != 0 ? no_memory(GpuArray_context(as[0])) : GA_MEMORY_ERROR;
+  }
+}
+
+}  // extern "C"

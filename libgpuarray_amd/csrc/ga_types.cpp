@@ -20,6 +20,7 @@ struct cd16 { double r, i; };             // complex double
 struct cq32 { q16 r, i; };                // complex quad
 
 const gpuarray_type k_none = {nullptr, 0, 0, -1};
+const gpuarray_type k_bfloat16 = {"ga_bfloat16", 2, ALIGN_OF(uint16_t), GA_BFLOAT16};
 const gpuarray_type k_buffer = {nullptr, sizeof(GpuArray *), ALIGN_OF(GpuArray *),
                                 GA_BUFFER};
 
@@ -104,6 +105,7 @@ extern "C" const gpuarray_type *gpuarray_get_type(int typecode) {
   if (typecode < GA_NBASE) return &k_scalar[typecode];
   if (typecode < 256) return &k_none;
   if (typecode < GA_NVEC) return &vectors().rows[typecode - 256];
+  if (typecode == GA_BFLOAT16) return &k_bfloat16;
   if (typecode < GA_ENDVEC) return &k_none;
   std::lock_guard<std::mutex> lk(g_custom_mu);
   size_t i = (size_t)(typecode - GA_ENDVEC);

@@ -20,6 +20,7 @@
 #include <gpuarray/error.h>
 #include <gpuarray/extension.h>
 #include <gpuarray/kernel.h>
+#include <gpuarray/language.h>
 #include <gpuarray/reduction.h>
 #include <gpuarray/types.h>
 #include <gpuarray/util.h>
@@ -135,11 +136,14 @@ int GpuArray_is_aligned(const GpuArray *a);
 extern const char ga_device_rt_src[];
 extern const char ga_cluda_hip_src[];
 extern const char ga_reduce_kernels_src[];
+extern const char ga_language_kernels_src[];
 
 // Grow-only scratch buffer owned by the context (partials of two-pass
 // reductions).  Work on a context is in stream order, so one buffer is
 // shared by consecutive calls.
 gpudata *ga_hip_scratch(gpucontext *ctx, size_t bytes);
+// Its present size: a request up to that allocates nothing.
+size_t ga_hip_scratch_size(gpucontext *ctx);
 // Counters of split reductions that finish in one launch: a buffer of
 // ga_hip_redux_counters_max 32-bit zeros, made on first use; every kernel
 // that counts on it leaves it zeroed.  NULL (error set) when it cannot be made.
@@ -176,6 +180,9 @@ void **ga_hip_redux_cache_slot(gpucontext *ctx);
 // Frees the per-context kernels of GpuArray_take1 (array.cpp).
 void ga_take1_cache_free(gpucontext *ctx);
 void **ga_hip_take1_cache_slot(gpucontext *ctx);
+// Frees the per-context kernels of the operators in gpuarray/language.h (ga_language.cpp).
+void ga_language_cache_free(gpucontext *ctx);
+void **ga_hip_language_cache_slot(gpucontext *ctx);
 
 // Typecode of the opaque by-value "plan" kernel argument of `bytes` bytes
 // (registered on first use through gpuarray_register_type).

@@ -8,6 +8,23 @@ _CTYPES = {"bool": "ga_bool", "int8": "ga_byte", "uint8": "ga_ubyte", "int16": "
            "float64": "ga_double", "complex64": "ga_cfloat", "complex128": "ga_cdouble"}
 
 
+# NumPy has no bfloat16: on the host such elements are records of their 16 bits.
+bfloat16 = np.dtype([("bfloat16", "<u2")])
+
+
+def to_bfloat16(a):
+    """Host array of bfloat16 records, rounded to nearest even from float32."""
+    bits = np.asarray(a, dtype=np.float32).view(np.uint32)
+    half = (bits + (0x7fff + ((bits >> 16) & 1))) >> 16
+    nan = (bits & 0x7fffffff) > 0x7f800000
+    return np.where(nan, (bits >> 16) | 0x40, half).astype(np.uint16).view(bfloat16)
+
+
+def from_bfloat16(a):
+    """float32 values of a host array of bfloat16 records."""
+    return (np.ascontiguousarray(a).view(np.uint16).astype(np.uint32) << 16).view(np.float32)
+
+
 _REGISTERED = {}     # dtype -> C name, for element types added with register_dtype
 _BY_DTYPE = {}       # dtype object -> C name of a built-in type (dtype.name is slow to form)
 NAME_TO_DTYPE = {}   # C spelling -> dtype, for parsing C argument lists
@@ -24,6 +41,8 @@ def dtype_to_ctype(dtype):
     dtype = np.dtype(dtype)
     if dtype in _REGISTERED:
         return _REGISTERED[dtype]
+    if dtype == bfloat16:
+        return "ga_bfloat16"
     try:
         res = _BY_DTYPE[dtype] = _CTYPES[dtype.name]
         return res

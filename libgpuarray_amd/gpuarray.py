@@ -13,6 +13,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import lib, check, GpuArrayException, UnsupportedException, GpuArrayStruct, c_ssize_t
+from .dtypes import bfloat16
 from .dtypes import dtype_to_ctype  # noqa: F401  (part of this module's interface, as in the reference)
 
 # numpy dtype.num equals the typecode on LP64 Linux
@@ -25,6 +26,7 @@ _TYPECODES = {
     np.dtype("uint64"): _lib.GA_ULONG, np.dtype("float32"): _lib.GA_FLOAT,
     np.dtype("float64"): _lib.GA_DOUBLE, np.dtype("float16"): _lib.GA_HALF,
     np.dtype("complex64"): _lib.GA_CFLOAT, np.dtype("complex128"): _lib.GA_CDOUBLE,
+    bfloat16: _lib.GA_BFLOAT16,
 }
 _DTYPES = {v: k for k, v in _TYPECODES.items()}
 

@@ -1,0 +1,36 @@
+"""The refusals of the language operators where there is no device, against the
+stand-in runtime and the three builds of the library; and their kernel texts,
+which must compile for gfx950 for every combination of types."""
+import ctypes as C
+import subprocess
+import sys
+
+import pytest
+
+from test_host_logic_without_device import ROOT, build, mock_runtime  # noqa: F401  (fixtures)
+
+HOST_ONLY = ["tests/test_gpu_language.py::test_refusals",
+             "tests/test_gpu_language.py::test_refusal_of_arrays_of_two_contexts"]
+
+
+def test_refusals_without_a_device(build):  # noqa: F811
+    variant, env = build
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-m", "gpu", "-p", "no:cacheprovider", "--timeout", "300"]
+                       + HOST_ONLY, cwd=ROOT, env=env, capture_output=True, text=True, timeout=900)
+    assert r.returncode == 0, r.stdout[-4000:] + r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("x", [11, 23, 511])
+@pytest.mark.parametrize("o", [11, 23, 511])
+def test_kernel_texts_compile(x, o):
+    from libgpuarray_amd import _lib
+    source = _lib.extension("hip_language_source", C.c_void_p, [C.c_ulonglong])
+    compile_only = _lib.extension("hip_compile_only", C.c_int, [C.c_uint, C.POINTER(C.c_char_p), C.POINTER(C.c_size_t),
+                                                                C.POINTER(C.c_char_p)])
+    for kind in range(6):
+        if kind > 1 and o != 11:
+            continue
+        for ids in (5, 8):
+            text = C.string_at(source(kind | x << 8 | o << 20 | ids << 32))
+            log = C.c_char_p()
+            assert compile_only(1, (C.c_char_p * 1)(text), None, C.byref(log)) == 0, (log.value or b"").decode()[-2000:]
