@@ -87,7 +87,8 @@ GPUARRAY_PUBLIC int GpuArray_embedding_grad(GpuArray *grad,
  *   Logits of -inf have probability 0.  In a row with nothing but -inf every log probability and
  * the second statistic are -inf, the entropy is 0 and the alternatives are
  * ids 0 to k - 1.  In a row with a NaN or a +inf every value is NaN (the first
- * statistic is the largest number) and the alternatives are ids 0 to k - 1. */
+ * statistic is the largest number, or NaN if a NaN is a signaling one) and the
+ * alternatives are ids 0 to k - 1. */
 GPUARRAY_PUBLIC int GpuArray_token_logprobs(GpuArray *logp, GpuArray *entropy,
                                             GpuArray *stats,
                                             GpuArray *top_logp,

@@ -259,6 +259,11 @@ def main():
             check("language operator %d types %d, %d" % (kind, x, o),
                   gen_l(kind | x << 8 | o << 20 | (GA_LONG if o == GA_FLOAT else GA_INT) << 32))
             lm += 1
+    # log probabilities: lanes of a row / 64, 32: entropy, 64: alternatives, 128: rows in pieces
+    for x, extra in [(GA_FLOAT, 1), (GA_FLOAT, 1 | 32 | 64), (GA_BFLOAT16, 4 | 32), (GA_BFLOAT16, 4 | 64 | 128),
+                     (GA_HALF, 16 | 32 | 64), (GA_HALF, 8)]:
+        check("log probabilities, type %d, variant %d" % (x, extra), gen_l(2 | x << 8 | GA_FLOAT << 20 | GA_LONG << 32 | extra << 44))
+        lm += 1
     print("device sources compile for gfx950 (%d reduction variants, %d map-reduce, %d take1, "
           "50 elementwise, %d of language operators)" % (n + 20, m, t, lm))
 

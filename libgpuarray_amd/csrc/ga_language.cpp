@@ -55,12 +55,19 @@ struct logprobs_args {
   const void *logits, *ids;
   void *logp, *entropy, *stats, *top_logp, *top_ids;
   void *err;
+  void *partials;
   int64_t row, id_step, logp_step, entropy_step, stats_row, stats_col;
   int64_t topl_row, topl_col, topi_row, topi_col;
   int64_t t, v, ignore;
-  float scale;
+  float scale, by;
   int32_t top, top_long;
+  uint32_t pieces, piece_chunks, partial_bytes;
 };
+// What the variant of the log probability kernels is specialised on: the lanes
+// of a row, the entropy, the alternatives, rows in pieces.
+inline unsigned logprobs_extra(unsigned lanes, bool entropy, bool top, bool split) {
+  return lanes / 64 | (entropy ? 32u : 0) | (top ? 64u : 0) | (split ? 128u : 0);
+}
 struct logprobs_grad_args {
   void *out;
   const void *logits, *ids, *stats, *dlogp, *entropy, *dentropy;
@@ -91,6 +98,11 @@ std::string lm_source(const lm_variant &v) {
   name("LM_X", v.x);
   name("LM_O", v.o);
   name("LM_ID", v.id);
+  if (v.kind == LM_LOGPROBS) {
+    s += "#define LM_LANES " + std::to_string((v.extra & 31 ? v.extra & 31 : 1) * 64) + "\n";
+    s += std::string("#define LM_ENT ") + (v.extra & 32 ? "1" : "0") + "\n#define LM_TOP " + (v.extra & 64 ? "1" : "0") +
+         "\n#define LM_SPLIT " + (v.extra & 128 ? "1" : "0") + "\n";
+  }
   return s + ga_language_kernels_src;
 }
 
@@ -404,20 +416,51 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
   if (t == 0 || (logp == nullptr && entropy == nullptr && stats == nullptr && top == 0)) return GA_NO_ERROR;
   if (v == 0) return c.fail(GA_VALUE_ERROR, "empty vocabulary");
   if (t > MAX_GROUPS || v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many rows or columns");
-  GpuKernel *k;
+  // A row that a wavefront covers in two rounds of loads belongs to one
+  // wavefront, longer ones to a group, which grows while there are too few
+  // rows to fill the chip; below that, rows are cut in pieces of at least two
+  // chunks per lane and joined by a second launch.
+  const size_t row_chunks = v * gpuarray_get_elsize(logits->typecode) / 16 + 1;
+  const size_t cus = ga_hip_numprocs(ctx) ? ga_hip_numprocs(ctx) : 256;
+  unsigned lanes = 64;
+  if (row_chunks > 512) {
+    lanes = 256;
+    while (lanes < 1024 && t * lanes < cus * 1024 && row_chunks > 8 * lanes) lanes *= 2;
+  }
+  size_t pieces = 1, piece_chunks = row_chunks;
+  if (row_chunks > 512 && t * 2 <= cus) {
+    lanes = 256;
+    pieces = std::min((2 * cus + t - 1) / t, (row_chunks + 511) / 512);
+    piece_chunks = (row_chunks + pieces - 1) / pieces;
+    pieces = (row_chunks + piece_chunks - 1) / piece_chunks;
+  }
+  const bool split = pieces > 1;
+  const size_t partial_bytes = 16 + 8 * top;
+  const lm_variant var(LM_LOGPROBS, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT,
+                       logprobs_extra(lanes, entropy != nullptr, top != 0, split));
+  GpuKernel *k, *kjoin = nullptr;
   gpudata *errbuf = nullptr;
-  int err = lm_kernel(ctx, lm_variant(LM_LOGPROBS, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT, 0),
-                      "lm_logprobs_rows", sizeof(logprobs_args), &k);
+  char *scratch = nullptr;
+  int err = lm_kernel(ctx, var, "lm_logprobs_rows", sizeof(logprobs_args), &k);
+  if (err == GA_NO_ERROR && split) err = lm_kernel(ctx, var, "lm_logprobs_join", sizeof(logprobs_args), &kjoin);
+  if (err == GA_NO_ERROR && split) err = lm_scratch(ctx, t * pieces * partial_bytes, &scratch);
   if (err == GA_NO_ERROR) err = lm_errbuf(ctx, logits, &errbuf);
   if (err != GA_NO_ERROR) return err;
   auto ptr = [](const GpuArray *x) -> void * { return x ? at(x) : nullptr; };
   auto step = [](const GpuArray *x, unsigned i) -> int64_t { return x ? x->strides[i] : 0; };
   logprobs_args a = {at(logits), ptr(ids), ptr(logp), ptr(entropy), ptr(stats), ptr(top_logp), ptr(top_ids),
-                     errbuf->devptr, logits->strides[0], step(ids, 0), step(logp, 0), step(entropy, 0), step(stats, 0),
-                     step(stats, 1), step(top_logp, 0), step(top_logp, 1), step(top_ids, 0), step(top_ids, 1),
-                     (int64_t)t, (int64_t)v, ignore, (float)scale, (int32_t)top,
-                     top_ids != nullptr && top_ids->typecode == GA_LONG};
-  err = lm_launch(k, t, 64, &a);
+                     errbuf->devptr, scratch, logits->strides[0], step(ids, 0), step(logp, 0), step(entropy, 0),
+                     step(stats, 0), step(stats, 1), step(top_logp, 0), step(top_logp, 1), step(top_ids, 0),
+                     step(top_ids, 1), (int64_t)t, (int64_t)v, ignore, (float)scale,
+                     (float)((double)(float)scale * 1.4426950408889634), (int32_t)top,
+                     top_ids != nullptr && top_ids->typecode == GA_LONG, (uint32_t)pieces, (uint32_t)piece_chunks,
+                     (uint32_t)partial_bytes};
+  if (split) {
+    err = lm_launch(k, t * pieces, lanes, &a);
+    if (err == GA_NO_ERROR) err = lm_launch(kjoin, t, lanes, &a);
+  } else {
+    err = lanes < 256 ? lm_launch(k, (t + 3) / 4, 256, &a) : lm_launch(k, t, lanes, &a);
+  }
   return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
 }
 

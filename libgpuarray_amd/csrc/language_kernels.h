@@ -44,16 +44,53 @@ LM_FN ga_long lm_id(ga_long id, ga_long ignore, ga_long none, ga_long v) {
 /* the value of ignore that no id is compared with */
 #define LM_NONE ((ga_long)1 << 63)
 
-LM_FN float lm_wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((int)(((LID_0 & 63) ^ d) << 2), __builtin_bit_cast(int, v)));
-  return v;
+/* The value of lane ^ MASK: through the data-parallel moves where one of them
+ * is that exchange, else through the LDS crossbar. */
+template <int MASK> LM_FN ga_uint lm_xor(ga_uint v) {
+  if constexpr (MASK == 1) return (ga_uint)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);
+  else if constexpr (MASK == 2) return (ga_uint)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true);
+  else if constexpr (MASK == 3) return (ga_uint)__builtin_amdgcn_update_dpp(0, (int)v, 0x1B, 0xF, 0xF, true);
+  else if constexpr (MASK == 7) return (ga_uint)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true);
+  else if constexpr (MASK == 8) return (ga_uint)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, true);
+  else if constexpr (MASK == 15) return (ga_uint)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true);
+  else if constexpr (MASK < 32) return (ga_uint)__builtin_amdgcn_ds_swizzle((int)v, (MASK << 10) | 0x1F);
+  else return (ga_uint)__builtin_amdgcn_ds_bpermute((int)(((LID_0 & 63) ^ MASK) << 2), (int)v);
 }
-LM_FN float lm_wave_max(float v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = __builtin_fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((int)(((LID_0 & 63) ^ d) << 2), __builtin_bit_cast(int, v))));
-  return v;
+template <int MASK> LM_FN float lm_xor(float v) {
+  return __builtin_bit_cast(float, lm_xor<MASK>(__builtin_bit_cast(ga_uint, v)));
 }
+template <int MASK> LM_FN ga_ulong lm_xor(ga_ulong v) {
+  return (ga_ulong)lm_xor<MASK>((ga_uint)(v >> 32)) << 32 | lm_xor<MASK>((ga_uint)v);
+}
+
+/* ---- 16-byte chunks of a row -------------------------------------------------- */
+typedef ga_uint lm_u4 __attribute__((ext_vector_type(4)));
+#define LM_E (16 / (int)sizeof(LM_X))   /* elements of a chunk */
+
+LM_FN void lm_unpack(const lm_u4 &q, float *y, ga_float) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const ga_uint word = q[e];   /* (a bit cast of the vector's element itself gives the first one) */
+    y[e] = __builtin_bit_cast(float, word);
+  }
+}
+LM_FN void lm_unpack(const lm_u4 &q, float *y, ga_half) {
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  const h8 h = __builtin_bit_cast(h8, q);
+#pragma unroll
+  for (int e = 0; e < 8; e++) y[e] = (float)h[e];
+}
+LM_FN void lm_unpack(const lm_u4 &q, float *y, ga_bfloat16) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    y[2 * e] = __builtin_bit_cast(float, q[e] << 16);
+    y[2 * e + 1] = __builtin_bit_cast(float, q[e] & 0xffff0000u);
+  }
+}
+/* a word of -inf elements */
+LM_FN ga_uint lm_minus_inf(ga_float) { return 0xff800000u; }
+LM_FN ga_uint lm_minus_inf(ga_half) { return 0xfc00fc00u; }
+LM_FN ga_uint lm_minus_inf(ga_bfloat16) { return 0xff80ff80u; }
 
 #if LM_KIND == LM_K_EMBED
 struct lm_embed {
@@ -136,91 +173,381 @@ struct lm_logprobs {
   GLOBAL_MEM float *logp, *entropy, *stats, *top_logp;   /* NULL: not wanted */
   GLOBAL_MEM void *top_ids;
   GLOBAL_MEM ga_int *err;
+  GLOBAL_MEM char *partials;     /* of rows in pieces: lm_state, then the alternatives' keys */
   ga_long row, id_step, logp_step, entropy_step, stats_row, stats_col;
   ga_long topl_row, topl_col, topi_row, topi_col;
   ga_long t, v, ignore;
-  float scale;
+  float scale, by;               /* by = scale * log2(e) */
   ga_int top, top_long;
+  ga_uint pieces, piece_chunks, partial_bytes;
 };
 
-/* what is written for row r, from its statistics; one lane */
-LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, float m, float ls, float entropy) {
-  if (p.ids != nullptr) {
-    const ga_long id = lm_id((ga_long)*lm_at(p.ids, r * p.id_step), p.ignore, LM_NONE, p.v);
-    float lp = 0.0f;
-    if (id == -2) {
-      *p.err = -1;
-      lp = NAN;
-    } else if (id >= 0) {
-      lp = ls == -INFINITY ? -INFINITY : (lm_get(lm_at(p.logits, r * p.row)[id]) - m) * p.scale - ls;
-      if (ls != ls) lp = NAN;
-    }
-    *lm_at(p.logp, r * p.logp_step) = lp;
-  }
-  if (p.entropy != nullptr) *lm_at(p.entropy, r * p.entropy_step) = ls == -INFINITY ? 0.0f : entropy;
-  if (p.stats != nullptr) {
-    *lm_at(p.stats, r * p.stats_row) = m;
-    *lm_at(p.stats, r * p.stats_row + p.stats_col) = ls;
-  }
+/* Softmax statistics of some elements x of a row.  With R(m) = by * m, rounded,
+ *   s = sum of 2^(by * x - R(m)),   w = sum of (by * x - R(m)) 2^(by * x - R(m)),
+ * where m is the largest x; R(m) being a number that is known exactly, its
+ * rounding is no error of s or w.  One multiply-add and one exponential per
+ * element.  -inf has no part in either sum.  Where |R| is past 1e30 the
+ * difference between neighbouring values is past 1e22, so that s counts the
+ * elements that are equal to m and w is 0: rows of a type's lowest value. */
+struct lm_state {
+  float m, s, w, pad;
+};
+#define LM_LOWEST (-3.402823466e+38f)
+#define LM_FAR 1e30f
+
+/* R(from) - R(to), from <= to; far below, and where either is far out, -300, which
+ * is as good as -inf for the exponential and safe to multiply with 0 */
+LM_FN float lm_shift(float from, float to, float by) {
+  const float d = __builtin_fmaxf(from * by - to * by, -300.0f);
+  return from == to ? 0.0f : d;
 }
-LM_FN void lm_put_top(const lm_logprobs &p, ga_long r, ga_int k, float lp, ga_long id) {
-  *lm_at(p.top_logp, r * p.topl_row + k * p.topl_col) = lp;
-  const ga_long at = r * p.topi_row + k * p.topi_col;
-  if (p.top_long) *lm_at((GLOBAL_MEM ga_long *)p.top_ids, at) = id;
-  else *lm_at((GLOBAL_MEM ga_int *)p.top_ids, at) = (ga_int)id;
+LM_FN void lm_rescale(lm_state &a, float m, float by) {
+  const float d = lm_shift(a.m, m, by), f = __builtin_amdgcn_exp2f(d);
+#if LM_ENT
+  a.w = f * __builtin_fmaf(a.s, d, a.w);
+#endif
+  a.s *= f;
+  a.m = m;
+}
+LM_FN void lm_join(lm_state &a, lm_state b, float by) {
+  const float m = __builtin_fmaxf(a.m, b.m);
+  lm_rescale(a, m, by);
+  lm_rescale(b, m, by);
+  a.s += b.s;
+  a.w += b.w;
+}
+template <int MASK> LM_FN void lm_join_xor(lm_state &a, float by) {
+  lm_state b;
+  b.m = lm_xor<MASK>(a.m);
+  b.s = lm_xor<MASK>(a.s);
+  b.w = LM_ENT ? lm_xor<MASK>(a.w) : 0.0f;
+  lm_join(a, b, by);
+}
+LM_FN void lm_join_wave(lm_state &a, float by) {
+  lm_join_xor<1>(a, by);
+  lm_join_xor<2>(a, by);
+  lm_join_xor<7>(a, by);
+  lm_join_xor<15>(a, by);
+  lm_join_xor<16>(a, by);
+  lm_join_xor<32>(a, by);
+}
+LM_FN float lm_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+/* the largest of y[0..N) and a */
+template <int N> LM_FN float lm_max_of(const float (&y)[N], float a) {
+#pragma unroll
+  for (int i = 0; i + 1 < N; i += 2) a = lm_max3(a, y[i], y[i + 1]);
+  if (N & 1) a = __builtin_fmaxf(a, y[N - 1]);
+  return a;
 }
 
-/* One wavefront per row, in passes: the maximum; the sums; then one pass for
- * each alternative, the largest value after the one before it. */
-KERNEL void __launch_bounds__(64) lm_logprobs_rows(const lm_logprobs p) {
-  const ga_long r = GID_0;
-  const ga_uint lane = LID_0;
-  GLOBAL_MEM const LM_X *x = lm_at(p.logits, r * p.row);
-  float m = -INFINITY;
-  for (ga_long c = lane; c < p.v; c += 64) m = __builtin_fmaxf(m, lm_get(x[c]));
-  m = lm_wave_max(m);
-  const float m0 = m == -INFINITY ? 0.0f : m;
-  float s = 0.0f, w = 0.0f;
-  for (ga_long c = lane; c < p.v; c += 64) {
-    const float z = (lm_get(x[c]) - m0) * p.scale, e = __builtin_expf(z);
-    s += e;
-    w += e * __builtin_fmaxf(z, -1000.0f);
-  }
-  s = lm_wave_sum(s);
-  w = lm_wave_sum(w);
-  const float ls = __builtin_logf(s);
-  if (lane == 0) lm_logprobs_finish(p, r, m, ls, ls - w / s);
-  float lv = INFINITY;
-  ga_int li = -1;
-  for (ga_int k = 0; k < p.top; k++) {
-    if (ls != ls) {
-      if (lane == 0) lm_put_top(p, r, k, NAN, k);
-      continue;
-    }
-    float bv = -INFINITY;
-    ga_int bi = 0x7fffffff;
-    for (ga_int c = lane; c < p.v; c += 64) {
-      const float y = lm_get(x[c]);
-      if ((y < lv || (y == lv && c > li)) && (y > bv || bi == 0x7fffffff)) {
-        bv = y;
-        bi = c;
-      }
-    }
+/* N elements of every lane join its statistics. */
+template <int N> LM_FN void lm_add(lm_state &a, const float (&y)[N], float most, float by) {
+  lm_rescale(a, __builtin_fmaxf(a.m, most), by);
+  const float r = a.m * by;
+  const bool far = !(__builtin_fabsf(r) <= LM_FAR);
+  float s[2] = {0.0f, 0.0f}, w[2] = {0.0f, 0.0f};
+  if (__builtin_amdgcn_ballot_w64(far) == 0) {
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      const int from = (int)((lane ^ d) << 2);
-      const float ov = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from, __builtin_bit_cast(int, bv)));
-      const ga_int oi = __builtin_amdgcn_ds_bpermute(from, bi);
-      if (ov > bv || (ov == bv && oi < bi)) {
-        bv = ov;
-        bi = oi;
+    for (int i = 0; i < N; i++) {
+      const float t = __builtin_fmaf(y[i], by, -r), e = __builtin_amdgcn_exp2f(t);
+      s[i & 1] += e;
+#if LM_ENT
+      w[i & 1] = __builtin_fmaf(e, t, w[i & 1]);
+#endif
+    }
+#if LM_ENT
+    /* 0 * -inf: some element is -inf.  Once more, with products that stay finite. */
+    if (__builtin_amdgcn_ballot_w64(w[0] + w[1] != w[0] + w[1]) != 0) {
+      w[0] = w[1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const float t = __builtin_fmaf(y[i], by, -r), e = __builtin_amdgcn_exp2f(t);
+        w[i & 1] = __builtin_fmaf(e, __builtin_fmaxf(t, -300.0f), w[i & 1]);
       }
     }
-    if (lane == 0) lm_put_top(p, r, k, ls == -INFINITY ? -INFINITY : (bv - m) * p.scale - ls, bi);
-    lv = bv;
-    li = bi;
+#endif
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float t = far ? 0.0f : __builtin_fmaf(y[i], by, -r);
+      float e = __builtin_amdgcn_exp2f(t);
+      if (far) e = y[i] == a.m ? 1.0f : (y[i] != y[i] ? y[i] : 0.0f);
+      s[i & 1] += e;
+      w[i & 1] = __builtin_fmaf(e, __builtin_fmaxf(t, -300.0f), w[i & 1]);
+    }
+  }
+  a.s += s[0] + s[1];
+#if LM_ENT
+  a.w += w[0] + w[1];
+#endif
+}
+
+/* ---- the alternatives -----------------------------------------------------------
+ * A wavefront keeps its best 64 elements as keys, sorted, one per lane: the
+ * upper half orders the values (-0 as 0), the lower one prefers low indices;
+ * 0 is no element.  -inf is never kept: what is missing in the end is filled
+ * up by a look at the row. */
+LM_FN ga_ulong lm_key(float y, ga_uint index) {
+  const ga_uint b = __builtin_bit_cast(ga_uint, y + 0.0f);
+  return (ga_ulong)(b ^ ((ga_uint)((ga_int)b >> 31) | 0x80000000u)) << 32 | (0xffffffffu - index);
+}
+LM_FN float lm_key_value(ga_ulong k) {
+  const ga_uint b = (ga_uint)(k >> 32);
+  return __builtin_bit_cast(float, b ^ ((b & 0x80000000u) ? 0x80000000u : 0xffffffffu));
+}
+LM_FN ga_uint lm_key_index(ga_ulong k) { return 0xffffffffu - (ga_uint)k; }
+
+/* one step of a sorting network: of lane and lane ^ MASK the lower one keeps the larger key */
+template <int MASK> LM_FN void lm_step(ga_ulong &k) {
+  const ga_ulong other = lm_xor<MASK>(k);
+  const ga_uint top_bit = 1u << (31 - __builtin_clz(MASK));
+  const bool lower = (LID_0 & top_bit) == 0;
+  k = (k > other) == lower ? k : other;
+}
+LM_FN void lm_sort(ga_ulong &k) {   /* descending over the 64 lanes */
+  lm_step<1>(k);
+  lm_step<3>(k); lm_step<1>(k);
+  lm_step<7>(k); lm_step<2>(k); lm_step<1>(k);
+  lm_step<15>(k); lm_step<4>(k); lm_step<2>(k); lm_step<1>(k);
+  lm_step<31>(k); lm_step<8>(k); lm_step<4>(k); lm_step<2>(k); lm_step<1>(k);
+  lm_step<63>(k); lm_step<16>(k); lm_step<8>(k); lm_step<4>(k); lm_step<2>(k); lm_step<1>(k);
+}
+/* list := the best 64 of two sorted lists, sorted */
+LM_FN void lm_merge(ga_ulong &list, ga_ulong other) {
+  const ga_ulong r = lm_xor<63>(other);
+  list = list > r ? list : r;
+  lm_step<32>(list); lm_step<16>(list); lm_step<8>(list); lm_step<4>(list); lm_step<2>(list); lm_step<1>(list);
+}
+LM_FN ga_ulong lm_lane(ga_ulong k, int lane) {
+  return (ga_ulong)(ga_uint)__builtin_amdgcn_readlane((int)(ga_uint)(k >> 32), lane) << 32 |
+         (ga_uint)__builtin_amdgcn_readlane((int)(ga_uint)k, lane);
+}
+
+/* The N elements of every lane against the list, whose k-th key is the bar: in
+ * rounds, each lane offers its best element that passes the bar, until none
+ * does.  Element i of a lane has the index at + (i / LM_E) * step + i % LM_E. */
+template <int N> LM_FN void lm_offer(ga_ulong &list, float (&y)[N], float most, ga_int top, ga_uint at, ga_uint step) {
+  ga_ulong bar = lm_lane(list, top - 1);
+  float bar_y = bar ? lm_key_value(bar) : -INFINITY;
+  if (__builtin_amdgcn_ballot_w64(most > bar_y || (most == bar_y && at < lm_key_index(bar) && bar)) == 0) return;
+  for (;;) {
+    int best = 0;
+#pragma unroll
+    for (int i = N - 1; i > 0; i--) best = y[i] == most ? i : best;
+    if (y[0] == most) best = 0;
+    const ga_ulong mine = most > -INFINITY ? lm_key(most, at + (ga_uint)(best / LM_E) * step + (ga_uint)(best % LM_E)) : 0;
+    const bool offers = mine > bar;
+    if (__builtin_amdgcn_ballot_w64(offers) == 0) return;
+    ga_ulong k = offers ? mine : 0;
+    lm_sort(k);
+    lm_merge(list, k);
+    bar = lm_lane(list, top - 1);
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = offers && i == best ? -INFINITY : y[i];
+    most = lm_max_of(y, -INFINITY);
   }
 }
+
+/* What is written for row r; a whole wavefront. */
+LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a, ga_ulong list) {
+  const ga_uint lane = LID_0 & 63;
+  const float rm = a.m * p.by;
+  const bool nothing = a.s == 0.0f;
+  const float s = a.m == INFINITY ? NAN : a.s;
+  const float m = nothing ? -INFINITY : a.m;
+  const float lg = __builtin_logf(s);
+  /* R(m) is off by * m by a rounding; past LM_FAR the sum is relative to m itself */
+  const float off = __builtin_fabsf(rm) <= LM_FAR ? __builtin_fmaf(a.m, p.by, -rm) * 0.6931471805599453f : 0.0f;
+  const float ls = nothing ? -INFINITY : lg - off;
+  if (lane == 0) {
+    if (p.ids != nullptr) {
+      const ga_long id = lm_id((ga_long)*lm_at(p.ids, r * p.id_step), p.ignore, LM_NONE, p.v);
+      float lp = 0.0f;
+      if (id == -2) {
+        *p.err = -1;
+        lp = NAN;
+      } else if (id >= 0) {
+        lp = nothing ? -INFINITY : (lm_get(lm_at(p.logits, r * p.row)[id]) - m) * p.scale - ls;
+        if (ls != ls) lp = NAN;
+      }
+      *lm_at(p.logp, r * p.logp_step) = lp;
+    }
+#if LM_ENT
+    if (p.entropy != nullptr)
+      *lm_at(p.entropy, r * p.entropy_step) = nothing ? 0.0f : lg - 0.6931471805599453f * (a.w / s);
+#endif
+    if (p.stats != nullptr) {
+      *lm_at(p.stats, r * p.stats_row) = m;
+      *lm_at(p.stats, r * p.stats_row + p.stats_col) = ls;
+    }
+  }
+#if LM_TOP
+  const ga_ulong got = __builtin_amdgcn_ballot_w64(list != 0 && lane < p.top);
+  ga_uint n = (ga_uint)__builtin_popcountll(got);
+  const auto put = [&](ga_uint k, float lp, ga_uint id) {
+    *lm_at(p.top_logp, r * p.topl_row + k * p.topl_col) = lp;
+    const ga_long at = r * p.topi_row + k * p.topi_col;
+    if (p.top_long) *lm_at((GLOBAL_MEM ga_long *)p.top_ids, at) = id;
+    else *lm_at((GLOBAL_MEM ga_int *)p.top_ids, at) = (ga_int)id;
+  };
+  if (ls != ls) {
+    if (lane < p.top) put(lane, NAN, lane);
+    return;
+  }
+  if (lane < n) put(lane, (lm_key_value(list) - m) * p.scale - ls, lm_key_index(list));
+  /* fewer than `top` elements above -inf: the lowest indices of -inf follow.
+   * They are among the first 2 * 64 elements, or the row is shorter. */
+  for (ga_long base = 0; n < p.top && base < p.v; base += 64) {
+    const ga_long c = base + lane;
+    const bool is = c < p.v && lm_get(lm_at(p.logits, r * p.row)[c]) == -INFINITY;
+    const ga_ulong hits = __builtin_amdgcn_ballot_w64(is);
+    const ga_uint k = n + __builtin_amdgcn_mbcnt_hi((ga_uint)(hits >> 32), __builtin_amdgcn_mbcnt_lo((ga_uint)hits, 0));
+    if (is && k < p.top) put(k, -INFINITY, (ga_uint)c);
+    n += (ga_uint)__builtin_popcountll(hits);
+  }
+#endif
+}
+
+/* The statistics and lists of a group's wavefronts meet in the first one. */
+#define LM_WAVES (LM_LANES / 64)
+LM_FN void lm_join_group(lm_state &a, ga_ulong &list, float by) {
+#if LM_WAVES > 1
+  LOCAL_MEM lm_state states[LM_WAVES];
+  const ga_uint wave = LID_0 >> 6, lane = LID_0 & 63;
+  if (lane == 0) states[wave] = a;
+#if LM_TOP
+  LOCAL_MEM ga_ulong lists[LM_WAVES][64];
+  lists[wave][lane] = list;
+#endif
+  local_barrier();
+  if (wave != 0) return;
+#pragma unroll
+  for (int i = 1; i < LM_WAVES; i++) lm_join(a, states[i], by);
+#if LM_TOP
+  for (int i = 1; i < LM_WAVES; i++) lm_merge(list, lists[i][lane]);
+#endif
+#endif
+}
+
+template <int N> LM_FN void lm_take(lm_state &a, ga_ulong &list, float (&y)[N], const lm_logprobs &p, ga_uint at, ga_uint step) {
+  const float most = lm_max_of(y, LM_LOWEST);
+  lm_add(a, y, most, p.by);
+#if LM_TOP
+  /* (a lane with -inf alone offers nothing: its largest must not pass for LM_LOWEST) */
+  lm_offer(list, y, most > LM_LOWEST ? most : lm_max_of(y, -INFINITY), p.top, at, step);
+#endif
+}
+
+#define LM_U (16 / LM_E)   /* chunks of a lane at a time: 16 elements */
+
+/* LM_LANES lanes share a row, or one of its pieces (LM_SPLIT): a loop over
+ * the row's aligned 16-byte chunks, LM_U per lane at a time, the next ones
+ * loading while the present ones are summed.  The elements before the first
+ * and after the last whole chunk go one to a lane. */
+KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(const lm_logprobs p) {
+#if LM_LANES < 256
+  const ga_long r = (ga_long)GID_0 * (256 / LM_LANES) + (LID_0 / LM_LANES);
+  if (r >= p.t) return;
+  const ga_uint lane = LID_0 % LM_LANES;
+#else
+  const ga_uint lane = LID_0;
+#if LM_SPLIT
+  const ga_long r = GID_0 / p.pieces;
+#else
+  const ga_long r = GID_0;
+#endif
+#endif
+#if LM_SPLIT
+  const ga_uint piece = GID_0 % p.pieces;
+#else
+  const ga_uint piece = 0;
+#endif
+  GLOBAL_MEM const LM_X *x = lm_at(p.logits, r * p.row);
+  const ga_uint v = (ga_uint)p.v;
+  ga_uint head = (ga_uint)(-(ga_size)x & 15) / (ga_uint)sizeof(LM_X);
+  if (head > v) head = v;
+  const ga_uint chunks = (v - head) / LM_E;
+  const ga_uint tail0 = head + chunks * LM_E;
+  GLOBAL_MEM const lm_u4 *q = (GLOBAL_MEM const lm_u4 *)(x + head);
+#if LM_SPLIT
+  const ga_uint from = piece * p.piece_chunks;
+  const ga_uint to = from + p.piece_chunks < chunks ? from + p.piece_chunks : chunks;
+#else
+  const ga_uint from = 0, to = chunks;
+#endif
+  const ga_uint minus_inf = lm_minus_inf(LM_X());
+  lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
+  ga_ulong list = 0;
+  lm_u4 raw[LM_U];
+  const auto fetch = [&](ga_uint base) {
+#pragma unroll
+    for (int u = 0; u < LM_U; u++) {
+      const ga_uint c = base + u * LM_LANES + lane;
+      raw[u] = minus_inf;
+      if (c < to) raw[u] = __builtin_nontemporal_load(q + c);
+    }
+  };
+  if (from < to) fetch(from);
+  if (piece == 0 && lane < 64 && v != chunks * LM_E) {
+    float y[1] = {-INFINITY};
+    ga_uint c = lane < head ? lane : tail0 + (lane - head);
+    if (c < v) y[0] = lm_get(x[c]);
+    lm_take(a, list, y, p, c, 0);
+  }
+  for (ga_uint base = from; base < to; base += LM_U * LM_LANES) {
+    const ga_uint at = head + (base + lane) * LM_E;
+    if (base + (lane & ~63u) + LM_LANES < to) {
+      float y[LM_U * LM_E];
+#pragma unroll
+      for (int u = 0; u < LM_U; u++) lm_unpack(raw[u], y + u * LM_E, LM_X());
+      if (base + LM_U * LM_LANES < to) fetch(base + LM_U * LM_LANES);
+      lm_take(a, list, y, p, at, LM_LANES * LM_E);
+    } else {          /* the last ones: no more than one chunk for any lane of this wavefront */
+      float y[LM_E];
+      lm_unpack(raw[0], y, LM_X());
+      lm_take(a, list, y, p, at, LM_LANES * LM_E);
+    }
+  }
+  lm_join_wave(a, p.by);
+  lm_join_group(a, list, p.by);
+  if (LID_0 >= 64 && LM_WAVES > 1) return;
+#if LM_SPLIT
+  GLOBAL_MEM char *to_p = p.partials + (ga_size)GID_0 * p.partial_bytes;
+  if (lane == 0) *(GLOBAL_MEM lm_state *)to_p = a;
+#if LM_TOP
+  if (lane < p.top) ((GLOBAL_MEM ga_ulong *)(to_p + sizeof(lm_state)))[lane] = list;
+#endif
+#else
+  lm_logprobs_finish(p, r, a, list);
+#endif
+}
+
+#if LM_SPLIT
+/* The pieces of a row: a group per row, a piece's statistics to a lane and
+ * its list to a wavefront at a time, in fixed order. */
+KERNEL void __launch_bounds__(LM_LANES) lm_logprobs_join(const lm_logprobs p) {
+  const ga_long r = GID_0;
+  const ga_uint wave = LID_0 >> 6, lane = LID_0 & 63;
+  GLOBAL_MEM const char *from = p.partials + (ga_size)r * p.pieces * p.partial_bytes;
+  lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
+  ga_ulong list = 0;
+  for (ga_uint i = LID_0; i < p.pieces; i += LM_LANES)
+    lm_join(a, *(GLOBAL_MEM const lm_state *)(from + (ga_size)i * p.partial_bytes), p.by);
+  lm_join_wave(a, p.by);
+#if LM_TOP
+  for (ga_uint i = wave; i < p.pieces; i += LM_WAVES) {
+    const ga_ulong k = lane < p.top ? ((GLOBAL_MEM const ga_ulong *)(from + (ga_size)i * p.partial_bytes + sizeof(lm_state)))[lane] : 0;
+    lm_merge(list, k);
+  }
+#endif
+  lm_join_group(a, list, p.by);
+  if (wave == 0) lm_logprobs_finish(p, r, a, list);
+}
+#endif
 #endif
 
 #if LM_KIND == LM_K_LOGPROBS_GRAD

@@ -30,7 +30,7 @@ def test_kernel_texts_compile(x, o):
     for kind in range(6):
         if kind > 1 and o != 11:
             continue
-        for ids in (5, 8):
-            text = C.string_at(source(kind | x << 8 | o << 20 | ids << 32))
+        for ids, extra in ((5, 0), (8, 0)) if kind != 2 else ((5, 1), (8, 1 | 32 | 64), (7, 4 | 32 | 128), (7, 16 | 64)):
+            text = C.string_at(source(kind | x << 8 | o << 20 | ids << 32 | extra << 44))
             log = C.c_char_p()
             assert compile_only(1, (C.c_char_p * 1)(text), None, C.byref(log)) == 0, (log.value or b"").decode()[-2000:]
