@@ -15,7 +15,7 @@ namespace {
 
 // ---- kernels of a context ------------------------------------------------------
 
-enum lm_kind { LM_EMBED, LM_EMBED_GRAD, LM_LOGPROBS, LM_LOGPROBS_GRAD, LM_NORM, LM_CLIP };
+enum lm_kind { LM_EMBED, LM_EMBED_GRAD, LM_LOGPROBS, LM_LOGPROBS_GRAD, LM_NORM, LM_CLIP, LM_SORT };
 
 // What a kernel text is specialised on; packed into the key it is kept under.
 struct lm_variant {
@@ -42,14 +42,22 @@ struct embed_args {
   int64_t n, v, d, ignore;
   float scale;
 };
+struct sorting_args {
+  const void *ids, *key_in, *order_in;
+  void *key, *order, *counts, *err;
+  int64_t id_step, ignore, v;
+  uint32_t n, groups, shift, bits, passes, pad;
+  void *fill;
+  int64_t fill_rows, fill_row, fill_bytes, fill_unit0, fill_unit1;
+};
 struct embed_grad_args {
   void *grad;
-  const void *dout, *ids;
-  void *err;
-  int64_t grad_row, dout_row, id_step;
-  int64_t n, v, d, ignore;
+  const void *dout, *key, *order;
+  void *partials;
+  int64_t grad_row, dout_row, v, d;
   float scale;
   int32_t accumulate;
+  uint32_t n, chunk, chunks, tiles;
 };
 struct logprobs_args {
   const void *logits, *ids;
@@ -98,6 +106,7 @@ std::string lm_source(const lm_variant &v) {
   name("LM_X", v.x);
   name("LM_O", v.o);
   name("LM_ID", v.id);
+  if (v.kind == LM_SORT) s += "#define LM_R " + std::to_string(v.extra ? v.extra : 4) + "\n";
   if (v.kind == LM_LOGPROBS) {
     s += "#define LM_LANES " + std::to_string((v.extra & 31 ? v.extra & 31 : 1) * 64) + "\n";
     s += std::string("#define LM_ENT ") + (v.extra & 32 ? "1" : "0") + "\n#define LM_TOP " + (v.extra & 64 ? "1" : "0") +
@@ -361,15 +370,107 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   if (c.err != GA_NO_ERROR) return c.err;
   if (d == 0 || (v == 0 && n == 0)) return GA_NO_ERROR;
   if (v > MAX_GROUPS || n > MAX_GROUPS) return c.fail(GA_XLARGE_ERROR, "too many rows");
-  GpuKernel *k;
+
+  const size_t osize = gpuarray_get_elsize(grad->typecode);
+  const size_t cols = 64 * 16 / gpuarray_get_elsize(dout->typecode);   // of a wavefront
+  const size_t tiles = (d + cols - 1) / cols;
+  // Tokens of a chunk: enough chunks to fill the chip with wavefronts, and
+  // not so few tokens that partial sums (two rows a chunk at most) count.
+  size_t chunk = 8;
+  while (chunk < 256 && n / (chunk * 2) * tiles >= 8192) chunk *= 2;
+  const size_t chunks = (n + chunk - 1) / chunk;
+  if (chunks * tiles > MAX_GROUPS) return c.fail(GA_XLARGE_ERROR, "too many elements");
+  // The digits: as few passes as ten bits a digit allow.
+  unsigned bits = 1;
+  while (v >> bits != 0) bits++;
+  const unsigned passes = (bits + 9) / 10;
+  bits = (bits + passes - 1) / passes;
+  const size_t per_lane = n <= 16384 ? (n + 1023) / 1024 : 4;
+  unsigned items = 1;
+  while (items < per_lane) items *= 2;
+  const bool small = n <= 16384;
+  const size_t groups = small ? 1 : (n + 4095) / 4096;
+
+  // scratch: two sets of keys and places, the counts of the digits, the partial sums
+  const size_t list = (n * 4 + 255) & ~(size_t)255;
+  const size_t counts = small ? 0 : (((groups + 1) << bits) * 4 + 255) & ~(size_t)255;
+  const size_t partials = chunks * 2 * tiles * cols * 4;
+  char *scratch = nullptr;
   gpudata *errbuf = nullptr;
-  int err = lm_kernel(ctx, lm_variant(LM_EMBED_GRAD, dout->typecode, grad->typecode, ids->typecode, 0),
-                      "lm_embed_grad_rows", sizeof(embed_grad_args), &k);
+  GpuKernel *ksmall = nullptr, *kcount = nullptr, *kscan = nullptr, *kmove = nullptr, *ksum = nullptr, *kjoin = nullptr;
+  const lm_variant vs(LM_SORT, GA_FLOAT, GA_FLOAT, ids->typecode, items);
+  const lm_variant vg(LM_EMBED_GRAD, dout->typecode, grad->typecode, GA_INT, 0);
+  int err = GA_NO_ERROR;
+  if (small) {
+    err = lm_kernel(ctx, vs, "lm_sort_small", sizeof(sorting_args), &ksmall);
+  } else {
+    err = lm_kernel(ctx, vs, "lm_sort_count", sizeof(sorting_args), &kcount);
+    if (err == GA_NO_ERROR) err = lm_kernel(ctx, vs, "lm_sort_scan", sizeof(sorting_args), &kscan);
+    if (err == GA_NO_ERROR) err = lm_kernel(ctx, vs, "lm_sort_move", sizeof(sorting_args), &kmove);
+  }
+  if (err == GA_NO_ERROR) err = lm_kernel(ctx, vg, "lm_embed_grad_sum", sizeof(embed_grad_args), &ksum);
+  if (err == GA_NO_ERROR) err = lm_kernel(ctx, vg, "lm_embed_grad_join", sizeof(embed_grad_args), &kjoin);
+  if (err == GA_NO_ERROR) err = lm_scratch(ctx, 4 * list + counts + partials + 256, &scratch);
   if (err == GA_NO_ERROR) err = lm_errbuf(ctx, grad, &errbuf);
   if (err != GA_NO_ERROR) return err;
-  embed_grad_args a = {at(grad), at(dout), at(ids), errbuf->devptr, grad->strides[0], dout->strides[0],
-                       ids->strides[0], (int64_t)n, (int64_t)v, (int64_t)d, ignore, (float)scale, accumulate != 0};
-  err = lm_launch(k, v ? (v + 3) / 4 : 1, 256, &a);
+
+  char *lists[4] = {scratch, scratch + list, scratch + 2 * list, scratch + 3 * list};
+  sorting_args s;
+  memset(&s, 0, sizeof(s));
+  s.ids = at(ids);
+  s.id_step = ids->strides[0];
+  s.err = errbuf->devptr;
+  s.counts = scratch + 4 * list;
+  s.ignore = ignore;
+  s.v = (int64_t)v;
+  s.n = (uint32_t)n;
+  s.groups = (uint32_t)groups;
+  s.bits = bits;
+  s.passes = passes;
+  // rows to clear, as one where they lie end to end
+  size_t units = 0;
+  if (!accumulate && v > 0) {
+    const bool dense = v == 1 || grad->strides[0] == (ssize_t)(d * osize);
+    s.fill = at(grad);
+    s.fill_rows = dense ? 1 : (int64_t)v;
+    s.fill_row = grad->strides[0];
+    s.fill_bytes = (int64_t)(dense ? v * d * osize : d * osize);
+    units = (size_t)s.fill_rows * (((size_t)s.fill_bytes + 16383) / 16384);
+  }
+  // launches of the sort that clear a share each, with up to 1024 groups more for it
+  const size_t launches = small ? 1 : 3 * passes;
+  size_t launched = 0;
+  auto sort_launch = [&](GpuKernel *k, size_t busy) -> int {
+    s.fill_unit0 = (int64_t)(units * launched / launches);
+    s.fill_unit1 = (int64_t)(units * (launched + 1) / launches);
+    launched++;
+    const size_t more = std::min<size_t>(((size_t)(s.fill_unit1 - s.fill_unit0) + 15) / 16, 1024);
+    return lm_launch(k, busy + more, 1024, &s);
+  };
+  if (small) {
+    s.key = lists[0];
+    s.order = lists[1];
+    err = sort_launch(ksmall, 1);
+  } else {
+    for (unsigned pass = 0; pass < passes && err == GA_NO_ERROR; pass++) {
+      const int from = pass & 1 ? 0 : 2, to = 2 - from;
+      s.shift = pass * bits;
+      s.key_in = lists[from];
+      s.order_in = lists[from + 1];
+      s.key = lists[to];
+      s.order = lists[to + 1];
+      err = sort_launch(kcount, groups);
+      if (err == GA_NO_ERROR) err = sort_launch(kscan, (((size_t)1 << bits) + 15) / 16);
+      if (err == GA_NO_ERROR) err = sort_launch(kmove, groups);
+    }
+  }
+  if (err == GA_NO_ERROR && n > 0) {
+    embed_grad_args a = {at(grad), at(dout), s.key, s.order, scratch + 4 * list + counts, grad->strides[0],
+                         dout->strides[0], (int64_t)v, (int64_t)d, (float)scale, accumulate != 0, (uint32_t)n,
+                         (uint32_t)chunk, (uint32_t)chunks, (uint32_t)tiles};
+    err = lm_launch(ksum, (chunks * tiles + 3) / 4, 256, &a);
+    if (err == GA_NO_ERROR && chunks > 1) err = lm_launch(kjoin, chunks * tiles, 256, &a);
+  }
   return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
 }
 

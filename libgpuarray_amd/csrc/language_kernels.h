@@ -19,6 +19,7 @@
 #define LM_K_LOGPROBS_GRAD 3
 #define LM_K_NORM 4
 #define LM_K_CLIP 5
+#define LM_K_SORT 6
 
 #define LM_FN static __device__ __forceinline__
 
@@ -115,54 +116,393 @@ KERNEL void __launch_bounds__(256) lm_embed_rows(const lm_embed p) {
 }
 #endif
 
+#if LM_KIND == LM_K_SORT
+/* ---- tokens in the order of their ids ---------------------------------------------
+ * The gradient of the table adds the rows of equal ids, so the tokens are
+ * sorted by id first: least significant digit first, every pass stable, so that
+ * the tokens of one id stay in their order and sums are the same on every call.
+ * No token and out of range become the key v, past all rows.  LM_R items per
+ * lane, 1024 lanes per group; an item's place among the equal digits of its
+ * wavefront is counted with ballots, one per bit.
+ *
+ * All that is short next to clearing the gradient's rows, which needs none of
+ * it: every launch of the sort has more groups than it needs for that, and those
+ * clear a share of the rows meanwhile. */
+struct lm_sorting {
+  GLOBAL_MEM const LM_ID *ids;      /* of the first pass */
+  GLOBAL_MEM const ga_uint *key_in, *order_in;
+  GLOBAL_MEM ga_uint *key, *order;  /* results of the pass */
+  GLOBAL_MEM ga_uint *counts;       /* [digit][group], then [digit] totals */
+  GLOBAL_MEM ga_int *err;
+  ga_long id_step, ignore, v;
+  ga_uint n, groups, shift, bits, passes;
+  ga_uint pad;
+  GLOBAL_MEM char *fill;            /* rows to clear: */
+  ga_long fill_rows, fill_row, fill_bytes, fill_unit0, fill_unit1;
+};
+#define LM_SEGMENT 16384   /* bytes that a wavefront clears at a time */
+
+/* Units [fill_unit0, fill_unit1) of rows x segments, over the wavefronts of the groups past `first`. */
+LM_FN void lm_clear(const lm_sorting &p, ga_uint first) {
+  const ga_long segments = (p.fill_bytes + LM_SEGMENT - 1) / LM_SEGMENT;
+  const ga_uint lane = LID_0 & 63;
+  const ga_long waves = (ga_long)(GDIM_0 - first) * 16;
+  for (ga_long u = p.fill_unit0 + (ga_long)(GID_0 - first) * 16 + (LID_0 >> 6); u < p.fill_unit1; u += waves) {
+    const ga_long row = u / segments, seg = u % segments;
+    GLOBAL_MEM char *b = p.fill + row * p.fill_row + seg * LM_SEGMENT;
+    ga_long bytes = p.fill_bytes - seg * LM_SEGMENT;
+    if (bytes > LM_SEGMENT) bytes = LM_SEGMENT;
+    ga_long head = (ga_long)(-(ga_size)b & 15);
+    if (head > bytes) head = bytes;
+    const ga_long chunks = (bytes - head) / 16, tail = head + chunks * 16;
+    GLOBAL_MEM lm_u4 *q = (GLOBAL_MEM lm_u4 *)(b + head);
+    const lm_u4 zero = {0, 0, 0, 0};
+    for (ga_long c = lane; c < chunks; c += 64) __builtin_nontemporal_store(zero, q + c);
+    const ga_long at = lane * 2 < head ? lane * 2 : tail + (lane * 2 - head);   /* elements are 2 or 4 bytes */
+    if (at < bytes) *(GLOBAL_MEM ga_ushort *)(b + at) = 0;
+  }
+}
+
+LM_FN ga_uint lm_first_key(const lm_sorting &p, ga_uint i) {
+  const ga_long id = lm_id((ga_long)*lm_at(p.ids, (ga_long)i * p.id_step), p.ignore, LM_NONE, p.v);
+  if (id == -2) *p.err = -1;
+  return id < 0 ? (ga_uint)p.v : (ga_uint)id;
+}
+
+/* exclusive prefix sum over 1024 lanes */
+LM_FN ga_uint lm_scan(ga_uint x) {
+  LOCAL_MEM ga_uint sums[16];
+  const ga_uint lane = LID_0 & 63, wave = LID_0 >> 6;
+  ga_uint s = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const ga_uint y = (ga_uint)__builtin_amdgcn_ds_bpermute((int)((lane - d) << 2), (int)s);
+    if (lane >= d) s += y;
+  }
+  if (lane == 63) sums[wave] = s;
+  local_barrier();
+  ga_uint before = 0;
+  for (ga_uint i = 0; i < wave; i++) before += sums[i];
+  local_barrier();
+  return before + s - x;
+}
+
+#define LM_BINS 1024   /* digits of up to 10 bits */
+/* rank[r]: how many equal digits this wavefront has before item r of this lane;
+ * counts[wave]: how many it has of each digit in all.  Item r of lane l is item r * 64 + l of the
+ * wavefront. */
+LM_FN void lm_rank(const ga_uint (&k)[LM_R], ga_uint (&rank)[LM_R], volatile ga_ushort (*counts)[LM_BINS], ga_uint shift, ga_uint bits) {
+  const ga_uint lane = LID_0 & 63, wave = LID_0 >> 6, mask = (1u << bits) - 1;
+  for (ga_uint b = LID_0; b < 16 * LM_BINS / 2; b += 1024) ((volatile ga_uint *)counts)[b] = 0;
+  local_barrier();
+#pragma unroll
+  for (int r = 0; r < LM_R; r++) {
+    const ga_uint d = (k[r] >> shift) & mask;
+    ga_ulong peers = ~(ga_ulong)0;
+    for (ga_uint b = 0; b < bits; b++) {
+      const bool one = (d >> b) & 1;
+      const ga_ulong with = __builtin_amdgcn_ballot_w64(one);
+      peers &= one ? with : ~with;
+    }
+    const ga_uint before = __builtin_amdgcn_mbcnt_hi((ga_uint)(peers >> 32), __builtin_amdgcn_mbcnt_lo((ga_uint)peers, 0));
+    const ga_uint have = counts[wave][d];
+    rank[r] = have + before;
+    __builtin_amdgcn_wave_barrier();
+    if (before == 0) counts[wave][d] = (ga_ushort)(have + (ga_uint)__builtin_popcountll(peers));
+    __builtin_amdgcn_wave_barrier();
+  }
+  local_barrier();
+}
+/* counts[wave][digit] becomes what the earlier wavefronts have of the digit; returns, in
+ * lane b, how many of digit b the group has */
+LM_FN ga_uint lm_wave_prefix(volatile ga_ushort (*counts)[LM_BINS], ga_uint bits) {
+  ga_uint total = 0;
+  if (LID_0 < (1u << bits)) {
+    for (int w = 0; w < 16; w++) {
+      const ga_uint c = counts[w][LID_0];
+      counts[w][LID_0] = (ga_ushort)total;
+      total += c;
+    }
+  }
+  return total;
+}
+
+/* Up to 1024 * LM_R tokens: group 0 sorts them by itself, in its LDS. */
+KERNEL void __launch_bounds__(1024) lm_sort_small(const lm_sorting p) {
+  if (GID_0 != 0) {
+    lm_clear(p, 1);
+    return;
+  }
+  LOCAL_MEM ga_ushort counts[16][LM_BINS] __attribute__((aligned(16)));
+  LOCAL_MEM ga_uint keys[1024 * LM_R];
+  LOCAL_MEM ga_ushort places[1024 * LM_R];
+  const ga_uint first = (LID_0 >> 6) * 64 * LM_R + (LID_0 & 63);
+  ga_uint k[LM_R], at[LM_R], rank[LM_R];
+#pragma unroll
+  for (int r = 0; r < LM_R; r++) {
+    at[r] = first + r * 64;
+    k[r] = at[r] < p.n ? lm_first_key(p, at[r]) : 0xffffffffu;
+  }
+  for (ga_uint pass = 0; pass < p.passes; pass++) {
+    const ga_uint shift = pass * p.bits, mask = (1u << p.bits) - 1;
+    lm_rank(k, rank, counts, shift, p.bits);
+    const ga_uint total = lm_wave_prefix(counts, p.bits);
+    const ga_uint base = lm_scan(total);
+    if (LID_0 < (1u << p.bits))
+      for (int w = 0; w < 16; w++) counts[w][LID_0] = (ga_ushort)(counts[w][LID_0] + base);
+    local_barrier();
+#pragma unroll
+    for (int r = 0; r < LM_R; r++) {
+      const ga_uint to = counts[LID_0 >> 6][(k[r] >> shift) & mask] + rank[r];
+      keys[to] = k[r];
+      places[to] = (ga_ushort)at[r];
+    }
+    local_barrier();
+#pragma unroll
+    for (int r = 0; r < LM_R; r++) {
+      k[r] = keys[first + r * 64];
+      at[r] = places[first + r * 64];
+    }
+    local_barrier();
+  }
+#pragma unroll
+  for (int r = 0; r < LM_R; r++) {
+    const ga_uint i = first + r * 64;
+    if (i < p.n) {
+      p.key[i] = k[r];
+      p.order[i] = at[r];
+    }
+  }
+}
+
+/* More tokens: a pass is three launches.  What every group has of each digit; */
+KERNEL void __launch_bounds__(1024) lm_sort_count(const lm_sorting p) {
+  if (GID_0 >= p.groups) {
+    lm_clear(p, p.groups);
+    return;
+  }
+  LOCAL_MEM ga_uint bins[LM_BINS];
+  bins[LID_0] = 0;
+  local_barrier();
+  const ga_uint first = GID_0 * 1024 * LM_R + LID_0;
+#pragma unroll
+  for (int r = 0; r < LM_R; r++) {
+    const ga_uint i = first + r * 1024;
+    if (i < p.n) {
+      const ga_uint k = p.shift == 0 ? lm_first_key(p, i) : p.key_in[i];
+      atomicAdd(&bins[(k >> p.shift) & ((1u << p.bits) - 1)], 1u);
+    }
+  }
+  local_barrier();
+  if (LID_0 < (1u << p.bits)) p.counts[(ga_size)LID_0 * p.groups + GID_0] = bins[LID_0];
+}
+/* what the earlier groups have of a digit, a wavefront per digit; */
+KERNEL void __launch_bounds__(1024) lm_sort_scan(const lm_sorting p) {
+  const ga_uint busy = ((1u << p.bits) + 15) / 16;
+  if (GID_0 >= busy) {
+    lm_clear(p, busy);
+    return;
+  }
+  const ga_uint digit = GID_0 * 16 + (LID_0 >> 6), lane = LID_0 & 63;
+  if (digit >= (1u << p.bits)) return;
+  GLOBAL_MEM ga_uint *c = p.counts + (ga_size)digit * p.groups;
+  ga_uint before = 0;
+  for (ga_uint base = 0; base < p.groups; base += 64) {
+    const ga_uint x = base + lane < p.groups ? c[base + lane] : 0;
+    ga_uint s = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const ga_uint y = (ga_uint)__builtin_amdgcn_ds_bpermute((int)((lane - d) << 2), (int)s);
+      if (lane >= d) s += y;
+    }
+    if (base + lane < p.groups) c[base + lane] = before + s - x;
+    before += (ga_uint)__builtin_amdgcn_readlane((int)s, 63);
+  }
+  if (lane == 0) p.counts[((ga_size)p.groups << p.bits) + digit] = before;
+}
+/* every token to its place. */
+KERNEL void __launch_bounds__(1024) lm_sort_move(const lm_sorting p) {
+  if (GID_0 >= p.groups) {
+    lm_clear(p, p.groups);
+    return;
+  }
+  LOCAL_MEM ga_ushort counts[16][LM_BINS] __attribute__((aligned(16)));
+  LOCAL_MEM ga_uint base[LM_BINS];
+  const ga_uint first = GID_0 * 1024 * LM_R + (LID_0 >> 6) * 64 * LM_R + (LID_0 & 63);
+  ga_uint k[LM_R], rank[LM_R];
+#pragma unroll
+  for (int r = 0; r < LM_R; r++) {
+    const ga_uint i = first + r * 64;
+    k[r] = i < p.n ? (p.shift == 0 ? lm_first_key(p, i) : p.key_in[i]) : 0xffffffffu;
+  }
+  lm_rank(k, rank, counts, p.shift, p.bits);
+  (void)lm_wave_prefix(counts, p.bits);
+  const bool mine = LID_0 < (1u << p.bits);
+  const ga_uint start = lm_scan(mine ? p.counts[((ga_size)p.groups << p.bits) + LID_0] : 0);
+  if (mine) base[LID_0] = start + p.counts[(ga_size)LID_0 * p.groups + GID_0];
+  local_barrier();
+#pragma unroll
+  for (int r = 0; r < LM_R; r++) {
+    const ga_uint i = first + r * 64, d = (k[r] >> p.shift) & ((1u << p.bits) - 1);
+    if (i < p.n) {
+      const ga_uint to = base[d] + counts[LID_0 >> 6][d] + rank[r];
+      p.key[to] = k[r];
+      p.order[to] = p.shift == 0 ? i : p.order_in[i];
+    }
+  }
+}
+#endif
+
 #if LM_KIND == LM_K_EMBED_GRAD
 struct lm_embed_grad {
   GLOBAL_MEM LM_O *grad;
   GLOBAL_MEM const LM_X *dout;
-  GLOBAL_MEM const LM_ID *ids;
-  GLOBAL_MEM ga_int *err;
-  ga_long grad_row, dout_row, id_step;
-  ga_long n, v, d, ignore;
+  GLOBAL_MEM const ga_uint *key, *order;   /* the sorted tokens */
+  GLOBAL_MEM float *partials;              /* [chunk][2][tiles * 64 * LM_E] */
+  ga_long grad_row, dout_row, v, d;
   float scale;
   ga_int accumulate;
+  ga_uint n, chunk, chunks, tiles;
 };
-/* One wavefront per row of the table: it looks through all ids for its own and
- * adds the rows of dout that have it, in order. */
-KERNEL void __launch_bounds__(256) lm_embed_grad_rows(const lm_embed_grad p) {
-  const ga_long r = (ga_long)GID_0 * 4 + (LID_0 >> 6);
-  const ga_uint lane = LID_0 & 63;
-  if (r >= p.v && r != 0) return;   /* (row 0 also looks for ids out of range) */
-  for (ga_long c0 = 0; c0 < p.d || c0 == 0; c0 += 512) {
-    float sum[8];
-    bool any = false;
+
+/* n of LM_E adjacent elements from p; a row may start anywhere */
+typedef ga_uint lm_u4a __attribute__((ext_vector_type(4), aligned(2)));
+LM_FN void lm_load(GLOBAL_MEM const LM_X *p, ga_int n, float (&y)[LM_E]) {
+  if (n >= LM_E) {
+    lm_unpack(*(GLOBAL_MEM const lm_u4a *)p, y, LM_X());
+  } else {
 #pragma unroll
-    for (int u = 0; u < 8; u++) sum[u] = 0.0f;
-    for (ga_long base = 0; base < p.n; base += 64) {
-      const ga_long i = base + lane;
-      const ga_long id = i < p.n ? lm_id((ga_long)*lm_at(p.ids, i * p.id_step), p.ignore, LM_NONE, p.v) : -1;
-      if (id == -2 && r == 0) *p.err = -1;
-      ga_ulong hits = __builtin_amdgcn_ballot_w64(id == r);
-      any = any || hits != 0;
-      while (hits != 0) {
-        const ga_long at = base + __builtin_ctzll(hits);
-        hits &= hits - 1;
+    for (int e = 0; e < LM_E; e++) y[e] = e < n ? (float)lm_get(p[e]) : 0.0f;
+  }
+}
+
+/* One run's sum is complete. */
+LM_FN void lm_write_run(const lm_embed_grad &p, ga_uint key, ga_long col, ga_int cols, const float (&sum)[LM_E]) {
+  GLOBAL_MEM LM_O *g = lm_at(p.grad, (ga_long)key * p.grad_row) + col;
+  float y[LM_E];
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-          const ga_long c = c0 + u * 64 + lane;
-          if (c < p.d) sum[u] += lm_get(lm_at(p.dout, at * p.dout_row)[c]);
+  for (int e = 0; e < LM_E; e++) {
+    y[e] = p.scale * sum[e];
+    if (p.accumulate && e < cols) y[e] += lm_get(g[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < LM_E; e++)
+    if (e < cols) lm_put(g + e, y[e]);
+}
+
+/* A wavefront adds the rows of a chunk of the sorted tokens, in their order, over
+ * 64 * LM_E columns.  A run of equal ids that lies inside the chunk is written
+ * when it ends; what a chunk has of a run that began earlier (slot 0), or that
+ * goes on in the next (slot 1), is left for lm_embed_grad_join. */
+#define LM_AHEAD 8   /* rows in flight */
+KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
+  const ga_uint unit = (ga_uint)__builtin_amdgcn_readfirstlane((int)(GID_0 * 4 + (LID_0 >> 6)));
+  const ga_uint chunk = unit / p.tiles, tile = unit % p.tiles, lane = LID_0 & 63;
+  if (chunk >= p.chunks) return;
+  const ga_uint p0 = chunk * p.chunk;
+  const ga_uint n = p.n - p0 < p.chunk ? p.n - p0 : p.chunk;
+  const ga_long col = ((ga_long)tile * 64 + lane) * LM_E;
+  const ga_int cols = p.d - col >= LM_E ? LM_E : (ga_int)(p.d - col);
+  const ga_uint none = (ga_uint)p.v;
+  GLOBAL_MEM float *slots = p.partials + (ga_size)chunk * 2 * p.tiles * 64 * LM_E + col;
+  float sum[LM_E];
+#pragma unroll
+  for (int e = 0; e < LM_E; e++) sum[e] = 0.0f;
+  const auto leave = [&](int slot) {
+#pragma unroll
+    for (int e = 0; e < LM_E; e++) slots[(ga_size)slot * p.tiles * 64 * LM_E + e] = sum[e];
+  };
+  const ga_uint before = p0 > 0 ? p.key[p0 - 1] : 0xffffffffu;
+  const ga_uint after = p0 + n < p.n ? p.key[p0 + n] : 0xffffffffu;
+  ga_uint run = p.key[p0];
+  bool here = run != before;   /* the run began in this chunk */
+  for (ga_uint sub = 0; sub < n; sub += 64) {
+    const ga_uint i = p0 + sub + lane;
+    const bool in = sub + lane < n;
+    const ga_uint keys = in ? p.key[i] : none, places = in ? p.order[i] : 0;
+    const ga_uint m = n - sub < 64 ? n - sub : 64;
+    for (ga_uint j = 0; j < m; j += LM_AHEAD) {
+      float y[LM_AHEAD][LM_E];
+      ga_uint k[LM_AHEAD];
+#pragma unroll
+      for (int u = 0; u < LM_AHEAD; u++) {
+        k[u] = j + u < m ? (ga_uint)__builtin_amdgcn_readlane((int)keys, (int)(j + u)) : none;
+        if (k[u] != none) {
+          const ga_uint at = (ga_uint)__builtin_amdgcn_readlane((int)places, (int)(j + u));
+          lm_load(lm_at(p.dout, (ga_long)at * p.dout_row) + col, cols, y[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < LM_AHEAD; u++) {
+        if (j + u >= m) continue;
+        if (k[u] != run) {
+          if (here) lm_write_run(p, run, col, cols, sum);
+          else leave(0);
+#pragma unroll
+          for (int e = 0; e < LM_E; e++) sum[e] = 0.0f;
+          run = k[u];
+          here = true;
+        }
+        if (k[u] != none) {
+#pragma unroll
+          for (int e = 0; e < LM_E; e++) sum[e] += y[u][e];
         }
       }
     }
+  }
+  if (run == none) return;
+  if (here && run != after) lm_write_run(p, run, col, cols, sum);
+  else leave(here ? 1 : 0);
+}
+
+/* The runs that cross chunks: the group of the chunk where a run begins adds
+ * its parts.  A long run's parts are split over the group's wavefronts. */
+KERNEL void __launch_bounds__(256) lm_embed_grad_join(const lm_embed_grad p) {
+  const ga_uint chunk = GID_0 / p.tiles, tile = GID_0 % p.tiles, lane = LID_0 & 63, wave = LID_0 >> 6;
+  const ga_uint p0 = chunk * p.chunk;
+  if (p0 + p.chunk >= p.n) return;             /* the last chunk: nothing goes on */
+  const ga_uint run = p.key[p0 + p.chunk];
+  if (run == (ga_uint)p.v || p.key[p0 + p.chunk - 1] != run) return;
+  if (p0 > 0 && p.key[p0 - 1] == run) return;  /* it began earlier */
+  /* the chunks after this one that begin inside the run */
+  ga_uint parts = 0;
+  for (;;) {
+    const ga_ulong at = (ga_ulong)(chunk + 1 + parts + lane) * p.chunk;
+    const ga_ulong in = __builtin_amdgcn_ballot_w64(at < p.n && p.key[at < p.n ? at : 0] == run);
+    if (~in == 0) {
+      parts += 64;
+      continue;
+    }
+    parts += (ga_uint)__builtin_ctzll(~in);
+    break;
+  }
+  const ga_long col = ((ga_long)tile * 64 + lane) * LM_E;
+  const ga_size pitch = (ga_size)p.tiles * 64 * LM_E;
+  GLOBAL_MEM const float *next = p.partials + (ga_size)(chunk + 1) * 2 * pitch + col;
+  const ga_uint share = parts > 16 ? (parts + 3) / 4 : parts;
+  const ga_uint from = wave * share < parts ? wave * share : parts, to = from + share < parts ? from + share : parts;
+  float sum[LM_E];
 #pragma unroll
-    for (int u = 0; u < 8; u++) {
-      const ga_long c = c0 + u * 64 + lane;
-      GLOBAL_MEM LM_O *g = lm_at(p.grad, r * p.grad_row) + c;
-      if (c < p.d && r < p.v) {
-        if (!p.accumulate) lm_put(g, p.scale * sum[u]);
-        else if (any) lm_put(g, lm_get(*g) + p.scale * sum[u]);
-      }
+  for (int e = 0; e < LM_E; e++) sum[e] = wave == 0 ? next[e - (ga_long)pitch] : 0.0f;
+#pragma unroll 8
+  for (ga_uint i = from; i < to; i++) {
+#pragma unroll
+    for (int e = 0; e < LM_E; e++) sum[e] += next[(ga_size)i * 2 * pitch + e];
+  }
+  if (parts > 16) {
+    LOCAL_MEM float meet[3][64][LM_E];
+    if (wave != 0) {
+#pragma unroll
+      for (int e = 0; e < LM_E; e++) meet[wave - 1][lane][e] = sum[e];
+    }
+    local_barrier();
+    if (wave == 0) {
+      for (int w = 0; w < 3; w++)
+#pragma unroll
+        for (int e = 0; e < LM_E; e++) sum[e] += meet[w][lane][e];
     }
   }
+  if (wave == 0) lm_write_run(p, run, col, p.d - col >= LM_E ? LM_E : (ga_int)(p.d - col), sum);
 }
 #endif
 
