@@ -41,6 +41,7 @@ struct embed_args {
   int64_t out_row, table_row, id_step;
   int64_t n, v, d, ignore;
   float scale;
+  uint32_t lanes_log2, segments;
 };
 struct sorting_args {
   const void *ids, *key_in, *order_in;
@@ -82,14 +83,15 @@ struct logprobs_grad_args {
   void *err;
   int64_t out_row, row, id_step, stats_row, stats_col, dlogp_step, entropy_step, dentropy_step;
   int64_t t, v, ignore;
-  float scale;
+  float scale, by;
+  uint32_t segments;
 };
-const int64_t LM_PIECE = 8192;
 struct tensors_args {
   void *partials, *result, *norm;
   double max_norm;
-  int64_t partial0, npartials;
-  int32_t n, norm_double, clip, pad;
+  uint32_t partial0, npartials;
+  int32_t n, norm_double;
+  uint32_t piece, in_place;
   const void *in[LM_TENSORS];
   void *out[LM_TENSORS];
   int64_t count[LM_TENSORS];
@@ -107,6 +109,7 @@ std::string lm_source(const lm_variant &v) {
   name("LM_O", v.o);
   name("LM_ID", v.id);
   if (v.kind == LM_SORT) s += "#define LM_R " + std::to_string(v.extra ? v.extra : 4) + "\n";
+  if (v.kind == LM_LOGPROBS_GRAD) s += std::string("#define LM_ENT ") + (v.extra ? "1\n" : "0\n");
   if (v.kind == LM_LOGPROBS) {
     s += "#define LM_LANES " + std::to_string((v.extra & 31 ? v.extra & 31 : 1) * 64) + "\n";
     s += std::string("#define LM_ENT ") + (v.extra & 32 ? "1" : "0") + "\n#define LM_TOP " + (v.extra & 64 ? "1" : "0") +
@@ -335,7 +338,13 @@ static int embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, 
   c.scale(scale, false);
   if (c.err != GA_NO_ERROR) return c.err;
   if (n == 0 || d == 0) return GA_NO_ERROR;
-  if (n > MAX_GROUPS) return c.fail(GA_XLARGE_ERROR, "too many rows");
+  // lanes of a row: a power of two, each with 16 bytes of the narrower side; a lane moves four rows
+  const size_t lane_cols = 16 / std::min(gpuarray_get_elsize(table->typecode), gpuarray_get_elsize(out->typecode));
+  const size_t row_lanes = (d + lane_cols - 1) / lane_cols, segments = (row_lanes + 255) / 256;
+  unsigned lanes_log2 = 0;
+  while (lanes_log2 < 8 && ((size_t)1 << lanes_log2) < row_lanes) lanes_log2++;
+  const size_t row_groups = (n + ((size_t)1024 >> lanes_log2) - 1) / ((size_t)1024 >> lanes_log2);
+  if (row_groups > MAX_GROUPS || segments > MAX_GROUPS / row_groups) return c.fail(GA_XLARGE_ERROR, "too many elements");
   GpuKernel *k;
   gpudata *errbuf = nullptr;
   int err = lm_kernel(ctx, lm_variant(LM_EMBED, table->typecode, out->typecode, ids->typecode, 0), "lm_embed_rows",
@@ -343,8 +352,8 @@ static int embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, 
   if (err == GA_NO_ERROR) err = lm_errbuf(ctx, out, &errbuf);
   if (err != GA_NO_ERROR) return err;
   embed_args a = {at(out), at(table), at(ids), errbuf->devptr, out->strides[0], table->strides[0], ids->strides[0],
-                  (int64_t)n, (int64_t)v, (int64_t)d, ignore, (float)scale};
-  err = lm_launch(k, n, 256, &a);
+                  (int64_t)n, (int64_t)v, (int64_t)d, ignore, (float)scale, lanes_log2, (uint32_t)segments};
+  err = lm_launch(k, row_groups * segments, 256, &a);
   return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
 }
 
@@ -603,9 +612,13 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
   if (c.err != GA_NO_ERROR) return c.err;
   if (t == 0 || v == 0) return GA_NO_ERROR;
   if (t > MAX_GROUPS || v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many rows or columns");
+  // a wavefront's share of a row: 32 elements a lane (and one chunk more, for rows that start inside one)
+  const size_t esize = gpuarray_get_elsize(logits->typecode);
+  const size_t segments = (v * esize / 16 + 2 + 128 * esize - 1) / (128 * esize);
+  if (segments > 2 * MAX_GROUPS / t) return c.fail(GA_XLARGE_ERROR, "too many elements");
   GpuKernel *k;
   gpudata *errbuf = nullptr;
-  int err = lm_kernel(ctx, lm_variant(LM_LOGPROBS_GRAD, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT, 0),
+  int err = lm_kernel(ctx, lm_variant(LM_LOGPROBS_GRAD, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT, entropy != nullptr),
                       "lm_logprobs_grad_rows", sizeof(logprobs_grad_args), &k);
   if (err == GA_NO_ERROR) err = lm_errbuf(ctx, logits, &errbuf);
   if (err != GA_NO_ERROR) return err;
@@ -614,8 +627,9 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
   logprobs_grad_args a = {at(dlogits), at(logits), ptr(ids), at(stats), ptr(dlogp), ptr(entropy), ptr(dentropy),
                           errbuf->devptr, dlogits->strides[0], logits->strides[0], step(ids, 0), stats->strides[0],
                           stats->strides[1], step(dlogp, 0), step(entropy, 0), step(dentropy, 0), (int64_t)t,
-                          (int64_t)v, ignore, (float)scale};
-  err = lm_launch(k, t, 256, &a);
+                          (int64_t)v, ignore, (float)scale, (float)((double)(float)scale * 1.4426950408889634),
+                          (uint32_t)segments};
+  err = lm_launch(k, (t * segments + 3) / 4, 256, &a);
   return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
 }
 
@@ -636,7 +650,8 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
   }
   if (std::isnan(max_norm) || max_norm < 0) return c.fail(GA_VALUE_ERROR, "max_norm must be 0 or above");
   if (c.err != GA_NO_ERROR) return c.err;
-  size_t pieces = 0;
+  size_t bytes = 0;
+  bool in_place = true;
   std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
   for (size_t i = 0; i < n; i++) {
     const GpuArray *a = as[i];
@@ -648,11 +663,12 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
     if (c.err != GA_NO_ERROR) return c.err;
     size_t count = 1;
     for (unsigned j = 0; j < a->nd; j++) count *= a->dimensions[j];
-    pieces += (count + LM_PIECE - 1) / LM_PIECE;
+    bytes += count * GpuArray_ITEMSIZE(a);
     if (norm != nullptr && overlap(norm, a)) return c.fail(GA_VALUE_ERROR, "overlaps an array", "norm");
     if (rs == nullptr) continue;
     const GpuArray *r = rs[i];
     if (r != a && !same_place(r, a)) {
+      in_place = false;
       if (GpuArray_context(r) != ctx) return c.fail(GA_INVALID_ERROR, "the arrays belong to different contexts");
       if (r->nd != a->nd || r->typecode != a->typecode)
         return c.fail(GA_INVALID_ERROR, "a result differs from its array in shape or type");
@@ -683,13 +699,19 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
     }
   }
 
+  // Pieces of 32 KiB, or more where that makes more than 4096 of them: a
+  // piece looks its array up, and a group of the norm takes several.
+  size_t piece = 2048;   // chunks of 16 bytes
+  while (bytes / 16 / piece > 4096 && piece < ((size_t)1 << 24)) piece *= 2;
+  const size_t max_groups = 1024;   // of the norm, per table
+  const size_t tables = (n + LM_TENSORS - 1) / LM_TENSORS + bytes / 16 / piece / 0x70000000;
   char *scratch = nullptr;
   GpuKernel *kpieces = nullptr, *kfinal = nullptr, *kclip = nullptr;
   const lm_variant vn(LM_NORM, GA_FLOAT, GA_FLOAT, GA_INT, 0), vc(LM_CLIP, GA_FLOAT, GA_FLOAT, GA_INT, 0);
   int err = lm_kernel(ctx, vn, "lm_norm_pieces", sizeof(tensors_args), &kpieces);
   if (err == GA_NO_ERROR) err = lm_kernel(ctx, vn, "lm_norm_final", sizeof(tensors_args), &kfinal);
   if (err == GA_NO_ERROR && rs != nullptr) err = lm_kernel(ctx, vc, "lm_clip_pieces", sizeof(tensors_args), &kclip);
-  if (err == GA_NO_ERROR) err = lm_scratch(ctx, 256 + pieces * sizeof(double), &scratch);
+  if (err == GA_NO_ERROR) err = lm_scratch(ctx, 256 + (tables + 1) * max_groups * sizeof(double), &scratch);
   if (err != GA_NO_ERROR) return err;
 
   tensors_args a;
@@ -699,11 +721,11 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
   a.norm = norm ? at(norm) : nullptr;
   a.norm_double = norm != nullptr && norm->typecode == GA_DOUBLE;
   a.max_norm = max_norm;
-  a.npartials = (int64_t)pieces;
-  // the arrays in tables of up to LM_TENSORS, each with fewer than 2^31 pieces
+  a.piece = (uint32_t)piece;
+  a.in_place = in_place;
+  // the arrays in tables of up to LM_TENSORS
   auto for_tables = [&](auto &&launch) -> int {
     size_t i = 0;
-    int64_t done = 0;
     while (i < n) {
       a.n = 0;
       a.first[0] = 0;
@@ -711,9 +733,9 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
         const GpuArray *x = as[i];
         int64_t count = 1;
         for (unsigned j = 0; j < x->nd; j++) count *= (int64_t)x->dimensions[j];
-        const int64_t p = (count + LM_PIECE - 1) / LM_PIECE;
+        const int64_t per = (int64_t)piece * (16 / (int64_t)GpuArray_ITEMSIZE(x)), p = (count + per - 1) / per;
         if (p == 0) continue;
-        if (a.first[a.n] + p > 0x7fffffff) {
+        if (a.first[a.n] + p > 0x70000000) {
           if (a.n == 0) return c.fail(GA_XLARGE_ERROR, "an array is too large");
           break;
         }
@@ -725,16 +747,19 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
         a.n++;
       }
       if (a.n == 0) break;
-      a.partial0 = done;
-      int e = launch();
+      const int e = launch(a.first[a.n]);
       if (e != GA_NO_ERROR) return e;
-      done += a.first[a.n];
     }
     return GA_NO_ERROR;
   };
-  err = for_tables([&] { return lm_launch(kpieces, a.first[a.n], 256, &a); });
-  if (err == GA_NO_ERROR) err = lm_launch(kfinal, 1, 256, &a);
-  if (err == GA_NO_ERROR && rs != nullptr) err = for_tables([&] { return lm_launch(kclip, a.first[a.n], 256, &a); });
+  err = for_tables([&](size_t pieces) -> int {
+    const size_t groups = std::min(pieces, max_groups);
+    a.partial0 = a.npartials;
+    a.npartials += (uint32_t)groups;
+    return lm_launch(kpieces, groups, 256, &a);
+  });
+  if (err == GA_NO_ERROR) err = lm_launch(kfinal, 1, 1024, &a);
+  if (err == GA_NO_ERROR && rs != nullptr) err = for_tables([&](size_t pieces) { return lm_launch(kclip, pieces, 256, &a); });
   return err;
 }
 

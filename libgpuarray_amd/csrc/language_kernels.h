@@ -88,6 +88,59 @@ LM_FN void lm_unpack(const lm_u4 &q, float *y, ga_bfloat16) {
     y[2 * e + 1] = __builtin_bit_cast(float, q[e] & 0xffff0000u);
   }
 }
+/* N adjacent elements, 8 or 16 or 32 bytes, from an address that is aligned to
+ * the element only; and the same for results. */
+typedef ga_uint lm_u2a __attribute__((ext_vector_type(2), aligned(2)));
+typedef ga_uint lm_u4a __attribute__((ext_vector_type(4), aligned(2)));
+template <int N, class T> LM_FN void lm_load(GLOBAL_MEM const T *p, float (&y)[N]) {
+  constexpr int per = 16 / (int)sizeof(T);
+  if constexpr (N * sizeof(T) == 8) {
+    const lm_u2a q = *(GLOBAL_MEM const lm_u2a *)p;
+    const lm_u4 wide = {q[0], q[1], 0, 0};
+    float z[8];
+    lm_unpack(wide, z, T());
+#pragma unroll
+    for (int e = 0; e < N; e++) y[e] = z[e];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / per; i++) {
+      const lm_u4 q = *(GLOBAL_MEM const lm_u4a *)(p + i * per);
+      lm_unpack(q, y + i * per, T());
+    }
+  }
+}
+LM_FN ga_uint lm_pair(float a, float b, ga_half) {
+  return (ga_uint)ga_float2half(a).data | (ga_uint)ga_float2half(b).data << 16;
+}
+LM_FN ga_uint lm_pair(float a, float b, ga_bfloat16) {   /* one conversion instruction for both */
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  const b2 r = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(ga_uint, r);
+}
+LM_FN void lm_pack(const float *y, ga_uint *w, int n, ga_float) {
+#pragma unroll
+  for (int i = 0; i < n; i++) w[i] = __builtin_bit_cast(ga_uint, y[i]);
+}
+template <class T> LM_FN void lm_pack(const float *y, ga_uint *w, int n, T) {
+#pragma unroll
+  for (int i = 0; i < n; i++) w[i] = lm_pair(y[2 * i], y[2 * i + 1], T());
+}
+template <int N, class T> LM_FN void lm_store(GLOBAL_MEM T *p, const float (&y)[N]) {
+  constexpr int words = N * (int)sizeof(T) / 4;
+  ga_uint w[words];
+  lm_pack(y, w, words, T());
+  if constexpr (words == 2) {
+    const lm_u2a q = {w[0], w[1]};
+    *(GLOBAL_MEM lm_u2a *)p = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < words; i += 4) {
+      const lm_u4a q = {w[i], w[i + 1], w[i + 2], w[i + 3]};
+      __builtin_nontemporal_store(q, (GLOBAL_MEM lm_u4a *)(p + i * 4 / (int)sizeof(T)));
+    }
+  }
+}
+
 /* a word of -inf elements */
 LM_FN ga_uint lm_minus_inf(ga_float) { return 0xff800000u; }
 LM_FN ga_uint lm_minus_inf(ga_half) { return 0xfc00fc00u; }
@@ -102,17 +155,55 @@ struct lm_embed {
   ga_long out_row, table_row, id_step;
   ga_long n, v, d, ignore;
   float scale;
+  ga_uint lanes_log2, segments;
 };
+/* elements of a lane: 16 bytes of the narrower side */
+#define LM_C (sizeof(LM_X) < sizeof(LM_O) ? 16 / (int)sizeof(LM_X) : 16 / (int)sizeof(LM_O))
+#define LM_ROWS 4
+
+/* 2^lanes_log2 lanes share a row's 256 * LM_C columns or fewer; a lane moves the
+ * same columns of LM_ROWS rows, so that the loads of the ids, of the rows and the
+ * stores each go out together.  Bound by memory. */
 KERNEL void __launch_bounds__(256) lm_embed_rows(const lm_embed p) {
-  const ga_long row = GID_0;
-  const ga_long id = lm_id((ga_long)*lm_at(p.ids, row * p.id_step), p.ignore, LM_NONE, p.v);
-  if (id == -2) {
-    if (LID_0 == 0) *p.err = -1;
-    return;
+  const ga_uint lane = LID_0 & ((1u << p.lanes_log2) - 1u), side = 256u >> p.lanes_log2;
+  const ga_long row0 = (ga_long)(GID_0 / p.segments) * side * LM_ROWS + (LID_0 >> p.lanes_log2);
+  const ga_long col = ((ga_long)(GID_0 % p.segments) * 256 + lane) * LM_C;
+  ga_long id[LM_ROWS];
+#pragma unroll
+  for (int u = 0; u < LM_ROWS; u++) {
+    const ga_long row = row0 + u * side;
+    id[u] = row < p.n ? lm_id((ga_long)*lm_at(p.ids, row * p.id_step), p.ignore, LM_NONE, p.v) : -3;
+    if (id[u] == -2) *p.err = -1;
   }
-  GLOBAL_MEM LM_O *o = lm_at(p.out, row * p.out_row);
-  GLOBAL_MEM const LM_X *x = lm_at(p.table, id * p.table_row);
-  for (ga_long c = LID_0; c < p.d; c += 256) lm_put(o + c, id < 0 ? 0.0f : p.scale * lm_get(x[c]));
+  if (col >= p.d) return;
+  const bool whole = p.d - col >= LM_C;
+  float y[LM_ROWS][LM_C];
+#pragma unroll
+  for (int u = 0; u < LM_ROWS; u++) {
+    GLOBAL_MEM const LM_X *x = lm_at(p.table, id[u] * p.table_row) + col;
+    if (id[u] >= 0 && whole) {
+      lm_load(x, y[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < LM_C; e++) y[u][e] = id[u] >= 0 && col + e < p.d ? lm_get(x[e]) : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < LM_ROWS; u++) {
+    if (id[u] < -1) continue;
+    GLOBAL_MEM LM_O *o = lm_at(p.out, (row0 + u * side) * p.out_row) + col;
+    if (id[u] >= 0) {       /* (a row of no token is 0 whatever the scale's sign) */
+#pragma unroll
+      for (int e = 0; e < LM_C; e++) y[u][e] *= p.scale;
+    }
+    if (whole) {
+      lm_store(o, y[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < LM_C; e++)
+        if (col + e < p.d) lm_put(o + e, y[u][e]);
+    }
+  }
 }
 #endif
 
@@ -365,11 +456,10 @@ struct lm_embed_grad {
   ga_uint n, chunk, chunks, tiles;
 };
 
-/* n of LM_E adjacent elements from p; a row may start anywhere */
-typedef ga_uint lm_u4a __attribute__((ext_vector_type(4), aligned(2)));
-LM_FN void lm_load(GLOBAL_MEM const LM_X *p, ga_int n, float (&y)[LM_E]) {
+/* n of LM_E adjacent elements from p */
+LM_FN void lm_load_some(GLOBAL_MEM const LM_X *p, ga_int n, float (&y)[LM_E]) {
   if (n >= LM_E) {
-    lm_unpack(*(GLOBAL_MEM const lm_u4a *)p, y, LM_X());
+    lm_load(p, y);
   } else {
 #pragma unroll
     for (int e = 0; e < LM_E; e++) y[e] = e < n ? (float)lm_get(p[e]) : 0.0f;
@@ -381,13 +471,20 @@ LM_FN void lm_write_run(const lm_embed_grad &p, ga_uint key, ga_long col, ga_int
   GLOBAL_MEM LM_O *g = lm_at(p.grad, (ga_long)key * p.grad_row) + col;
   float y[LM_E];
 #pragma unroll
-  for (int e = 0; e < LM_E; e++) {
-    y[e] = p.scale * sum[e];
-    if (p.accumulate && e < cols) y[e] += lm_get(g[e]);
-  }
+  for (int e = 0; e < LM_E; e++) y[e] = p.scale * sum[e];
+  if (cols >= LM_E) {
+    if (p.accumulate) {
+      float have[LM_E];
+      lm_load(g, have);
 #pragma unroll
-  for (int e = 0; e < LM_E; e++)
-    if (e < cols) lm_put(g + e, y[e]);
+      for (int e = 0; e < LM_E; e++) y[e] += have[e];
+    }
+    lm_store(g, y);
+  } else {
+#pragma unroll
+    for (int e = 0; e < LM_E; e++)
+      if (e < cols) lm_put(g + e, p.accumulate ? lm_get(g[e]) + y[e] : y[e]);
+  }
 }
 
 /* A wavefront adds the rows of a chunk of the sorted tokens, in their order, over
@@ -429,7 +526,7 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
         k[u] = j + u < m ? (ga_uint)__builtin_amdgcn_readlane((int)keys, (int)(j + u)) : none;
         if (k[u] != none) {
           const ga_uint at = (ga_uint)__builtin_amdgcn_readlane((int)places, (int)(j + u));
-          lm_load(lm_at(p.dout, (ga_long)at * p.dout_row) + col, cols, y[u]);
+          lm_load_some(lm_at(p.dout, (ga_long)at * p.dout_row) + col, cols, y[u]);
         }
       }
 #pragma unroll
@@ -899,48 +996,106 @@ struct lm_logprobs_grad {
   GLOBAL_MEM ga_int *err;
   ga_long out_row, row, id_step, stats_row, stats_col, dlogp_step, entropy_step, dentropy_step;
   ga_long t, v, ignore;
-  float scale;
+  float scale, by;               /* by = scale * log2(e) */
+  ga_uint segments;
 };
+#define LM_U (32 / LM_E)   /* chunks of a lane: 32 elements */
+
+/* A wavefront takes 64 * LM_U chunks of a row, on the result's 16-byte
+ * boundaries; what a row needs is a handful of scalars.  With
+ *   a = log2 p = (by * x - R) - rest,  R = by * m rounded,  rest = (by * m - R) + log2 of the sum
+ * an element is p * (A + B a), A = -scale (dlogp + dentropy * entropy), B = -scale * dentropy * ln 2, and the token's own has
+ * scale * dlogp besides.  One read and one write of every element: bound by memory. */
 KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad p) {
-  const ga_long r = GID_0;
+  const ga_uint unit = (ga_uint)__builtin_amdgcn_readfirstlane((int)(GID_0 * 4 + (LID_0 >> 6)));
+  const ga_long r = unit / p.segments;
+  if (r >= p.t) return;
+  const ga_uint segment = unit % p.segments, lane = LID_0 & 63;
   GLOBAL_MEM const LM_X *x = lm_at(p.logits, r * p.row);
   GLOBAL_MEM LM_X *o = lm_at(p.out, r * p.out_row);
+  const ga_int v = (ga_int)p.v;
+  /* chunk c has the elements first + c * LM_E .. of the row, those that it has */
+  const ga_int first = -(ga_int)(((ga_size)o & 15) / sizeof(LM_X));
+  const ga_int at = first + (ga_int)((segment * 64 * LM_U + lane) * LM_E);
+  float y[LM_U][LM_E];
+#pragma unroll
+  for (int u = 0; u < LM_U; u++) {
+    const ga_int c = at + u * 64 * LM_E;
+    if (c >= 0 && c + LM_E <= v) {
+      lm_u4 q = __builtin_nontemporal_load((GLOBAL_MEM const lm_u4a *)(x + c));
+      lm_unpack(q, y[u], LM_X());
+    } else {
+#pragma unroll
+      for (int e = 0; e < LM_E; e++) y[u][e] = c + e >= 0 && c + e < v ? (float)lm_get(x[c + e]) : 0.0f;
+    }
+  }
   const float m = *lm_at(p.stats, r * p.stats_row), ls = *lm_at(p.stats, r * p.stats_row + p.stats_col);
   float g = 0.0f, gh = 0.0f, h = 0.0f;
   ga_long id = -1;
   if (p.ids != nullptr) {
     id = lm_id((ga_long)*lm_at(p.ids, r * p.id_step), p.ignore, LM_NONE, p.v);
-    if (id == -2 && LID_0 == 0) *p.err = -1;
+    if (id == -2 && segment == 0 && lane == 0) *p.err = -1;
     if (id >= 0) g = *lm_at(p.dlogp, r * p.dlogp_step);
   }
-  if (p.entropy != nullptr) {
-    gh = *lm_at(p.dentropy, r * p.dentropy_step);
-    h = *lm_at(p.entropy, r * p.entropy_step);
-  }
-  for (ga_long c = LID_0; c < p.v; c += 256) {
-    float d = 0.0f;
-    if (ls != -INFINITY) {
-      const float lp = (lm_get(x[c]) - m) * p.scale - ls, q = __builtin_expf(lp);
-      d = p.scale * ((c == id ? g : 0.0f) - q * (g + gh * (__builtin_fmaxf(lp, -1000.0f) + h)));
+#if LM_ENT
+  gh = *lm_at(p.dentropy, r * p.dentropy_step);
+  h = *lm_at(p.entropy, r * p.entropy_step);
+#endif
+  const float big = p.by * m;
+  const bool nothing = ls == -INFINITY;
+  const bool far = !(__builtin_fabsf(big) <= 1e30f);   /* as for the statistics: p is exp(-ls) where x is m, else 0 */
+  const float rest = (far ? 0.0f : __builtin_fmaf(p.by, m, -big)) + ls * 1.4426950408889634f;
+  const float a = -p.scale * (g + gh * h) + (ls - ls), b = -p.scale * gh * 0.6931471805599453f;   /* (NaN where ls is) */
+  const float own = p.scale * g;
+#pragma unroll
+  for (int u = 0; u < LM_U; u++) {
+    const ga_int c = at + u * 64 * LM_E;
+    if (c >= v) break;
+    float d[LM_E];
+    if (nothing) {
+#pragma unroll
+      for (int e = 0; e < LM_E; e++) d[e] = 0.0f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < LM_E; e++) {
+        float l = __builtin_fmaf(y[u][e], p.by, -big) - rest;
+        if (far) l = y[u][e] == m ? -rest : -300.0f;
+        const float q = __builtin_amdgcn_exp2f(l);
+#if LM_ENT
+        d[e] = q * __builtin_fmaf(b, __builtin_fmaxf(l, -300.0f), a);
+#else
+        d[e] = q * a;
+#endif
+      }
+      if (id >= c && id < c + LM_E) {
+#pragma unroll
+        for (int e = 0; e < LM_E; e++) d[e] += c + e == id ? own : 0.0f;
+      }
     }
-    lm_put(o + c, d);
+    if (c >= 0 && c + LM_E <= v) {
+      lm_store(o + c, d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < LM_E; e++)
+        if (c + e >= 0 && c + e < v) lm_put(o + c + e, d[e]);
+    }
   }
 }
 #endif
 
 #if LM_KIND == LM_K_NORM || LM_KIND == LM_K_CLIP
-/* The arrays of a launch: up to LM_TENSORS of them, cut in pieces of LM_PIECE
- * elements that are numbered through; first[i] is the number of array i's
- * first piece.  The count of arrays is small next to the work, so a piece
- * finds its array by bisection of the table in its arguments. */
-#define LM_PIECE 8192
+/* The arrays of a launch: up to LM_TENSORS of them, cut in pieces of `piece`
+ * 16-byte chunks that are numbered through; first[i] is the number of array i's
+ * first piece.  Arguments are read through a long way, so a piece finds its
+ * array with one load a lane and a ballot, not by bisection. */
 struct lm_tensors {
-  GLOBAL_MEM double *partials;   /* sums of squares, one per piece */
-  GLOBAL_MEM double *result;     /* norm, factor */
+  GLOBAL_MEM double *partials;   /* sums of squares, one per group */
+  GLOBAL_MEM double *result;     /* the factor */
   GLOBAL_MEM void *norm;
   double max_norm;
-  ga_long partial0, npartials;
-  ga_int n, norm_double, clip, pad;
+  ga_uint partial0, npartials;
+  ga_int n, norm_double;
+  ga_uint piece, in_place;
   GLOBAL_MEM const void *in[LM_TENSORS];
   GLOBAL_MEM void *out[LM_TENSORS];
   ga_long count[LM_TENSORS];
@@ -948,55 +1103,110 @@ struct lm_tensors {
   unsigned char type[LM_TENSORS];   /* 0 float, 1 half, 2 bfloat16, 3 double */
 };
 LM_FN ga_int lm_find(const lm_tensors &p, ga_uint piece) {
-  ga_int lo = 0, hi = p.n;
-  while (hi - lo > 1) {
-    const ga_int mid = (lo + hi) >> 1;
-    if (p.first[mid] <= piece) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-#define LM_BY_TYPE(type, F)                     \
-  switch (type) {                               \
-    case 0: F(ga_float, float) break;           \
-    case 1: F(ga_half, float) break;            \
-    case 2: F(ga_bfloat16, float) break;        \
-    default: F(ga_double, double) break;        \
-  }
-/* the sum over a group of 256 lanes, in lane 0 */
-LM_FN double lm_group_sum(double v) {
-  LOCAL_MEM double part[256];
-  part[LID_0] = v;
-  local_barrier();
+  ga_int before = 0;
 #pragma unroll
-  for (int d = 128; d > 0; d >>= 1) {
-    if (LID_0 < d) part[LID_0] += part[LID_0 + d];
-    local_barrier();
+  for (int k = 0; k < LM_TENSORS; k += 64) {
+    const ga_int i = k + (ga_int)(LID_0 & 63);
+    const bool begun = i < p.n && p.first[i] <= piece;
+    before += (ga_int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(begun));
   }
-  return part[0];
+  return before - 1;
 }
+#define LM_BY_TYPE(type, F)       \
+  switch (type) {                 \
+    case 0: F(ga_float); break;   \
+    case 1: F(ga_half); break;    \
+    case 2: F(ga_bfloat16); break; \
+    default: F(ga_double); break; \
+  }
+LM_FN double lm_lane_xor(double v, int mask) {
+  const ga_ulong b = __builtin_bit_cast(ga_ulong, v);
+  const int from = (int)(((LID_0 & 63) ^ mask) << 2);
+  const ga_uint lo = (ga_uint)__builtin_amdgcn_ds_bpermute(from, (int)(ga_uint)b);
+  const ga_uint hi = (ga_uint)__builtin_amdgcn_ds_bpermute(from, (int)(ga_uint)(b >> 32));
+  return __builtin_bit_cast(double, (ga_ulong)hi << 32 | lo);
+}
+/* the sum over a group of WAVES wavefronts, in lane 0 */
+template <int WAVES> LM_FN double lm_group_sum(double v) {
+  LOCAL_MEM double part[WAVES];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += lm_lane_xor(v, d);
+  if ((LID_0 & 63) == 0) part[LID_0 >> 6] = v;
+  local_barrier();
+  v = part[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; w++) v += part[w];
+  return v;
+}
+LM_FN void lm_unpack(const lm_u4 &q, double *y, ga_double) {
+  typedef double d2 __attribute__((ext_vector_type(2)));
+  const d2 d = __builtin_bit_cast(d2, q);
+  y[0] = d[0];
+  y[1] = d[1];
+}
+template <class T> struct lm_wide { typedef float type; };
+template <> struct lm_wide<ga_double> { typedef double type; };
 #endif
 
 #if LM_KIND == LM_K_NORM
-KERNEL void __launch_bounds__(256) lm_norm_pieces(const lm_tensors p) {
-  const ga_int i = lm_find(p, GID_0);
-  const ga_long from = (ga_long)(GID_0 - p.first[i]) * LM_PIECE;
-  const ga_long left = p.count[i] - from;
-  const ga_int n = left < LM_PIECE ? (ga_int)left : LM_PIECE;
-  double s = 0.0;
-#define LM_SQUARES(T, A)                                        \
-  for (ga_int k = LID_0; k < n; k += 256) {                     \
-    const double x = lm_get(((GLOBAL_MEM const T *)p.in[i])[from + k]); \
-    s += x * x;                                                 \
+#define LM_GROUP 256
+#define LM_U 8   /* chunks in flight per lane */
+
+/* The squares of piece elements [from, from + n) of type T, summed in 64 bits:
+ * a multiply-add of doubles costs what one of floats does, and neither the
+ * largest nor the smallest float's square leaves their range. */
+template <class T> LM_FN double lm_squares(GLOBAL_MEM const T *x, ga_long n, ga_uint chunks) {
+  constexpr int E = 16 / (int)sizeof(T);
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  ga_long head = (ga_long)((-(ga_size)x & 15) / sizeof(T));
+  if (head > n) head = n;
+  const ga_uint whole = (ga_uint)((n - head) / E);
+  const ga_long tail = head + (ga_long)whole * E;
+  GLOBAL_MEM const lm_u4 *q = (GLOBAL_MEM const lm_u4 *)(x + head);
+  const ga_long k = LID_0 < head ? (ga_long)LID_0 : tail + (LID_0 - head);
+  if (k < n) {
+    const double y = (double)lm_get(x[k]);
+    s[0] = y * y;
   }
-  LM_BY_TYPE(p.type[i], LM_SQUARES)
-  s = lm_group_sum(s);
+  for (ga_uint c0 = 0; c0 < whole; c0 += LM_GROUP * LM_U) {
+    lm_u4 raw[LM_U];
+#pragma unroll
+    for (int u = 0; u < LM_U; u++) {
+      const ga_uint c = c0 + u * LM_GROUP + LID_0;
+      raw[u] = 0;
+      if (c < whole) raw[u] = q[c];
+    }
+#pragma unroll
+    for (int u = 0; u < LM_U; u++) {
+      typename lm_wide<T>::type y[E];
+      lm_unpack(raw[u], y, T());
+#pragma unroll
+      for (int e = 0; e < E; e++) s[e & 3] = __builtin_fma((double)y[e], (double)y[e], s[e & 3]);
+    }
+  }
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+/* A group adds every GDIM_0-th piece. */
+KERNEL void __launch_bounds__(LM_GROUP) lm_norm_pieces(const lm_tensors p) {
+  double s = 0.0;
+  const ga_uint pieces = p.first[p.n];
+  for (ga_uint piece = GID_0; piece < pieces; piece += GDIM_0) {
+    const ga_int i = lm_find(p, piece);
+#define LM_SQUARES(T)                                                        \
+  {                                                                          \
+    const ga_long per = (ga_long)p.piece * (16 / (ga_long)sizeof(T));        \
+    const ga_long from = (ga_long)(piece - p.first[i]) * per, left = p.count[i] - from; \
+    s += lm_squares((GLOBAL_MEM const T *)p.in[i] + from, left < per ? left : per, p.piece); \
+  }
+    LM_BY_TYPE(p.type[i], LM_SQUARES)
+  }
+  s = lm_group_sum<LM_GROUP / 64>(s);
   if (LID_0 == 0) p.partials[p.partial0 + GID_0] = s;
 }
-KERNEL void __launch_bounds__(256) lm_norm_final(const lm_tensors p) {
+KERNEL void __launch_bounds__(1024) lm_norm_final(const lm_tensors p) {
   double s = 0.0;
-  for (ga_long k = LID_0; k < p.npartials; k += 256) s += p.partials[k];
-  s = lm_group_sum(s);
+  for (ga_uint k = LID_0; k < p.npartials; k += 1024) s += p.partials[k];
+  s = lm_group_sum<16>(s);
   if (LID_0 == 0) {
     const double norm = __builtin_sqrt(s);
     p.result[0] = norm > p.max_norm && norm < (double)INFINITY ? p.max_norm / norm : 1.0;
@@ -1009,16 +1219,65 @@ KERNEL void __launch_bounds__(256) lm_norm_final(const lm_tensors p) {
 #endif
 
 #if LM_KIND == LM_K_CLIP
-KERNEL void __launch_bounds__(256) lm_clip_pieces(const lm_tensors p) {
+#define LM_GROUP 256
+#define LM_U 4
+
+LM_FN void lm_scaled(const lm_u4 &q, lm_u4a &r, double by, ga_double) {
+  typedef double d2 __attribute__((ext_vector_type(2)));
+  d2 d = __builtin_bit_cast(d2, q);
+  d[0] *= by;
+  d[1] *= by;
+  r = __builtin_bit_cast(lm_u4a, d);
+}
+template <class T> LM_FN void lm_scaled(const lm_u4 &q, lm_u4a &r, double by, T) {
+  constexpr int E = 16 / (int)sizeof(T);
+  float y[E];
+  lm_unpack(q, y, T());
+#pragma unroll
+  for (int e = 0; e < E; e++) y[e] *= (float)by;
+  ga_uint w[4];
+  lm_pack(y, w, 4, T());
+  r = lm_u4a{w[0], w[1], w[2], w[3]};
+}
+template <class T> LM_FN void lm_scale(GLOBAL_MEM const T *x, GLOBAL_MEM T *o, ga_long n, double by) {
+  constexpr int E = 16 / (int)sizeof(T);
+  ga_long head = (ga_long)((-(ga_size)o & 15) / sizeof(T));   /* chunks on the result's 16-byte boundaries */
+  if (head > n) head = n;
+  const ga_uint whole = (ga_uint)((n - head) / E);
+  const ga_long tail = head + (ga_long)whole * E;
+  const ga_long k = LID_0 < head ? (ga_long)LID_0 : tail + (LID_0 - head);
+  if (k < n) lm_put(o + k, (typename lm_wide<T>::type)by * lm_get(x[k]));
+  for (ga_uint c0 = 0; c0 < whole; c0 += LM_GROUP * LM_U) {
+    lm_u4 raw[LM_U];
+#pragma unroll
+    for (int u = 0; u < LM_U; u++) {
+      const ga_uint c = c0 + u * LM_GROUP + LID_0;
+      if (c < whole) raw[u] = *(GLOBAL_MEM const lm_u4a *)(x + head + (ga_long)c * E);
+    }
+#pragma unroll
+    for (int u = 0; u < LM_U; u++) {
+      const ga_uint c = c0 + u * LM_GROUP + LID_0;
+      if (c < whole) {
+        lm_u4a r;
+        lm_scaled(raw[u], r, by, T());
+        __builtin_nontemporal_store(r, (GLOBAL_MEM lm_u4a *)(o + head + (ga_long)c * E));
+      }
+    }
+  }
+}
+KERNEL void __launch_bounds__(LM_GROUP) lm_clip_pieces(const lm_tensors p) {
   const double by = p.result[0];
-  const ga_int i = lm_find(p, GID_0);
+  if (by == 1.0 && p.in_place) return;
+  /* from the end, where the norm's reads were last: what the caches still have of them comes first */
+  const ga_uint piece = p.first[p.n] - 1 - GID_0;
+  const ga_int i = lm_find(p, piece);
   if (by == 1.0 && p.in[i] == p.out[i]) return;
-  const ga_long from = (ga_long)(GID_0 - p.first[i]) * LM_PIECE;
-  const ga_long left = p.count[i] - from;
-  const ga_int n = left < LM_PIECE ? (ga_int)left : LM_PIECE;
-#define LM_SCALE(T, A)                                          \
-  for (ga_int k = LID_0; k < n; k += 256)                       \
-    lm_put((GLOBAL_MEM T *)p.out[i] + from + k, (A)by * lm_get(((GLOBAL_MEM const T *)p.in[i])[from + k]));
+#define LM_SCALE(T)                                                          \
+  {                                                                          \
+    const ga_long per = (ga_long)p.piece * (16 / (ga_long)sizeof(T));        \
+    const ga_long from = (ga_long)(piece - p.first[i]) * per, left = p.count[i] - from; \
+    lm_scale((GLOBAL_MEM const T *)p.in[i] + from, (GLOBAL_MEM T *)p.out[i] + from, left < per ? left : per, by); \
+  }
   LM_BY_TYPE(p.type[i], LM_SCALE)
 }
 #endif
