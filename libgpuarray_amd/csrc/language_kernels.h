@@ -175,33 +175,34 @@ KERNEL void __launch_bounds__(256) lm_embed_rows(const lm_embed p) {
     id[u] = row < p.n ? lm_id((ga_long)*lm_at(p.ids, row * p.id_step), p.ignore, LM_NONE, p.v) : -3;
     if (id[u] == -2) *p.err = -1;
   }
-  if (col >= p.d) return;
-  const bool whole = p.d - col >= LM_C;
+  if (col >= p.d || p.v == 0) return;
+  /* Loads are unconditional, so that all of them are in flight at once: rows
+   * of no token fetch row 0, and the lane at a row's end fetches the row's
+   * last LM_C columns, of which it writes its own. */
+  const ga_long from = p.d >= LM_C && p.d - col < LM_C ? p.d - LM_C : col;
+  const ga_int skip = (ga_int)(col - from);
   float y[LM_ROWS][LM_C];
+  if (p.d >= LM_C) {
 #pragma unroll
-  for (int u = 0; u < LM_ROWS; u++) {
-    GLOBAL_MEM const LM_X *x = lm_at(p.table, id[u] * p.table_row) + col;
-    if (id[u] >= 0 && whole) {
-      lm_load(x, y[u]);
-    } else {
+    for (int u = 0; u < LM_ROWS; u++) lm_load(lm_at(p.table, (id[u] > 0 ? id[u] : 0) * p.table_row) + from, y[u]);
+  } else {
 #pragma unroll
-      for (int e = 0; e < LM_C; e++) y[u][e] = id[u] >= 0 && col + e < p.d ? lm_get(x[e]) : 0.0f;
-    }
+    for (int u = 0; u < LM_ROWS; u++)
+#pragma unroll
+      for (int e = 0; e < LM_C; e++) y[u][e] = e < p.d ? (float)lm_get(lm_at(p.table, (id[u] > 0 ? id[u] : 0) * p.table_row)[e]) : 0.0f;
   }
 #pragma unroll
   for (int u = 0; u < LM_ROWS; u++) {
     if (id[u] < -1) continue;
-    GLOBAL_MEM LM_O *o = lm_at(p.out, (row0 + u * side) * p.out_row) + col;
-    if (id[u] >= 0) {       /* (a row of no token is 0 whatever the scale's sign) */
+    GLOBAL_MEM LM_O *o = lm_at(p.out, (row0 + u * side) * p.out_row) + from;
 #pragma unroll
-      for (int e = 0; e < LM_C; e++) y[u][e] *= p.scale;
-    }
-    if (whole) {
+    for (int e = 0; e < LM_C; e++) y[u][e] = id[u] >= 0 ? y[u][e] * p.scale : 0.0f;
+    if (skip == 0 && p.d >= LM_C) {
       lm_store(o, y[u]);
     } else {
 #pragma unroll
       for (int e = 0; e < LM_C; e++)
-        if (col + e < p.d) lm_put(o + e, y[u][e]);
+        if (e >= skip && from + e < p.d) lm_put(o + e, y[u][e]);
     }
   }
 }
@@ -456,23 +457,32 @@ struct lm_embed_grad {
   ga_uint n, chunk, chunks, tiles;
 };
 
-/* n of LM_E adjacent elements from p */
-LM_FN void lm_load_some(GLOBAL_MEM const LM_X *p, ga_int n, float (&y)[LM_E]) {
-  if (n >= LM_E) {
-    lm_load(p, y);
-  } else {
-#pragma unroll
-    for (int e = 0; e < LM_E; e++) y[e] = e < n ? (float)lm_get(p[e]) : 0.0f;
+/* The columns of a lane: LM_E from `from` on, of which the first `skip` belong
+ * to the lane before it (at a row's end, where the last LM_E columns are
+ * fetched), and `cols` are inside the row. */
+struct lm_columns {
+  ga_long from;
+  ga_int skip, cols;
+};
+LM_FN lm_columns lm_columns_of(ga_long col, ga_long d) {
+  lm_columns c = {col, 0, LM_E};
+  if (d < LM_E) {
+    c.cols = col == 0 ? (ga_int)d : 0;
+    c.from = 0;
+  } else if (d - col < LM_E) {
+    c.from = d - LM_E;
+    c.skip = col >= d ? LM_E : (ga_int)(col - c.from);
   }
+  return c;
 }
 
 /* One run's sum is complete. */
-LM_FN void lm_write_run(const lm_embed_grad &p, ga_uint key, ga_long col, ga_int cols, const float (&sum)[LM_E]) {
-  GLOBAL_MEM LM_O *g = lm_at(p.grad, (ga_long)key * p.grad_row) + col;
+LM_FN void lm_write_run(const lm_embed_grad &p, ga_uint key, const lm_columns &c, const float (&sum)[LM_E]) {
+  GLOBAL_MEM LM_O *g = lm_at(p.grad, (ga_long)key * p.grad_row) + c.from;
   float y[LM_E];
 #pragma unroll
   for (int e = 0; e < LM_E; e++) y[e] = p.scale * sum[e];
-  if (cols >= LM_E) {
+  if (c.skip == 0 && c.cols == LM_E) {
     if (p.accumulate) {
       float have[LM_E];
       lm_load(g, have);
@@ -483,7 +493,7 @@ LM_FN void lm_write_run(const lm_embed_grad &p, ga_uint key, ga_long col, ga_int
   } else {
 #pragma unroll
     for (int e = 0; e < LM_E; e++)
-      if (e < cols) lm_put(g + e, p.accumulate ? lm_get(g[e]) + y[e] : y[e]);
+      if (e >= c.skip && e < c.cols) lm_put(g + e, p.accumulate ? lm_get(g[e]) + y[e] : y[e]);
   }
 }
 
@@ -499,7 +509,7 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
   const ga_uint p0 = chunk * p.chunk;
   const ga_uint n = p.n - p0 < p.chunk ? p.n - p0 : p.chunk;
   const ga_long col = ((ga_long)tile * 64 + lane) * LM_E;
-  const ga_int cols = p.d - col >= LM_E ? LM_E : (ga_int)(p.d - col);
+  const lm_columns mine = lm_columns_of(col, p.d);
   const ga_uint none = (ga_uint)p.v;
   GLOBAL_MEM float *slots = p.partials + (ga_size)chunk * 2 * p.tiles * 64 * LM_E + col;
   float sum[LM_E];
@@ -521,19 +531,27 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
     for (ga_uint j = 0; j < m; j += LM_AHEAD) {
       float y[LM_AHEAD][LM_E];
       ga_uint k[LM_AHEAD];
+      if (p.d >= LM_E) {     /* (unconditional loads: all of them in flight) */
 #pragma unroll
-      for (int u = 0; u < LM_AHEAD; u++) {
-        k[u] = j + u < m ? (ga_uint)__builtin_amdgcn_readlane((int)keys, (int)(j + u)) : none;
-        if (k[u] != none) {
+        for (int u = 0; u < LM_AHEAD; u++) {
           const ga_uint at = (ga_uint)__builtin_amdgcn_readlane((int)places, (int)(j + u));
-          lm_load_some(lm_at(p.dout, (ga_long)at * p.dout_row) + col, cols, y[u]);
+          lm_load(lm_at(p.dout, (ga_long)at * p.dout_row) + mine.from, y[u]);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < LM_AHEAD; u++) {
+          const ga_uint at = (ga_uint)__builtin_amdgcn_readlane((int)places, (int)(j + u));
+#pragma unroll
+          for (int e = 0; e < LM_E; e++) y[u][e] = e < mine.cols ? (float)lm_get(lm_at(p.dout, (ga_long)at * p.dout_row)[e]) : 0.0f;
         }
       }
+#pragma unroll
+      for (int u = 0; u < LM_AHEAD; u++) k[u] = (ga_uint)__builtin_amdgcn_readlane((int)keys, (int)(j + u));
 #pragma unroll
       for (int u = 0; u < LM_AHEAD; u++) {
         if (j + u >= m) continue;
         if (k[u] != run) {
-          if (here) lm_write_run(p, run, col, cols, sum);
+          if (here) lm_write_run(p, run, mine, sum);
           else leave(0);
 #pragma unroll
           for (int e = 0; e < LM_E; e++) sum[e] = 0.0f;
@@ -548,7 +566,7 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
     }
   }
   if (run == none) return;
-  if (here && run != after) lm_write_run(p, run, col, cols, sum);
+  if (here && run != after) lm_write_run(p, run, mine, sum);
   else leave(here ? 1 : 0);
 }
 
@@ -599,7 +617,7 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_join(const lm_embed_grad p) {
         for (int e = 0; e < LM_E; e++) sum[e] += meet[w][lane][e];
     }
   }
-  if (wave == 0) lm_write_run(p, run, col, p.d - col >= LM_E ? LM_E : (ga_int)(p.d - col), sum);
+  if (wave == 0) lm_write_run(p, run, lm_columns_of(col, p.d), sum);
 }
 #endif
 
@@ -920,12 +938,22 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
   lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
   ga_ulong list = 0;
   lm_u4 raw[LM_U];
-  const auto fetch = [&](ga_uint base) {
+  const auto fetch = [&](ga_uint base) {   /* unconditional loads: all of them in flight */
+    if (base + LM_U * LM_LANES <= to) {
 #pragma unroll
-    for (int u = 0; u < LM_U; u++) {
-      const ga_uint c = base + u * LM_LANES + lane;
-      raw[u] = minus_inf;
-      if (c < to) raw[u] = __builtin_nontemporal_load(q + c);
+      for (int u = 0; u < LM_U; u++) raw[u] = __builtin_nontemporal_load(q + (base + u * LM_LANES + lane));
+    } else {
+#pragma unroll
+      for (int u = 0; u < LM_U; u++) {
+        const ga_uint c = base + u * LM_LANES + lane;
+        raw[u] = __builtin_nontemporal_load(q + (c < to ? c : to - 1));
+      }
+#pragma unroll
+      for (int u = 0; u < LM_U; u++) {
+        const bool in = base + u * LM_LANES + lane < to;
+#pragma unroll
+        for (int i = 0; i < 4; i++) raw[u][i] = in ? raw[u][i] : minus_inf;
+      }
     }
   };
   if (from < to) fetch(from);
@@ -1017,17 +1045,21 @@ KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad 
   /* chunk c has the elements first + c * LM_E .. of the row, those that it has */
   const ga_int first = -(ga_int)(((ga_size)o & 15) / sizeof(LM_X));
   const ga_int at = first + (ga_int)((segment * 64 * LM_U + lane) * LM_E);
+  /* Unconditional loads, all of them in flight: at the row's ends the first or
+   * last LM_E elements, of which the lane writes those of its chunk. */
   float y[LM_U][LM_E];
+  if (v >= LM_E) {
 #pragma unroll
-  for (int u = 0; u < LM_U; u++) {
-    const ga_int c = at + u * 64 * LM_E;
-    if (c >= 0 && c + LM_E <= v) {
-      lm_u4 q = __builtin_nontemporal_load((GLOBAL_MEM const lm_u4a *)(x + c));
+    for (int u = 0; u < LM_U; u++) {
+      const ga_int c = at + u * 64 * LM_E, from = c < 0 ? 0 : c > v - LM_E ? v - LM_E : c;
+      const lm_u4 q = __builtin_nontemporal_load((GLOBAL_MEM const lm_u4a *)(x + from));
       lm_unpack(q, y[u], LM_X());
-    } else {
-#pragma unroll
-      for (int e = 0; e < LM_E; e++) y[u][e] = c + e >= 0 && c + e < v ? (float)lm_get(x[c + e]) : 0.0f;
     }
+  } else {
+#pragma unroll
+    for (int u = 0; u < LM_U; u++)
+#pragma unroll
+      for (int e = 0; e < LM_E; e++) y[u][e] = e < v ? (float)lm_get(x[e]) : 0.0f;
   }
   const float m = *lm_at(p.stats, r * p.stats_row), ls = *lm_at(p.stats, r * p.stats_row + p.stats_col);
   float g = 0.0f, gh = 0.0f, h = 0.0f;
@@ -1050,6 +1082,7 @@ KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad 
 #pragma unroll
   for (int u = 0; u < LM_U; u++) {
     const ga_int c = at + u * 64 * LM_E;
+    const ga_int from = v < LM_E || c < 0 ? 0 : c > v - LM_E ? v - LM_E : c;
     if (c >= v) break;
     float d[LM_E];
     if (nothing) {
@@ -1067,17 +1100,17 @@ KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad 
         d[e] = q * a;
 #endif
       }
-      if (id >= c && id < c + LM_E) {
+      if (id >= from && id < from + LM_E) {
 #pragma unroll
-        for (int e = 0; e < LM_E; e++) d[e] += c + e == id ? own : 0.0f;
+        for (int e = 0; e < LM_E; e++) d[e] += from + e == id ? own : 0.0f;
       }
     }
-    if (c >= 0 && c + LM_E <= v) {
+    if (from == c && v >= LM_E) {
       lm_store(o + c, d);
     } else {
 #pragma unroll
       for (int e = 0; e < LM_E; e++)
-        if (c + e >= 0 && c + e < v) lm_put(o + c + e, d[e]);
+        if (from + e >= c && from + e < c + LM_E && from + e < v) lm_put(o + from + e, d[e]);
     }
   }
 }
@@ -1168,21 +1201,29 @@ template <class T> LM_FN double lm_squares(GLOBAL_MEM const T *x, ga_long n, ga_
     const double y = (double)lm_get(x[k]);
     s[0] = y * y;
   }
-  for (ga_uint c0 = 0; c0 < whole; c0 += LM_GROUP * LM_U) {
-    lm_u4 raw[LM_U];
+  const auto add = [&](const lm_u4 &raw) {
+    typename lm_wide<T>::type y[E];
+    lm_unpack(raw, y, T());
+#pragma unroll
+    for (int e = 0; e < E; e++) s[e & 3] = __builtin_fma((double)y[e], (double)y[e], s[e & 3]);
+  };
+  lm_u4 raw[LM_U];
+  ga_uint c0 = 0;
+  for (; c0 + LM_GROUP * LM_U <= whole; c0 += LM_GROUP * LM_U) {
+#pragma unroll
+    for (int u = 0; u < LM_U; u++) raw[u] = q[c0 + u * LM_GROUP + LID_0];
+#pragma unroll
+    for (int u = 0; u < LM_U; u++) add(raw[u]);
+  }
+  if (c0 < whole) {     /* (unconditional loads: all of them in flight) */
 #pragma unroll
     for (int u = 0; u < LM_U; u++) {
       const ga_uint c = c0 + u * LM_GROUP + LID_0;
-      raw[u] = 0;
-      if (c < whole) raw[u] = q[c];
+      raw[u] = q[c < whole ? c : whole - 1];
     }
 #pragma unroll
-    for (int u = 0; u < LM_U; u++) {
-      typename lm_wide<T>::type y[E];
-      lm_unpack(raw[u], y, T());
-#pragma unroll
-      for (int e = 0; e < E; e++) s[e & 3] = __builtin_fma((double)y[e], (double)y[e], s[e & 3]);
-    }
+    for (int u = 0; u < LM_U; u++)
+      if (c0 + u * LM_GROUP + LID_0 < whole) add(raw[u]);
   }
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
@@ -1248,29 +1289,26 @@ template <class T> LM_FN void lm_scale(GLOBAL_MEM const T *x, GLOBAL_MEM T *o, g
   const ga_long k = LID_0 < head ? (ga_long)LID_0 : tail + (LID_0 - head);
   if (k < n) lm_put(o + k, (typename lm_wide<T>::type)by * lm_get(x[k]));
   for (ga_uint c0 = 0; c0 < whole; c0 += LM_GROUP * LM_U) {
-    lm_u4 raw[LM_U];
+    lm_u4 raw[LM_U];     /* (unconditional loads: all of them in flight) */
 #pragma unroll
     for (int u = 0; u < LM_U; u++) {
       const ga_uint c = c0 + u * LM_GROUP + LID_0;
-      if (c < whole) raw[u] = *(GLOBAL_MEM const lm_u4a *)(x + head + (ga_long)c * E);
+      raw[u] = __builtin_nontemporal_load((GLOBAL_MEM const lm_u4a *)(x + head + (ga_long)(c < whole ? c : whole - 1) * E));
     }
 #pragma unroll
     for (int u = 0; u < LM_U; u++) {
       const ga_uint c = c0 + u * LM_GROUP + LID_0;
-      if (c < whole) {
-        lm_u4a r;
-        lm_scaled(raw[u], r, by, T());
-        __builtin_nontemporal_store(r, (GLOBAL_MEM lm_u4a *)(o + head + (ga_long)c * E));
-      }
+      lm_u4a r;
+      lm_scaled(raw[u], r, by, T());
+      if (c < whole) __builtin_nontemporal_store(r, (GLOBAL_MEM lm_u4a *)(o + head + (ga_long)c * E));
     }
   }
 }
 KERNEL void __launch_bounds__(LM_GROUP) lm_clip_pieces(const lm_tensors p) {
+  const ga_uint piece = GID_0;
+  const ga_int i = lm_find(p, piece);
   const double by = p.result[0];
   if (by == 1.0 && p.in_place) return;
-  /* from the end, where the norm's reads were last: what the caches still have of them comes first */
-  const ga_uint piece = p.first[p.n] - 1 - GID_0;
-  const ga_int i = lm_find(p, piece);
   if (by == 1.0 && p.in[i] == p.out[i]) return;
 #define LM_SCALE(T)                                                          \
   {                                                                          \
