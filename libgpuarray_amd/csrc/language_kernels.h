@@ -671,20 +671,19 @@ LM_FN void lm_join(lm_state &a, lm_state b, float by) {
   a.s += b.s;
   a.w += b.w;
 }
-template <int MASK> LM_FN void lm_join_xor(lm_state &a, float by) {
-  lm_state b;
-  b.m = lm_xor<MASK>(a.m);
-  b.s = lm_xor<MASK>(a.s);
-  b.w = LM_ENT ? lm_xor<MASK>(a.w) : 0.0f;
-  lm_join(a, b, by);
+template <int MASK> LM_FN void lm_max_xor(float &m) { m = __builtin_fmaxf(m, lm_xor<MASK>(m)); }
+template <int MASK> LM_FN void lm_sum_xor(lm_state &a) {
+  a.s += lm_xor<MASK>(a.s);
+#if LM_ENT
+  a.w += lm_xor<MASK>(a.w);
+#endif
 }
+/* The maximum first, so that a lane rescales once. */
 LM_FN void lm_join_wave(lm_state &a, float by) {
-  lm_join_xor<1>(a, by);
-  lm_join_xor<2>(a, by);
-  lm_join_xor<7>(a, by);
-  lm_join_xor<15>(a, by);
-  lm_join_xor<16>(a, by);
-  lm_join_xor<32>(a, by);
+  float m = a.m;
+  lm_max_xor<1>(m); lm_max_xor<2>(m); lm_max_xor<7>(m); lm_max_xor<15>(m); lm_max_xor<16>(m); lm_max_xor<32>(m);
+  lm_rescale(a, m, by);
+  lm_sum_xor<1>(a); lm_sum_xor<2>(a); lm_sum_xor<7>(a); lm_sum_xor<15>(a); lm_sum_xor<16>(a); lm_sum_xor<32>(a);
 }
 LM_FN float lm_max3(float a, float b, float c) {
   float r;
@@ -782,28 +781,91 @@ LM_FN ga_ulong lm_lane(ga_ulong k, int lane) {
          (ga_uint)__builtin_amdgcn_readlane((int)(ga_uint)k, lane);
 }
 
-/* The N elements of every lane against the list, whose k-th key is the bar: in
- * rounds, each lane offers its best element that passes the bar, until none
- * does.  Element i of a lane has the index at + (i / LM_E) * step + i % LM_E. */
-template <int N> LM_FN void lm_offer(ga_ulong &list, float (&y)[N], float most, ga_int top, ga_uint at, ga_uint step) {
-  ga_ulong bar = lm_lane(list, top - 1);
-  float bar_y = bar ? lm_key_value(bar) : -INFINITY;
-  if (__builtin_amdgcn_ballot_w64(most > bar_y || (most == bar_y && at < lm_key_index(bar) && bar)) == 0) return;
-  for (;;) {
-    int best = 0;
+/* The same network on 32-bit words: the k-th largest of 64 of them, for every lane. */
+template <int MASK> LM_FN void lm_step32(ga_uint &k) {
+  const ga_uint other = lm_xor<MASK>(k);
+  const bool lower = (LID_0 & (1u << (31 - __builtin_clz(MASK)))) == 0;
+  k = lower ? max(k, other) : min(k, other);
+}
+LM_FN ga_uint lm_kth(ga_uint k, ga_int n) {
+  lm_step32<1>(k);
+  lm_step32<3>(k); lm_step32<1>(k);
+  lm_step32<7>(k); lm_step32<2>(k); lm_step32<1>(k);
+  lm_step32<15>(k); lm_step32<4>(k); lm_step32<2>(k); lm_step32<1>(k);
+  lm_step32<31>(k); lm_step32<8>(k); lm_step32<4>(k); lm_step32<2>(k); lm_step32<1>(k);
+  lm_step32<63>(k); lm_step32<16>(k); lm_step32<8>(k); lm_step32<4>(k); lm_step32<2>(k); lm_step32<1>(k);
+  return (ga_uint)__builtin_amdgcn_readlane((int)k, n - 1);
+}
+
+/* A wavefront's best elements: a sorted list, and `n` that wait to join it, one
+ * per lane in no order.  An element that is not above `bar`, or equal to it at
+ * an index below bar_index, is none of the `top` best. */
+struct lm_best {
+  ga_ulong list, waiting;
+  ga_uint n, bar_index;
+  float bar;
+};
+LM_FN float lm_uniform(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+LM_FN void lm_settle(lm_best &b, ga_int top) {
+  if (b.n == 0) return;
+  const ga_uint lane = LID_0 & 63;
+  if (b.n <= 16) {
+    /* a few: every lane counts the keys above its own, and sends its key to that place */
+    ga_uint place = lane;
+    if (lane < b.n) place = 0;
+    for (ga_uint i = 0; i < b.n; i++) {
+      const ga_ulong k = lm_lane(b.waiting, (int)i);
+      place += lane < b.n && k > b.waiting;
+    }
+    const ga_uint lo = (ga_uint)__builtin_amdgcn_ds_permute((int)(place << 2), (int)(ga_uint)b.waiting);
+    const ga_uint hi = (ga_uint)__builtin_amdgcn_ds_permute((int)(place << 2), (int)(ga_uint)(b.waiting >> 32));
+    b.waiting = (ga_ulong)hi << 32 | lo;
+  } else {
+    lm_sort(b.waiting);
+  }
+  if (__builtin_amdgcn_ballot_w64(b.list != 0) == 0) b.list = b.waiting;
+  else lm_merge(b.list, b.waiting);
+  b.waiting = 0;
+  b.n = 0;
+  const ga_ulong k = lm_lane(b.list, top - 1);
+  if (k != 0) {
+    b.bar = lm_uniform(lm_key_value(k));
+    b.bar_index = lm_key_index(k);
+  }
+}
+/* The N elements of every lane, the largest of which is `most`.  Element i of a lane has the index
+ * at + (i / LM_E) * step + i % LM_E.  Where `top` lanes or more have one that
+ * passes the bar, the bar rises to the top-th largest of the lanes' largest:
+ * there are that many elements that are not below it.  So a first batch, or a
+ * row that rises, lets little more than `top` elements pass. */
+template <int N> LM_FN void lm_offer(lm_best &b, const float (&y)[N], float most, ga_int top, ga_uint at, ga_uint step) {
+  const ga_ulong pass = __builtin_amdgcn_ballot_w64((most > b.bar) | ((most == b.bar) & (at < b.bar_index)));
+  if (pass == 0) return;
+  if (__builtin_popcountll(pass) >= top) {
+    const float t = lm_uniform(lm_key_value((ga_ulong)lm_kth((ga_uint)(lm_key(most, 0) >> 32), top) << 32));
+    if (t > b.bar) {
+      b.bar = t;
+      b.bar_index = 0xffffffffu;
+    }
+  }
 #pragma unroll
-    for (int i = N - 1; i > 0; i--) best = y[i] == most ? i : best;
-    if (y[0] == most) best = 0;
-    const ga_ulong mine = most > -INFINITY ? lm_key(most, at + (ga_uint)(best / LM_E) * step + (ga_uint)(best % LM_E)) : 0;
-    const bool offers = mine > bar;
-    if (__builtin_amdgcn_ballot_w64(offers) == 0) return;
-    ga_ulong k = offers ? mine : 0;
-    lm_sort(k);
-    lm_merge(list, k);
-    bar = lm_lane(list, top - 1);
-#pragma unroll
-    for (int i = 0; i < N; i++) y[i] = offers && i == best ? -INFINITY : y[i];
-    most = lm_max_of(y, -INFINITY);
+  for (int i = 0; i < N; i++) {
+    ga_ulong hits = __builtin_amdgcn_ballot_w64(y[i] >= b.bar);
+    if (hits == 0) continue;
+    const ga_uint index = at + (ga_uint)(i / LM_E) * step + (ga_uint)(i % LM_E);
+    hits = __builtin_amdgcn_ballot_w64((y[i] > b.bar) | ((y[i] == b.bar) & (index < b.bar_index)));
+    const ga_ulong key = lm_key(y[i], index);
+    while (hits != 0) {
+      const int from = __builtin_ctzll(hits);
+      hits &= hits - 1;
+      if (b.n == 64) lm_settle(b, top);
+      const ga_ulong k = lm_lane(key, from);
+      const bool mine = (LID_0 & 63) == b.n;
+      b.waiting = mine ? k : b.waiting;
+      b.n = (ga_uint)__builtin_amdgcn_readfirstlane((int)(b.n + 1));
+    }
   }
 }
 
@@ -870,6 +932,7 @@ LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a
 /* The statistics and lists of a group's wavefronts meet in the first one. */
 #define LM_WAVES (LM_LANES / 64)
 LM_FN void lm_join_group(lm_state &a, ga_ulong &list, float by) {
+  (void)list;
 #if LM_WAVES > 1
   LOCAL_MEM lm_state states[LM_WAVES];
   const ga_uint wave = LID_0 >> 6, lane = LID_0 & 63;
@@ -888,12 +951,14 @@ LM_FN void lm_join_group(lm_state &a, ga_ulong &list, float by) {
 #endif
 }
 
-template <int N> LM_FN void lm_take(lm_state &a, ga_ulong &list, float (&y)[N], const lm_logprobs &p, ga_uint at, ga_uint step) {
+template <int N> LM_FN void lm_take(lm_state &a, lm_best &best, const float (&y)[N], const lm_logprobs &p, ga_uint at, ga_uint step) {
   const float most = lm_max_of(y, LM_LOWEST);
   lm_add(a, y, most, p.by);
 #if LM_TOP
   /* (a lane with -inf alone offers nothing: its largest must not pass for LM_LOWEST) */
-  lm_offer(list, y, most > LM_LOWEST ? most : lm_max_of(y, -INFINITY), p.top, at, step);
+  float largest = most;
+  if (__builtin_amdgcn_ballot_w64(!(most > LM_LOWEST)) != 0) largest = lm_max_of(y, -INFINITY);
+  lm_offer(best, y, largest, p.top, at, step);
 #endif
 }
 
@@ -905,7 +970,7 @@ template <int N> LM_FN void lm_take(lm_state &a, ga_ulong &list, float (&y)[N], 
  * and after the last whole chunk go one to a lane. */
 KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(const lm_logprobs p) {
 #if LM_LANES < 256
-  const ga_long r = (ga_long)GID_0 * (256 / LM_LANES) + (LID_0 / LM_LANES);
+  const ga_long r = (ga_long)GID_0 * (256 / LM_LANES) + __builtin_amdgcn_readfirstlane((int)(LID_0 / LM_LANES));
   if (r >= p.t) return;
   const ga_uint lane = LID_0 % LM_LANES;
 #else
@@ -936,7 +1001,7 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
 #endif
   const ga_uint minus_inf = lm_minus_inf(LM_X());
   lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
-  ga_ulong list = 0;
+  lm_best best = {0, 0, 0, 0, -INFINITY};
   lm_u4 raw[LM_U];
   const auto fetch = [&](ga_uint base) {   /* unconditional loads: all of them in flight */
     if (base + LM_U * LM_LANES <= to) {
@@ -957,12 +1022,6 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
     }
   };
   if (from < to) fetch(from);
-  if (piece == 0 && lane < 64 && v != chunks * LM_E) {
-    float y[1] = {-INFINITY};
-    ga_uint c = lane < head ? lane : tail0 + (lane - head);
-    if (c < v) y[0] = lm_get(x[c]);
-    lm_take(a, list, y, p, c, 0);
-  }
   for (ga_uint base = from; base < to; base += LM_U * LM_LANES) {
     const ga_uint at = head + (base + lane) * LM_E;
     if (base + (lane & ~63u) + LM_LANES < to) {
@@ -970,14 +1029,23 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
 #pragma unroll
       for (int u = 0; u < LM_U; u++) lm_unpack(raw[u], y + u * LM_E, LM_X());
       if (base + LM_U * LM_LANES < to) fetch(base + LM_U * LM_LANES);
-      lm_take(a, list, y, p, at, LM_LANES * LM_E);
+      lm_take(a, best, y, p, at, LM_LANES * LM_E);
     } else {          /* the last ones: no more than one chunk for any lane of this wavefront */
       float y[LM_E];
       lm_unpack(raw[0], y, LM_X());
-      lm_take(a, list, y, p, at, LM_LANES * LM_E);
+      lm_take(a, best, y, p, at, LM_LANES * LM_E);
     }
   }
+  /* (last, so that the bar of the alternatives comes from a full batch) */
+  if (piece == 0 && lane < 64 && v != chunks * LM_E) {
+    float y[1] = {-INFINITY};
+    ga_uint c = lane < head ? lane : tail0 + (lane - head);
+    if (c < v) y[0] = lm_get(x[c]);
+    lm_take(a, best, y, p, c, 0);
+  }
   lm_join_wave(a, p.by);
+  lm_settle(best, p.top);
+  ga_ulong list = best.list;
   lm_join_group(a, list, p.by);
   if (LID_0 >= 64 && LM_WAVES > 1) return;
 #if LM_SPLIT
