@@ -70,7 +70,8 @@ struct logprobs_args {
   int64_t t, v, ignore;
   float scale, by;
   int32_t top, top_long;
-  uint32_t pieces, piece_chunks, partial_bytes;
+  uint32_t pieces, piece_chunks, partial_bytes, pad;
+  void *counters;
 };
 // What the variant of the log probability kernels is specialised on: the lanes
 // of a row, the entropy, the alternatives, rows in pieces.
@@ -92,6 +93,7 @@ struct tensors_args {
   uint32_t partial0, npartials;
   int32_t n, norm_double;
   uint32_t piece, in_place;
+  void *counter;
   const void *in[LM_TENSORS];
   void *out[LM_TENSORS];
   int64_t count[LM_TENSORS];
@@ -552,7 +554,10 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
   gpudata *errbuf = nullptr;
   char *scratch = nullptr;
   int err = lm_kernel(ctx, var, "lm_logprobs_rows", sizeof(logprobs_args), &k);
-  if (err == GA_NO_ERROR && split) err = lm_kernel(ctx, var, "lm_logprobs_join", sizeof(logprobs_args), &kjoin);
+  // the last piece of a row joins them, or, where there are no counters, a second launch does
+  gpudata *counters = split && t <= ga_hip_redux_counters_max ? ga_hip_redux_counters(ctx) : nullptr;
+  if (err == GA_NO_ERROR && split && counters == nullptr)
+    err = lm_kernel(ctx, var, "lm_logprobs_join", sizeof(logprobs_args), &kjoin);
   if (err == GA_NO_ERROR && split) err = lm_scratch(ctx, t * pieces * partial_bytes, &scratch);
   if (err == GA_NO_ERROR) err = lm_errbuf(ctx, logits, &errbuf);
   if (err != GA_NO_ERROR) return err;
@@ -564,10 +569,10 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
                      step(top_ids, 1), (int64_t)t, (int64_t)v, ignore, (float)scale,
                      (float)((double)(float)scale * 1.4426950408889634), (int32_t)top,
                      top_ids != nullptr && top_ids->typecode == GA_LONG, (uint32_t)pieces, (uint32_t)piece_chunks,
-                     (uint32_t)partial_bytes};
+                     (uint32_t)partial_bytes, 0, counters ? counters->devptr : nullptr};
   if (split) {
     err = lm_launch(k, t * pieces, lanes, &a);
-    if (err == GA_NO_ERROR) err = lm_launch(kjoin, t, lanes, &a);
+    if (err == GA_NO_ERROR && counters == nullptr) err = lm_launch(kjoin, t, lanes, &a);
   } else {
     err = lanes < 256 ? lm_launch(k, (t + 3) / 4, 256, &a) : lm_launch(k, t, lanes, &a);
   }
@@ -709,7 +714,8 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
   GpuKernel *kpieces = nullptr, *kfinal = nullptr, *kclip = nullptr;
   const lm_variant vn(LM_NORM, GA_FLOAT, GA_FLOAT, GA_INT, 0), vc(LM_CLIP, GA_FLOAT, GA_FLOAT, GA_INT, 0);
   int err = lm_kernel(ctx, vn, "lm_norm_pieces", sizeof(tensors_args), &kpieces);
-  if (err == GA_NO_ERROR) err = lm_kernel(ctx, vn, "lm_norm_final", sizeof(tensors_args), &kfinal);
+  gpudata *counters = n != 0 ? ga_hip_redux_counters(ctx) : nullptr;
+  bool finished = false;
   if (err == GA_NO_ERROR && rs != nullptr) err = lm_kernel(ctx, vc, "lm_clip_pieces", sizeof(tensors_args), &kclip);
   if (err == GA_NO_ERROR) err = lm_scratch(ctx, 256 + (tables + 1) * max_groups * sizeof(double), &scratch);
   if (err != GA_NO_ERROR) return err;
@@ -747,19 +753,33 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
         a.n++;
       }
       if (a.n == 0) break;
-      const int e = launch(a.first[a.n]);
+      bool more = false;   // any element in the arrays that are left
+      for (size_t j = i; j < n && !more; j++) {
+        more = true;
+        for (unsigned d = 0; d < as[j]->nd; d++) more = more && as[j]->dimensions[d] != 0;
+      }
+      const int e = launch(a.first[a.n], !more);
       if (e != GA_NO_ERROR) return e;
     }
     return GA_NO_ERROR;
   };
-  err = for_tables([&](size_t pieces) -> int {
+  // Up to two groups for each compute unit of the last table finish the norm
+  // themselves; more of them would wait for one another's counting longer than
+  // a launch takes.
+  err = for_tables([&](size_t pieces, bool last) -> int {
     const size_t groups = std::min(pieces, max_groups);
     a.partial0 = a.npartials;
     a.npartials += (uint32_t)groups;
+    finished = last && counters != nullptr && groups <= 512;
+    a.counter = finished ? counters->devptr : nullptr;
     return lm_launch(kpieces, groups, 256, &a);
   });
-  if (err == GA_NO_ERROR) err = lm_launch(kfinal, 1, 1024, &a);
-  if (err == GA_NO_ERROR && rs != nullptr) err = for_tables([&](size_t pieces) { return lm_launch(kclip, pieces, 256, &a); });
+  if (err == GA_NO_ERROR && !finished) {
+    err = lm_kernel(ctx, vn, "lm_norm_final", sizeof(tensors_args), &kfinal);
+    if (err == GA_NO_ERROR) err = lm_launch(kfinal, 1, 1024, &a);
+  }
+  if (err == GA_NO_ERROR && rs != nullptr)
+    err = for_tables([&](size_t pieces, bool) { return lm_launch(kclip, pieces, 256, &a); });
   return err;
 }
 

@@ -64,6 +64,26 @@ template <int MASK> LM_FN ga_ulong lm_xor(ga_ulong v) {
   return (ga_ulong)lm_xor<MASK>((ga_uint)(v >> 32)) << 32 | lm_xor<MASK>((ga_uint)v);
 }
 
+/* ---- the group that finishes last finishes the call ---------------------------------
+ * Few groups leave partial results with device-scope stores, wait until those
+ * are acknowledged (past the L2 of their die) and count themselves in; the one
+ * that completes the count fetches all of them, in fixed order, with device-scope
+ * loads, and zeroes the counter.  Nobody waits for anybody. */
+template <class T> LM_FN void lm_publish(GLOBAL_MEM T *p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class T> LM_FN T lm_fetch(GLOBAL_MEM const T *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+/* by the lane, or the wavefront, that published; true for the last of `total` */
+LM_FN bool lm_count_in(GLOBAL_MEM ga_uint *counter, ga_uint total) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == total;
+  if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("" ::: "memory");
+  return last;
+}
+
 /* ---- 16-byte chunks of a row -------------------------------------------------- */
 typedef ga_uint lm_u4 __attribute__((ext_vector_type(4)));
 #define LM_E (16 / (int)sizeof(LM_X))   /* elements of a chunk */
@@ -635,6 +655,8 @@ struct lm_logprobs {
   float scale, by;               /* by = scale * log2(e) */
   ga_int top, top_long;
   ga_uint pieces, piece_chunks, partial_bytes;
+  ga_uint pad;
+  GLOBAL_MEM ga_uint *counters;  /* one zero per row, or NULL: lm_logprobs_join follows */
 };
 
 /* Softmax statistics of some elements x of a row.  With R(m) = by * m, rounded,
@@ -962,6 +984,44 @@ template <int N> LM_FN void lm_take(lm_state &a, lm_best &best, const float (&y)
 #endif
 }
 
+#if LM_SPLIT
+/* The pieces of row r: a piece's statistics to a lane and its list to a
+ * wavefront at a time, in fixed order. */
+LM_FN void lm_join_pieces(const lm_logprobs &p, ga_long r) {
+  const ga_uint wave = LID_0 >> 6, lane = LID_0 & 63;
+  GLOBAL_MEM const char *from = p.partials + (ga_size)r * p.pieces * p.partial_bytes;
+  lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
+  ga_ulong list = 0;
+  for (ga_uint i = LID_0; i < p.pieces; i += LM_LANES) {
+    GLOBAL_MEM const ga_ulong *words = (GLOBAL_MEM const ga_ulong *)(from + (ga_size)i * p.partial_bytes);
+    const ga_ulong ms = lm_fetch(words), w = lm_fetch(words + 1);
+    const lm_state b = {__builtin_bit_cast(float, (ga_uint)ms), __builtin_bit_cast(float, (ga_uint)(ms >> 32)),
+                        __builtin_bit_cast(float, (ga_uint)w), 0.0f};
+    lm_join(a, b, p.by);
+  }
+  lm_join_wave(a, p.by);
+#if LM_TOP
+  /* eight lists at a time, so that their loads are in flight together */
+  for (ga_uint i0 = wave; i0 < p.pieces; i0 += 8 * LM_WAVES) {
+    ga_ulong k[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const ga_uint i = i0 + u * LM_WAVES;
+      const ga_ulong v = lm_fetch((GLOBAL_MEM const ga_ulong *)(from + (ga_size)(i < p.pieces ? i : i0) * p.partial_bytes) + 2 +
+                                  (lane < p.top ? lane : 0));
+      k[u] = i < p.pieces && lane < p.top ? v : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (i0 + u * LM_WAVES < p.pieces) lm_merge(list, k[u]);
+  }
+#endif
+  local_barrier();   /* (the group's LDS is free again) */
+  lm_join_group(a, list, p.by);
+  if (wave == 0) lm_logprobs_finish(p, r, a, list);
+}
+#endif
+
 #define LM_U (16 / LM_E)   /* chunks of a lane at a time: 16 elements */
 
 /* LM_LANES lanes share a row, or one of its pieces (LM_SPLIT): a loop over
@@ -1047,39 +1107,33 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
   lm_settle(best, p.top);
   ga_ulong list = best.list;
   lm_join_group(a, list, p.by);
-  if (LID_0 >= 64 && LM_WAVES > 1) return;
 #if LM_SPLIT
-  GLOBAL_MEM char *to_p = p.partials + (ga_size)GID_0 * p.partial_bytes;
-  if (lane == 0) *(GLOBAL_MEM lm_state *)to_p = a;
+  if (LID_0 < 64) {
+    GLOBAL_MEM char *mine = p.partials + (ga_size)GID_0 * p.partial_bytes;
+    GLOBAL_MEM ga_ulong *words = (GLOBAL_MEM ga_ulong *)mine;
+    if (lane == 0) {
+      lm_publish(words, (ga_ulong)__builtin_bit_cast(ga_uint, a.s) << 32 | __builtin_bit_cast(ga_uint, a.m));
+      lm_publish(words + 1, (ga_ulong)__builtin_bit_cast(ga_uint, a.w));
+    }
 #if LM_TOP
-  if (lane < p.top) ((GLOBAL_MEM ga_ulong *)(to_p + sizeof(lm_state)))[lane] = list;
+    if (lane < p.top) lm_publish(words + 2 + lane, list);
 #endif
+  }
+  if (p.counters == nullptr) return;
+  LOCAL_MEM ga_uint last;
+  if (LID_0 < 64) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   /* (of every lane of the wavefront) */
+    if (lane == 0) last = lm_count_in(p.counters + r, p.pieces);
+  }
+  local_barrier();
+  if (last) lm_join_pieces(p, r);
 #else
-  lm_logprobs_finish(p, r, a, list);
+  if (LID_0 < 64 || LM_WAVES == 1) lm_logprobs_finish(p, r, a, list);
 #endif
 }
 
 #if LM_SPLIT
-/* The pieces of a row: a group per row, a piece's statistics to a lane and
- * its list to a wavefront at a time, in fixed order. */
-KERNEL void __launch_bounds__(LM_LANES) lm_logprobs_join(const lm_logprobs p) {
-  const ga_long r = GID_0;
-  const ga_uint wave = LID_0 >> 6, lane = LID_0 & 63;
-  GLOBAL_MEM const char *from = p.partials + (ga_size)r * p.pieces * p.partial_bytes;
-  lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
-  ga_ulong list = 0;
-  for (ga_uint i = LID_0; i < p.pieces; i += LM_LANES)
-    lm_join(a, *(GLOBAL_MEM const lm_state *)(from + (ga_size)i * p.partial_bytes), p.by);
-  lm_join_wave(a, p.by);
-#if LM_TOP
-  for (ga_uint i = wave; i < p.pieces; i += LM_WAVES) {
-    const ga_ulong k = lane < p.top ? ((GLOBAL_MEM const ga_ulong *)(from + (ga_size)i * p.partial_bytes + sizeof(lm_state)))[lane] : 0;
-    lm_merge(list, k);
-  }
-#endif
-  lm_join_group(a, list, p.by);
-  if (wave == 0) lm_logprobs_finish(p, r, a, list);
-}
+KERNEL void __launch_bounds__(LM_LANES) lm_logprobs_join(const lm_logprobs p) { lm_join_pieces(p, GID_0); }
 #endif
 #endif
 
@@ -1197,6 +1251,7 @@ struct lm_tensors {
   ga_uint partial0, npartials;
   ga_int n, norm_double;
   ga_uint piece, in_place;
+  GLOBAL_MEM ga_uint *counter;   /* a zero that the last table's groups count on, or NULL: lm_norm_final follows */
   GLOBAL_MEM const void *in[LM_TENSORS];
   GLOBAL_MEM void *out[LM_TENSORS];
   ga_long count[LM_TENSORS];
@@ -1295,6 +1350,22 @@ template <class T> LM_FN double lm_squares(GLOBAL_MEM const T *x, ga_long n, ga_
   }
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
+/* The norm and the factor from all partial sums, by one group. */
+template <int LANES> LM_FN void lm_norm_of_partials(const lm_tensors &p) {
+  double s = 0.0;
+  for (ga_uint k = LID_0; k < p.npartials; k += LANES)
+    s += __builtin_bit_cast(double, lm_fetch((GLOBAL_MEM const ga_ulong *)p.partials + k));
+  local_barrier();   /* (the LDS of an earlier sum is free again) */
+  s = lm_group_sum<LANES / 64>(s);
+  if (LID_0 == 0) {
+    const double norm = __builtin_sqrt(s);
+    p.result[0] = norm > p.max_norm && norm < (double)INFINITY ? p.max_norm / norm : 1.0;
+    if (p.norm != nullptr) {
+      if (p.norm_double) *(GLOBAL_MEM double *)p.norm = norm;
+      else *(GLOBAL_MEM float *)p.norm = (float)norm;
+    }
+  }
+}
 /* A group adds every GDIM_0-th piece. */
 KERNEL void __launch_bounds__(LM_GROUP) lm_norm_pieces(const lm_tensors p) {
   double s = 0.0;
@@ -1310,21 +1381,15 @@ KERNEL void __launch_bounds__(LM_GROUP) lm_norm_pieces(const lm_tensors p) {
     LM_BY_TYPE(p.type[i], LM_SQUARES)
   }
   s = lm_group_sum<LM_GROUP / 64>(s);
-  if (LID_0 == 0) p.partials[p.partial0 + GID_0] = s;
-}
-KERNEL void __launch_bounds__(1024) lm_norm_final(const lm_tensors p) {
-  double s = 0.0;
-  for (ga_uint k = LID_0; k < p.npartials; k += 1024) s += p.partials[k];
-  s = lm_group_sum<16>(s);
+  LOCAL_MEM ga_uint last;
   if (LID_0 == 0) {
-    const double norm = __builtin_sqrt(s);
-    p.result[0] = norm > p.max_norm && norm < (double)INFINITY ? p.max_norm / norm : 1.0;
-    if (p.norm != nullptr) {
-      if (p.norm_double) *(GLOBAL_MEM double *)p.norm = norm;
-      else *(GLOBAL_MEM float *)p.norm = (float)norm;
-    }
+    lm_publish((GLOBAL_MEM ga_ulong *)p.partials + p.partial0 + GID_0, __builtin_bit_cast(ga_ulong, s));
+    last = p.counter != nullptr && lm_count_in(p.counter, GDIM_0);
   }
+  local_barrier();
+  if (last) lm_norm_of_partials<LM_GROUP>(p);
 }
+KERNEL void __launch_bounds__(1024) lm_norm_final(const lm_tensors p) { lm_norm_of_partials<1024>(p); }
 #endif
 
 #if LM_KIND == LM_K_CLIP
