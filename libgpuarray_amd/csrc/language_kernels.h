@@ -764,25 +764,40 @@ template <int N> LM_FN void lm_add(lm_state &a, const float (&y)[N], float most,
 
 /* ---- the alternatives -----------------------------------------------------------
  * A wavefront keeps its best 64 elements as keys, sorted, one per lane: the
- * upper half orders the values (-0 as 0), the lower one prefers low indices;
- * 0 is no element.  -inf is never kept: what is missing in the end is filled
- * up by a look at the row. */
+ * upper 32 of a key's 62 bits order the values (-0 as 0), the lower 30 prefer
+ * low indices; 0 is no element.  Keys of 62 bits are ordered as the doubles below 2 that
+ * have these bits, so that a comparison and its two outcomes are the maximum
+ * and the minimum of two doubles, with no way through a scalar mask.
+ * -inf is never kept: what is missing in the end is filled up by a look at the row. */
+#define LM_INDEX 0x3fffffffu
 LM_FN ga_ulong lm_key(float y, ga_uint index) {
   const ga_uint b = __builtin_bit_cast(ga_uint, y + 0.0f);
-  return (ga_ulong)(b ^ ((ga_uint)((ga_int)b >> 31) | 0x80000000u)) << 32 | (0xffffffffu - index);
+  const ga_uint o = b ^ ((ga_uint)((ga_int)b >> 31) | 0x80000000u);
+  return (ga_ulong)(o >> 2) << 32 | (o << 30 | (LM_INDEX - index));
 }
 LM_FN float lm_key_value(ga_ulong k) {
-  const ga_uint b = (ga_uint)(k >> 32);
+  const ga_uint b = (ga_uint)(k >> 30);
   return __builtin_bit_cast(float, b ^ ((b & 0x80000000u) ? 0x80000000u : 0xffffffffu));
 }
-LM_FN ga_uint lm_key_index(ga_ulong k) { return 0xffffffffu - (ga_uint)k; }
+LM_FN ga_uint lm_key_index(ga_ulong k) { return LM_INDEX - ((ga_uint)k & LM_INDEX); }
+LM_FN ga_ulong lm_larger(ga_ulong a, ga_ulong b) {
+  double r;
+  asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(__builtin_bit_cast(double, a)), "v"(__builtin_bit_cast(double, b)));
+  return __builtin_bit_cast(ga_ulong, r);
+}
+LM_FN ga_ulong lm_smaller(ga_ulong a, ga_ulong b) {
+  double r;
+  asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(__builtin_bit_cast(double, a)), "v"(__builtin_bit_cast(double, b)));
+  return __builtin_bit_cast(ga_ulong, r);
+}
 
 /* one step of a sorting network: of lane and lane ^ MASK the lower one keeps the larger key */
 template <int MASK> LM_FN void lm_step(ga_ulong &k) {
   const ga_ulong other = lm_xor<MASK>(k);
   const ga_uint top_bit = 1u << (31 - __builtin_clz(MASK));
   const bool lower = (LID_0 & top_bit) == 0;
-  k = (k > other) == lower ? k : other;
+  const ga_ulong l = lm_larger(k, other), s = lm_smaller(k, other);
+  k = lower ? l : s;
 }
 LM_FN void lm_sort(ga_ulong &k) {   /* descending over the 64 lanes */
   lm_step<1>(k);
@@ -795,7 +810,7 @@ LM_FN void lm_sort(ga_ulong &k) {   /* descending over the 64 lanes */
 /* list := the best 64 of two sorted lists, sorted */
 LM_FN void lm_merge(ga_ulong &list, ga_ulong other) {
   const ga_ulong r = lm_xor<63>(other);
-  list = list > r ? list : r;
+  list = lm_larger(list, r);
   lm_step<32>(list); lm_step<16>(list); lm_step<8>(list); lm_step<4>(list); lm_step<2>(list); lm_step<1>(list);
 }
 LM_FN ga_ulong lm_lane(ga_ulong k, int lane) {
@@ -857,42 +872,95 @@ LM_FN void lm_settle(lm_best &b, ga_int top) {
     b.bar_index = lm_key_index(k);
   }
 }
+/* The wavefronts of a row share the highest of their bars: `top` elements are
+ * not below it, wherever they are.  It is only ever raised, and whoever misses a
+ * rise keeps more than it needs. */
+LM_FN ga_uint lm_ordered(float y) { return (ga_uint)(lm_key(y, 0) >> 30); }
+#if LM_LANES > 64 && LM_TOP
+static LOCAL_MEM ga_uint lm_shared_bar;
+LM_FN void lm_reset_bar() {
+  if (LID_0 == 0) lm_shared_bar = lm_ordered(-INFINITY);
+  local_barrier();
+}
+LM_FN void lm_heed_bar(lm_best &b) {
+  const ga_uint s = (ga_uint)__builtin_amdgcn_readfirstlane((int)__hip_atomic_load(&lm_shared_bar, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+  const float t = lm_key_value((ga_ulong)s << 30);
+  if (t > b.bar) {
+    b.bar = t;
+    b.bar_index = LM_INDEX;
+  }
+}
+LM_FN void lm_share_bar(float bar) {
+  if ((LID_0 & 63) == 0) atomicMax(&lm_shared_bar, lm_ordered(bar));
+}
+#else
+LM_FN void lm_reset_bar() {}
+LM_FN void lm_heed_bar(lm_best &) {}
+LM_FN void lm_share_bar(float) {}
+#endif
+
 /* The N elements of every lane, the largest of which is `most`.  Element i of a lane has the index
  * at + (i / LM_E) * step + i % LM_E.  Where `top` lanes or more have one that
  * passes the bar, the bar rises to the top-th largest of the lanes' largest:
  * there are that many elements that are not below it.  So a first batch, or a
- * row that rises, lets little more than `top` elements pass. */
-template <int N> LM_FN void lm_offer(lm_best &b, const float (&y)[N], float most, ga_int top, ga_uint at, ga_uint step) {
+ * row that rises, lets little more than `top` elements pass.  Then in rounds:
+ * each lane's largest goes to wait if it passes the bar, until none does. */
+template <int N> LM_FN void lm_offer(lm_best &b, float (&y)[N], float most, ga_int top, ga_uint at, ga_uint step) {
+  const ga_uint lane = LID_0 & 63;
+  lm_heed_bar(b);
   const ga_ulong pass = __builtin_amdgcn_ballot_w64((most > b.bar) | ((most == b.bar) & (at < b.bar_index)));
   if (pass == 0) return;
   if (__builtin_popcountll(pass) >= top) {
-    const float t = lm_uniform(lm_key_value((ga_ulong)lm_kth((ga_uint)(lm_key(most, 0) >> 32), top) << 32));
+    const float t = lm_uniform(lm_key_value((ga_ulong)lm_kth(lm_ordered(most), top) << 30));
     if (t > b.bar) {
       b.bar = t;
-      b.bar_index = 0xffffffffu;
+      b.bar_index = LM_INDEX;
     }
   }
+  do {
+    int best = N - 1;
 #pragma unroll
-  for (int i = 0; i < N; i++) {
-    ga_ulong hits = __builtin_amdgcn_ballot_w64(y[i] >= b.bar);
-    if (hits == 0) continue;
-    const ga_uint index = at + (ga_uint)(i / LM_E) * step + (ga_uint)(i % LM_E);
-    hits = __builtin_amdgcn_ballot_w64((y[i] > b.bar) | ((y[i] == b.bar) & (index < b.bar_index)));
-    const ga_ulong key = lm_key(y[i], index);
-    while (hits != 0) {
-      const int from = __builtin_ctzll(hits);
-      hits &= hits - 1;
-      if (b.n == 64) lm_settle(b, top);
-      const ga_ulong k = lm_lane(key, from);
-      const bool mine = (LID_0 & 63) == b.n;
-      b.waiting = mine ? k : b.waiting;
-      b.n = (ga_uint)__builtin_amdgcn_readfirstlane((int)(b.n + 1));
-    }
-  }
+    for (int i = N - 2; i >= 0; i--) best = y[i] == most ? i : best;
+    const ga_uint index = at + (ga_uint)(best / LM_E) * step + (ga_uint)(best % LM_E);
+    const bool passes = (most > b.bar) | ((most == b.bar) & (index < b.bar_index));
+    const ga_ulong all = __builtin_amdgcn_ballot_w64(passes);
+    if (all == 0) break;
+    const ga_uint count = (ga_uint)__builtin_popcountll(all);
+    if (b.n + count > 64) lm_settle(b, top);
+    /* those that pass go to lanes n, n + 1, ..; the others behind them, all lanes round */
+    const ga_uint before = __builtin_amdgcn_mbcnt_hi((ga_uint)(all >> 32), __builtin_amdgcn_mbcnt_lo((ga_uint)all, 0));
+    const int to = (int)((b.n + (passes ? before : count + lane - before)) << 2);
+    const ga_ulong key = lm_key(most, index);
+    const ga_uint lo = (ga_uint)__builtin_amdgcn_ds_permute(to, (int)(ga_uint)key);
+    const ga_uint hi = (ga_uint)__builtin_amdgcn_ds_permute(to, (int)(ga_uint)(key >> 32));
+    if (lane - b.n < count) b.waiting = (ga_ulong)hi << 32 | lo;
+    b.n = (ga_uint)__builtin_amdgcn_readfirstlane((int)(b.n + count));
+    best = passes ? best : N;
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = best == i ? -INFINITY : y[i];
+    most = lm_max_of(y, -INFINITY);
+  } while (__builtin_amdgcn_ballot_w64(most >= b.bar) != 0);
+  lm_share_bar(b.bar);
 }
 
+/* The token of a row and its logit, which are fetched before the row is summed. */
+struct lm_token {
+  ga_long id;   /* -1: no token, -2: out of range */
+  float x;
+};
+LM_FN ga_long lm_token_id(const lm_logprobs &p, ga_long r) {
+  return p.ids != nullptr ? (ga_long)*lm_at(p.ids, r * p.id_step) : 0;
+}
+LM_FN lm_token lm_token_of(const lm_logprobs &p, ga_long r, ga_long id) {
+  lm_token k = {-1, 0.0f};
+  if (p.ids != nullptr) {
+    k.id = lm_id(id, p.ignore, LM_NONE, p.v);
+    k.x = lm_get(lm_at(p.logits, r * p.row)[k.id > 0 ? k.id : 0]);
+  }
+  return k;
+}
 /* What is written for row r; a whole wavefront. */
-LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a, ga_ulong list) {
+LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a, ga_ulong list, lm_token token) {
   const ga_uint lane = LID_0 & 63;
   const float rm = a.m * p.by;
   const bool nothing = a.s == 0.0f;
@@ -904,13 +972,12 @@ LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a
   const float ls = nothing ? -INFINITY : lg - off;
   if (lane == 0) {
     if (p.ids != nullptr) {
-      const ga_long id = lm_id((ga_long)*lm_at(p.ids, r * p.id_step), p.ignore, LM_NONE, p.v);
       float lp = 0.0f;
-      if (id == -2) {
+      if (token.id == -2) {
         *p.err = -1;
         lp = NAN;
-      } else if (id >= 0) {
-        lp = nothing ? -INFINITY : (lm_get(lm_at(p.logits, r * p.row)[id]) - m) * p.scale - ls;
+      } else if (token.id >= 0) {
+        lp = nothing ? -INFINITY : (token.x - m) * p.scale - ls;
         if (ls != ls) lp = NAN;
       }
       *lm_at(p.logp, r * p.logp_step) = lp;
@@ -973,7 +1040,7 @@ LM_FN void lm_join_group(lm_state &a, ga_ulong &list, float by) {
 #endif
 }
 
-template <int N> LM_FN void lm_take(lm_state &a, lm_best &best, const float (&y)[N], const lm_logprobs &p, ga_uint at, ga_uint step) {
+template <int N> LM_FN void lm_take(lm_state &a, lm_best &best, float (&y)[N], const lm_logprobs &p, ga_uint at, ga_uint step) {
   const float most = lm_max_of(y, LM_LOWEST);
   lm_add(a, y, most, p.by);
 #if LM_TOP
@@ -992,33 +1059,43 @@ LM_FN void lm_join_pieces(const lm_logprobs &p, ga_long r) {
   GLOBAL_MEM const char *from = p.partials + (ga_size)r * p.pieces * p.partial_bytes;
   lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
   ga_ulong list = 0;
+  /* Every load has a long way: all of them go out before the first is used. */
+  const ga_long token_id = lm_token_id(p, r);
+  const auto word = [&](ga_uint i, ga_uint place) {
+    return lm_fetch((GLOBAL_MEM const ga_ulong *)(from + (ga_size)(i < p.pieces ? i : 0) * p.partial_bytes) + place);
+  };
+  ga_ulong ms = word(LID_0, 0), ws = word(LID_0, 1);
+#if LM_TOP
+  const ga_uint place = 2 + (lane < p.top ? lane : 0);
+  ga_ulong k[8];     /* the lists: pieces wave, wave + LM_WAVES, .. to each wavefront */
+#pragma unroll
+  for (int u = 0; u < 8; u++) k[u] = word(wave + u * LM_WAVES, place);
+#endif
+  const lm_token token = lm_token_of(p, r, token_id);
   for (ga_uint i = LID_0; i < p.pieces; i += LM_LANES) {
-    GLOBAL_MEM const ga_ulong *words = (GLOBAL_MEM const ga_ulong *)(from + (ga_size)i * p.partial_bytes);
-    const ga_ulong ms = lm_fetch(words), w = lm_fetch(words + 1);
+    if (i != LID_0) {
+      ms = word(i, 0);
+      ws = word(i, 1);
+    }
     const lm_state b = {__builtin_bit_cast(float, (ga_uint)ms), __builtin_bit_cast(float, (ga_uint)(ms >> 32)),
-                        __builtin_bit_cast(float, (ga_uint)w), 0.0f};
+                        __builtin_bit_cast(float, (ga_uint)ws), 0.0f};
     lm_join(a, b, p.by);
   }
   lm_join_wave(a, p.by);
 #if LM_TOP
-  /* eight lists at a time, so that their loads are in flight together */
   for (ga_uint i0 = wave; i0 < p.pieces; i0 += 8 * LM_WAVES) {
-    ga_ulong k[8];
+    if (i0 != wave) {
 #pragma unroll
-    for (int u = 0; u < 8; u++) {
-      const ga_uint i = i0 + u * LM_WAVES;
-      const ga_ulong v = lm_fetch((GLOBAL_MEM const ga_ulong *)(from + (ga_size)(i < p.pieces ? i : i0) * p.partial_bytes) + 2 +
-                                  (lane < p.top ? lane : 0));
-      k[u] = i < p.pieces && lane < p.top ? v : 0;
+      for (int u = 0; u < 8; u++) k[u] = word(i0 + u * LM_WAVES, place);
     }
 #pragma unroll
     for (int u = 0; u < 8; u++)
-      if (i0 + u * LM_WAVES < p.pieces) lm_merge(list, k[u]);
+      if (i0 + u * LM_WAVES < p.pieces) lm_merge(list, lane < p.top ? k[u] : 0);
   }
 #endif
   local_barrier();   /* (the group's LDS is free again) */
   lm_join_group(a, list, p.by);
-  if (wave == 0) lm_logprobs_finish(p, r, a, list);
+  if (wave == 0) lm_logprobs_finish(p, r, a, list, token);
 }
 #endif
 
@@ -1062,6 +1139,9 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
   const ga_uint minus_inf = lm_minus_inf(LM_X());
   lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
   lm_best best = {0, 0, 0, 0, -INFINITY};
+#if !LM_SPLIT
+  const ga_long token_id = lm_token_id(p, r);
+#endif
   lm_u4 raw[LM_U];
   const auto fetch = [&](ga_uint base) {   /* unconditional loads: all of them in flight */
     if (base + LM_U * LM_LANES <= to) {
@@ -1082,6 +1162,10 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
     }
   };
   if (from < to) fetch(from);
+  lm_reset_bar();
+#if !LM_SPLIT
+  const lm_token token = lm_token_of(p, r, token_id);
+#endif
   for (ga_uint base = from; base < to; base += LM_U * LM_LANES) {
     const ga_uint at = head + (base + lane) * LM_E;
     if (base + (lane & ~63u) + LM_LANES < to) {
@@ -1128,7 +1212,7 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
   local_barrier();
   if (last) lm_join_pieces(p, r);
 #else
-  if (LID_0 < 64 || LM_WAVES == 1) lm_logprobs_finish(p, r, a, list);
+  if (LID_0 < 64 || LM_WAVES == 1) lm_logprobs_finish(p, r, a, list, token);
 #endif
 }
 
