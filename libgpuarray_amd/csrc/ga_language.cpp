@@ -55,10 +55,13 @@ struct embed_grad_args {
   void *grad;
   const void *dout, *key, *order;
   void *partials;
+  const void *ids;
+  void *err;
+  int64_t id_step, ignore;
   int64_t grad_row, dout_row, v, d;
   float scale;
   int32_t accumulate;
-  uint32_t n, chunk, chunks, tiles;
+  uint32_t n, chunk, chunks, tiles, rows;
 };
 struct logprobs_args {
   const void *logits, *ids;
@@ -385,6 +388,22 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   const size_t osize = gpuarray_get_elsize(grad->typecode);
   const size_t cols = 64 * 16 / gpuarray_get_elsize(dout->typecode);   // of a wavefront
   const size_t tiles = (d + cols - 1) / cols;
+  const lm_variant vg(LM_EMBED_GRAD, dout->typecode, grad->typecode, ids->typecode, 0);
+  gpudata *errbuf = nullptr;
+  embed_grad_args a = {at(grad), at(dout), nullptr, nullptr, nullptr, at(ids), nullptr, ids->strides[0], ignore,
+                       grad->strides[0], dout->strides[0], (int64_t)v, (int64_t)d, (float)scale, accumulate != 0,
+                       (uint32_t)n, 0, 0, (uint32_t)tiles, (uint32_t)(16 / std::min<size_t>(tiles, 4))};
+  int err = lm_errbuf(ctx, grad, &errbuf);
+  if (err != GA_NO_ERROR) return err;
+  a.err = errbuf->devptr;
+  if (n <= 256) {
+    GpuKernel *kfew = nullptr;
+    err = lm_kernel(ctx, vg, "lm_embed_grad_few", sizeof(embed_grad_args), &kfew);
+    const size_t parts = (tiles + 3) / 4, row_groups = v ? (v + a.rows - 1) / a.rows : 1;
+    if (parts > MAX_GROUPS / row_groups) return c.fail(GA_XLARGE_ERROR, "too many elements");
+    if (err == GA_NO_ERROR) err = lm_launch(kfew, row_groups * parts, 256, &a);
+    return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
+  }
   // Tokens of a chunk: enough chunks to fill the chip with wavefronts, and
   // not so few tokens that partial sums (two rows a chunk at most) count.
   size_t chunk = 8;
@@ -407,11 +426,8 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   const size_t counts = small ? 0 : (((groups + 1) << bits) * 4 + 255) & ~(size_t)255;
   const size_t partials = chunks * 2 * tiles * cols * 4;
   char *scratch = nullptr;
-  gpudata *errbuf = nullptr;
   GpuKernel *ksmall = nullptr, *kcount = nullptr, *kscan = nullptr, *kmove = nullptr, *ksum = nullptr, *kjoin = nullptr;
   const lm_variant vs(LM_SORT, GA_FLOAT, GA_FLOAT, ids->typecode, items);
-  const lm_variant vg(LM_EMBED_GRAD, dout->typecode, grad->typecode, GA_INT, 0);
-  int err = GA_NO_ERROR;
   if (small) {
     err = lm_kernel(ctx, vs, "lm_sort_small", sizeof(sorting_args), &ksmall);
   } else {
@@ -422,7 +438,6 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   if (err == GA_NO_ERROR) err = lm_kernel(ctx, vg, "lm_embed_grad_sum", sizeof(embed_grad_args), &ksum);
   if (err == GA_NO_ERROR) err = lm_kernel(ctx, vg, "lm_embed_grad_join", sizeof(embed_grad_args), &kjoin);
   if (err == GA_NO_ERROR) err = lm_scratch(ctx, 4 * list + counts + partials + 256, &scratch);
-  if (err == GA_NO_ERROR) err = lm_errbuf(ctx, grad, &errbuf);
   if (err != GA_NO_ERROR) return err;
 
   char *lists[4] = {scratch, scratch + list, scratch + 2 * list, scratch + 3 * list};
@@ -476,9 +491,11 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
     }
   }
   if (err == GA_NO_ERROR && n > 0) {
-    embed_grad_args a = {at(grad), at(dout), s.key, s.order, scratch + 4 * list + counts, grad->strides[0],
-                         dout->strides[0], (int64_t)v, (int64_t)d, (float)scale, accumulate != 0, (uint32_t)n,
-                         (uint32_t)chunk, (uint32_t)chunks, (uint32_t)tiles};
+    a.key = s.key;
+    a.order = s.order;
+    a.partials = scratch + 4 * list + counts;
+    a.chunk = (uint32_t)chunk;
+    a.chunks = (uint32_t)chunks;
     err = lm_launch(ksum, (chunks * tiles + 3) / 4, 256, &a);
     if (err == GA_NO_ERROR && chunks > 1) err = lm_launch(kjoin, chunks * tiles, 256, &a);
   }

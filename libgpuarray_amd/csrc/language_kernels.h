@@ -156,7 +156,9 @@ template <int N, class T> LM_FN void lm_store(GLOBAL_MEM T *p, const float (&y)[
 #pragma unroll
     for (int i = 0; i < words; i += 4) {
       const lm_u4a q = {w[i], w[i + 1], w[i + 2], w[i + 3]};
-      __builtin_nontemporal_store(q, (GLOBAL_MEM lm_u4a *)(p + i * 4 / (int)sizeof(T)));
+      /* two halves of 32 bytes are put together by the L2, which a streamed store passes by */
+      if constexpr (words == 4) __builtin_nontemporal_store(q, (GLOBAL_MEM lm_u4a *)(p + i * 4 / (int)sizeof(T)));
+      else *(GLOBAL_MEM lm_u4a *)(p + i * 4 / (int)sizeof(T)) = q;
     }
   }
 }
@@ -471,10 +473,13 @@ struct lm_embed_grad {
   GLOBAL_MEM const LM_X *dout;
   GLOBAL_MEM const ga_uint *key, *order;   /* the sorted tokens */
   GLOBAL_MEM float *partials;              /* [chunk][2][tiles * 64 * LM_E] */
+  GLOBAL_MEM const LM_ID *ids;             /* of few tokens */
+  GLOBAL_MEM ga_int *err;
+  ga_long id_step, ignore;
   ga_long grad_row, dout_row, v, d;
   float scale;
   ga_int accumulate;
-  ga_uint n, chunk, chunks, tiles;
+  ga_uint n, chunk, chunks, tiles, rows;
 };
 
 /* The columns of a lane: LM_E from `from` on, of which the first `skip` belong
@@ -517,11 +522,87 @@ LM_FN void lm_write_run(const lm_embed_grad &p, ga_uint key, const lm_columns &c
   }
 }
 
+#define LM_AHEAD 8   /* rows in flight */
+/* the columns of rows at[..] of dout; unconditional loads: all of them in flight */
+LM_FN void lm_fetch_rows(const lm_embed_grad &p, const ga_uint (&at)[LM_AHEAD], const lm_columns &c, float (&y)[LM_AHEAD][LM_E]) {
+  if (p.d >= LM_E) {
+#pragma unroll
+    for (int u = 0; u < LM_AHEAD; u++) lm_load(lm_at(p.dout, (ga_long)at[u] * p.dout_row) + c.from, y[u]);
+  } else {
+#pragma unroll
+    for (int u = 0; u < LM_AHEAD; u++)
+#pragma unroll
+      for (int e = 0; e < LM_E; e++) y[u][e] = e < c.cols ? (float)lm_get(lm_at(p.dout, (ga_long)at[u] * p.dout_row)[e]) : 0.0f;
+  }
+}
+
+/* Few tokens need no sorting: a group takes p.rows rows of the table and up to
+ * four times 64 * LM_E columns of them (as many rows as give each of its wavefronts
+ * four pieces), looks all ids through once, which leaves a mask of the tokens of
+ * each row, and adds those in order; one launch in place of three. */
+#define LM_FEW 256        /* tokens at most */
+#define LM_FEW_ROWS 16    /* rows at most */
+KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
+  LOCAL_MEM ga_ulong masks[LM_FEW_ROWS][LM_FEW / 64];
+  const ga_uint lane = LID_0 & 63, wave = LID_0 >> 6;
+  const ga_uint parts = (p.tiles + 3) / 4, part = GID_0 % parts;
+  const ga_uint tiles = p.tiles - part * 4 < 4 ? p.tiles - part * 4 : 4;
+  const ga_long r0 = (ga_long)(GID_0 / parts) * p.rows;
+  const ga_long id = LID_0 < p.n ? lm_id((ga_long)*lm_at(p.ids, (ga_long)LID_0 * p.id_step), p.ignore, LM_NONE, p.v) : -1;
+  if (id == -2) *p.err = -1;
+  const ga_uint row = id >= r0 && id < r0 + p.rows ? (ga_uint)(id - r0) : LM_FEW_ROWS;
+  for (ga_uint k = 0; k < p.rows; k++) {
+    const ga_ulong m = __builtin_amdgcn_ballot_w64(row == k);
+    if (lane == k) masks[k][wave] = m;
+  }
+  local_barrier();
+  for (ga_uint unit = wave; unit < p.rows * tiles; unit += 4) {
+    const ga_uint k = unit / tiles, tile = part * 4 + unit % tiles;
+    if (r0 + k >= p.v) break;
+    ga_ulong left[LM_FEW / 64];
+    ga_ulong any = 0;
+#pragma unroll
+    for (int w = 0; w < LM_FEW / 64; w++) {
+      left[w] = masks[k][w];
+      left[w] = (ga_ulong)(ga_uint)__builtin_amdgcn_readfirstlane((int)(left[w] >> 32)) << 32 |
+                (ga_uint)__builtin_amdgcn_readfirstlane((int)left[w]);
+      any |= left[w];
+    }
+    if (any == 0 && p.accumulate) continue;
+    const lm_columns mine = lm_columns_of(((ga_long)tile * 64 + lane) * LM_E, p.d);
+    float sum[LM_E];
+#pragma unroll
+    for (int e = 0; e < LM_E; e++) sum[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < LM_FEW / 64; w++) {
+      while (left[w] != 0) {
+        ga_uint at[LM_AHEAD];
+        ga_uint n = 0;
+#pragma unroll
+        for (int u = 0; u < LM_AHEAD; u++) {
+          at[u] = left[w] != 0 ? w * 64 + (ga_uint)__builtin_ctzll(left[w]) : at[u > 0 ? u - 1 : 0];
+          n += left[w] != 0;
+          left[w] &= left[w] - 1;
+        }
+        float y[LM_AHEAD][LM_E];
+        lm_fetch_rows(p, at, mine, y);
+#pragma unroll
+        for (int u = 0; u < LM_AHEAD; u++) {
+          if (u < n) {
+#pragma unroll
+            for (int e = 0; e < LM_E; e++) sum[e] += y[u][e];
+          }
+        }
+      }
+    }
+    lm_write_run(p, (ga_uint)(r0 + k), mine, sum);
+  }
+}
+
 /* A wavefront adds the rows of a chunk of the sorted tokens, in their order, over
  * 64 * LM_E columns.  A run of equal ids that lies inside the chunk is written
  * when it ends; what a chunk has of a run that began earlier (slot 0), or that
  * goes on in the next (slot 1), is left for lm_embed_grad_join. */
-#define LM_AHEAD 8   /* rows in flight */
 KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
   const ga_uint unit = (ga_uint)__builtin_amdgcn_readfirstlane((int)(GID_0 * 4 + (LID_0 >> 6)));
   const ga_uint chunk = unit / p.tiles, tile = unit % p.tiles, lane = LID_0 & 63;
@@ -551,20 +632,10 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
     for (ga_uint j = 0; j < m; j += LM_AHEAD) {
       float y[LM_AHEAD][LM_E];
       ga_uint k[LM_AHEAD];
-      if (p.d >= LM_E) {     /* (unconditional loads: all of them in flight) */
+      ga_uint at[LM_AHEAD];
 #pragma unroll
-        for (int u = 0; u < LM_AHEAD; u++) {
-          const ga_uint at = (ga_uint)__builtin_amdgcn_readlane((int)places, (int)(j + u));
-          lm_load(lm_at(p.dout, (ga_long)at * p.dout_row) + mine.from, y[u]);
-        }
-      } else {
-#pragma unroll
-        for (int u = 0; u < LM_AHEAD; u++) {
-          const ga_uint at = (ga_uint)__builtin_amdgcn_readlane((int)places, (int)(j + u));
-#pragma unroll
-          for (int e = 0; e < LM_E; e++) y[u][e] = e < mine.cols ? (float)lm_get(lm_at(p.dout, (ga_long)at * p.dout_row)[e]) : 0.0f;
-        }
-      }
+      for (int u = 0; u < LM_AHEAD; u++) at[u] = (ga_uint)__builtin_amdgcn_readlane((int)places, (int)(j + u));
+      lm_fetch_rows(p, at, mine, y);
 #pragma unroll
       for (int u = 0; u < LM_AHEAD; u++) k[u] = (ga_uint)__builtin_amdgcn_readlane((int)keys, (int)(j + u));
 #pragma unroll
