@@ -61,7 +61,7 @@ struct embed_grad_args {
   int64_t grad_row, dout_row, v, d;
   float scale;
   int32_t accumulate;
-  uint32_t n, chunk, chunks, tiles, rows;
+  uint32_t n, chunk, chunks, tiles, rows, lanes_log2;
 };
 struct logprobs_args {
   const void *logits, *ids;
@@ -113,6 +113,7 @@ std::string lm_source(const lm_variant &v) {
   name("LM_X", v.x);
   name("LM_O", v.o);
   name("LM_ID", v.id);
+  if (v.kind == LM_EMBED_GRAD) s += std::string("#define LM_NARROW ") + (v.extra ? "1\n" : "0\n");
   if (v.kind == LM_SORT) s += "#define LM_R " + std::to_string(v.extra ? v.extra : 4) + "\n";
   if (v.kind == LM_LOGPROBS_GRAD) s += std::string("#define LM_ENT ") + (v.extra ? "1\n" : "0\n");
   if (v.kind == LM_LOGPROBS) {
@@ -386,13 +387,17 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   if (v > MAX_GROUPS || n > MAX_GROUPS) return c.fail(GA_XLARGE_ERROR, "too many rows");
 
   const size_t osize = gpuarray_get_elsize(grad->typecode);
-  const size_t cols = 64 * 16 / gpuarray_get_elsize(dout->typecode);   // of a wavefront
+  const size_t cols = 64 * 16 / std::max(osize, gpuarray_get_elsize(dout->typecode));   // of a wavefront
   const size_t tiles = (d + cols - 1) / cols;
-  const lm_variant vg(LM_EMBED_GRAD, dout->typecode, grad->typecode, ids->typecode, 0);
+  // rows that half a wavefront covers: several chunks of tokens side by side in one
+  unsigned lanes_log2 = 3;
+  while (((size_t)cols / 64 << lanes_log2) < d && lanes_log2 < 6) lanes_log2++;
+  const bool narrow = lanes_log2 < 6;
+  const lm_variant vg(LM_EMBED_GRAD, dout->typecode, grad->typecode, ids->typecode, narrow);
   gpudata *errbuf = nullptr;
   embed_grad_args a = {at(grad), at(dout), nullptr, nullptr, nullptr, at(ids), nullptr, ids->strides[0], ignore,
                        grad->strides[0], dout->strides[0], (int64_t)v, (int64_t)d, (float)scale, accumulate != 0,
-                       (uint32_t)n, 0, 0, (uint32_t)tiles, (uint32_t)(16 / std::min<size_t>(tiles, 4))};
+                       (uint32_t)n, 0, 0, (uint32_t)tiles, (uint32_t)(16 / std::min<size_t>(tiles, 4)), lanes_log2};
   int err = lm_errbuf(ctx, grad, &errbuf);
   if (err != GA_NO_ERROR) return err;
   a.err = errbuf->devptr;
@@ -405,9 +410,11 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
     return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
   }
   // Tokens of a chunk: enough chunks to fill the chip with wavefronts, and
-  // not so few tokens that partial sums (two rows a chunk at most) count.
+  // not so few tokens that partial sums (two rows a chunk at most) count, nor
+  // the parts of a token that comes very often.
+  const size_t per_wave = narrow ? (size_t)64 >> lanes_log2 : 1;   // chunks
   size_t chunk = 8;
-  while (chunk < 256 && n / (chunk * 2) * tiles >= 8192) chunk *= 2;
+  while (chunk < 256 && n / (chunk * 2) / per_wave * tiles >= (narrow ? 2048u : 8192u)) chunk *= 2;
   const size_t chunks = (n + chunk - 1) / chunk;
   if (chunks * tiles > MAX_GROUPS) return c.fail(GA_XLARGE_ERROR, "too many elements");
   // The digits: as few passes as ten bits a digit allow.
@@ -415,11 +422,17 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   while (v >> bits != 0) bits++;
   const unsigned passes = (bits + 9) / 10;
   bits = (bits + passes - 1) / passes;
-  const size_t per_lane = n <= 16384 ? (n + 1023) / 1024 : 4;
+  // Up to 4096 tokens one group sorts by itself, up to 16384 where clearing the
+  // rows takes longer than that (2.2 us for 1024 tokens); more are sorted by many,
+  // with few tokens a lane while there are few groups (kernel time of the sort of
+  // 8192 ids below 50257: one group 17 us, many 15; 16384: 37 and 16; 65536: one token a
+  // lane 17, four 26; 8192 tokens into 50257 rows of 1024 floats that are cleared: one group 50 us, many 59).
+  const size_t clear_bytes = accumulate ? 0 : v * d * osize;
+  const bool small = n <= 4096 || (n <= 16384 && clear_bytes / n >= 14000);
+  const size_t per_lane = small ? (n + 1023) / 1024 : n <= ((size_t)1 << 18) ? 1 : n <= ((size_t)1 << 20) ? 2 : 4;
   unsigned items = 1;
   while (items < per_lane) items *= 2;
-  const bool small = n <= 16384;
-  const size_t groups = small ? 1 : (n + 4095) / 4096;
+  const size_t groups = small ? 1 : (n + 1024 * items - 1) / (1024 * items);
 
   // scratch: two sets of keys and places, the counts of the digits, the partial sums
   const size_t list = (n * 4 + 255) & ~(size_t)255;
@@ -496,7 +509,7 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
     a.partials = scratch + 4 * list + counts;
     a.chunk = (uint32_t)chunk;
     a.chunks = (uint32_t)chunks;
-    err = lm_launch(ksum, (chunks * tiles + 3) / 4, 256, &a);
+    err = lm_launch(ksum, (chunks * tiles + 4 * per_wave - 1) / (4 * per_wave), 256, &a);
     if (err == GA_NO_ERROR && chunks > 1) err = lm_launch(kjoin, chunks * tiles, 256, &a);
   }
   return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;

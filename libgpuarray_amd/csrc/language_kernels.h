@@ -468,76 +468,78 @@ KERNEL void __launch_bounds__(1024) lm_sort_move(const lm_sorting p) {
 #endif
 
 #if LM_KIND == LM_K_EMBED_GRAD
+/* columns of a lane: 16 bytes of the wider side, so that either side's accesses are whole lines */
+#define LM_W (sizeof(LM_X) > sizeof(LM_O) ? 16 / (int)sizeof(LM_X) : 16 / (int)sizeof(LM_O))
 struct lm_embed_grad {
   GLOBAL_MEM LM_O *grad;
   GLOBAL_MEM const LM_X *dout;
   GLOBAL_MEM const ga_uint *key, *order;   /* the sorted tokens */
-  GLOBAL_MEM float *partials;              /* [chunk][2][tiles * 64 * LM_E] */
+  GLOBAL_MEM float *partials;              /* [chunk][2][tiles * 64 * LM_W] */
   GLOBAL_MEM const LM_ID *ids;             /* of few tokens */
   GLOBAL_MEM ga_int *err;
   ga_long id_step, ignore;
   ga_long grad_row, dout_row, v, d;
   float scale;
   ga_int accumulate;
-  ga_uint n, chunk, chunks, tiles, rows;
+  ga_uint n, chunk, chunks, tiles, rows, lanes_log2;
 };
 
-/* The columns of a lane: LM_E from `from` on, of which the first `skip` belong
- * to the lane before it (at a row's end, where the last LM_E columns are
+/* The columns of a lane: LM_W from `from` on, of which the first `skip` belong
+ * to the lane before it (at a row's end, where the last LM_W columns are
  * fetched), and `cols` are inside the row. */
 struct lm_columns {
   ga_long from;
   ga_int skip, cols;
 };
 LM_FN lm_columns lm_columns_of(ga_long col, ga_long d) {
-  lm_columns c = {col, 0, LM_E};
-  if (d < LM_E) {
+  lm_columns c = {col, 0, LM_W};
+  if (d < LM_W) {
     c.cols = col == 0 ? (ga_int)d : 0;
     c.from = 0;
-  } else if (d - col < LM_E) {
-    c.from = d - LM_E;
-    c.skip = col >= d ? LM_E : (ga_int)(col - c.from);
+  } else if (d - col < LM_W) {
+    c.from = d - LM_W;
+    c.skip = col >= d ? LM_W : (ga_int)(col - c.from);
   }
   return c;
 }
 
 /* One run's sum is complete. */
-LM_FN void lm_write_run(const lm_embed_grad &p, ga_uint key, const lm_columns &c, const float (&sum)[LM_E]) {
+LM_FN void lm_write_run(const lm_embed_grad &p, ga_uint key, const lm_columns &c, const float (&sum)[LM_W]) {
   GLOBAL_MEM LM_O *g = lm_at(p.grad, (ga_long)key * p.grad_row) + c.from;
-  float y[LM_E];
+  float y[LM_W];
 #pragma unroll
-  for (int e = 0; e < LM_E; e++) y[e] = p.scale * sum[e];
-  if (c.skip == 0 && c.cols == LM_E) {
+  for (int e = 0; e < LM_W; e++) y[e] = p.scale * sum[e];
+  if (c.skip == 0 && c.cols == LM_W) {
     if (p.accumulate) {
-      float have[LM_E];
+      float have[LM_W];
       lm_load(g, have);
 #pragma unroll
-      for (int e = 0; e < LM_E; e++) y[e] += have[e];
+      for (int e = 0; e < LM_W; e++) y[e] += have[e];
     }
     lm_store(g, y);
   } else {
 #pragma unroll
-    for (int e = 0; e < LM_E; e++)
+    for (int e = 0; e < LM_W; e++)
       if (e >= c.skip && e < c.cols) lm_put(g + e, p.accumulate ? lm_get(g[e]) + y[e] : y[e]);
   }
 }
 
 #define LM_AHEAD 8   /* rows in flight */
 /* the columns of rows at[..] of dout; unconditional loads: all of them in flight */
-LM_FN void lm_fetch_rows(const lm_embed_grad &p, const ga_uint (&at)[LM_AHEAD], const lm_columns &c, float (&y)[LM_AHEAD][LM_E]) {
-  if (p.d >= LM_E) {
+LM_FN void lm_fetch_rows(const lm_embed_grad &p, const ga_uint (&at)[LM_AHEAD], const lm_columns &c, float (&y)[LM_AHEAD][LM_W]) {
+  if (p.d >= LM_W) {
 #pragma unroll
     for (int u = 0; u < LM_AHEAD; u++) lm_load(lm_at(p.dout, (ga_long)at[u] * p.dout_row) + c.from, y[u]);
   } else {
 #pragma unroll
     for (int u = 0; u < LM_AHEAD; u++)
 #pragma unroll
-      for (int e = 0; e < LM_E; e++) y[u][e] = e < c.cols ? (float)lm_get(lm_at(p.dout, (ga_long)at[u] * p.dout_row)[e]) : 0.0f;
+      for (int e = 0; e < LM_W; e++) y[u][e] = e < c.cols ? (float)lm_get(lm_at(p.dout, (ga_long)at[u] * p.dout_row)[e]) : 0.0f;
   }
 }
 
 /* Few tokens need no sorting: a group takes p.rows rows of the table and up to
- * four times 64 * LM_E columns of them (as many rows as give each of its wavefronts
+ * four times 64 * LM_W columns of them (as many rows as give each of its wavefronts
  * four pieces), looks all ids through once, which leaves a mask of the tokens of
  * each row, and adds those in order; one launch in place of three. */
 #define LM_FEW 256        /* tokens at most */
@@ -569,10 +571,10 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
       any |= left[w];
     }
     if (any == 0 && p.accumulate) continue;
-    const lm_columns mine = lm_columns_of(((ga_long)tile * 64 + lane) * LM_E, p.d);
-    float sum[LM_E];
+    const lm_columns mine = lm_columns_of(((ga_long)tile * 64 + lane) * LM_W, p.d);
+    float sum[LM_W];
 #pragma unroll
-    for (int e = 0; e < LM_E; e++) sum[e] = 0.0f;
+    for (int e = 0; e < LM_W; e++) sum[e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < LM_FEW / 64; w++) {
       while (left[w] != 0) {
@@ -584,13 +586,13 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
           n += left[w] != 0;
           left[w] &= left[w] - 1;
         }
-        float y[LM_AHEAD][LM_E];
+        float y[LM_AHEAD][LM_W];
         lm_fetch_rows(p, at, mine, y);
 #pragma unroll
         for (int u = 0; u < LM_AHEAD; u++) {
           if (u < n) {
 #pragma unroll
-            for (int e = 0; e < LM_E; e++) sum[e] += y[u][e];
+            for (int e = 0; e < LM_W; e++) sum[e] += y[u][e];
           }
         }
       }
@@ -600,44 +602,60 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
 }
 
 /* A wavefront adds the rows of a chunk of the sorted tokens, in their order, over
- * 64 * LM_E columns.  A run of equal ids that lies inside the chunk is written
+ * 64 * LM_W columns.  A run of equal ids that lies inside the chunk is written
  * when it ends; what a chunk has of a run that began earlier (slot 0), or that
  * goes on in the next (slot 1), is left for lm_embed_grad_join. */
+#if LM_NARROW
+/* Short rows: 2^lanes_log2 lanes have a chunk, several chunks lie side by side in
+ * a wavefront, and what is uniform in a wavefront with one chunk is so here
+ * among the lanes of each. */
+#define LM_FROM(x, i) ((ga_uint)__builtin_amdgcn_ds_bpermute((int)((first + (i)) << 2), (int)(x)))
+#else
+#define LM_FROM(x, i) ((ga_uint)__builtin_amdgcn_readlane((int)(x), (int)(i)))
+#endif
 KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
+#if LM_NARROW
+  const ga_uint lanes = 1u << p.lanes_log2;
+  const ga_uint lane = LID_0 & (lanes - 1), first = (LID_0 & 63) - lane;
+  const ga_uint chunk = (GID_0 * 256 + LID_0) >> p.lanes_log2, tile = 0;
+#else
+  const ga_uint lanes = 64;
   const ga_uint unit = (ga_uint)__builtin_amdgcn_readfirstlane((int)(GID_0 * 4 + (LID_0 >> 6)));
   const ga_uint chunk = unit / p.tiles, tile = unit % p.tiles, lane = LID_0 & 63;
+#endif
   if (chunk >= p.chunks) return;
   const ga_uint p0 = chunk * p.chunk;
   const ga_uint n = p.n - p0 < p.chunk ? p.n - p0 : p.chunk;
-  const ga_long col = ((ga_long)tile * 64 + lane) * LM_E;
+  const ga_long col = ((ga_long)tile * 64 + lane) * LM_W;
   const lm_columns mine = lm_columns_of(col, p.d);
   const ga_uint none = (ga_uint)p.v;
-  GLOBAL_MEM float *slots = p.partials + (ga_size)chunk * 2 * p.tiles * 64 * LM_E + col;
-  float sum[LM_E];
+  GLOBAL_MEM float *slots = p.partials + (ga_size)chunk * 2 * p.tiles * 64 * LM_W + col;
+  float sum[LM_W];
 #pragma unroll
-  for (int e = 0; e < LM_E; e++) sum[e] = 0.0f;
+  for (int e = 0; e < LM_W; e++) sum[e] = 0.0f;
   const auto leave = [&](int slot) {
 #pragma unroll
-    for (int e = 0; e < LM_E; e++) slots[(ga_size)slot * p.tiles * 64 * LM_E + e] = sum[e];
+    for (int e = 0; e < LM_W; e++) slots[(ga_size)slot * p.tiles * 64 * LM_W + e] = sum[e];
   };
   const ga_uint before = p0 > 0 ? p.key[p0 - 1] : 0xffffffffu;
   const ga_uint after = p0 + n < p.n ? p.key[p0 + n] : 0xffffffffu;
   ga_uint run = p.key[p0];
   bool here = run != before;   /* the run began in this chunk */
-  for (ga_uint sub = 0; sub < n; sub += 64) {
+  for (ga_uint sub = 0; sub < n; sub += lanes) {
     const ga_uint i = p0 + sub + lane;
     const bool in = sub + lane < n;
     const ga_uint keys = in ? p.key[i] : none, places = in ? p.order[i] : 0;
-    const ga_uint m = n - sub < 64 ? n - sub : 64;
+    const ga_uint m = n - sub < lanes ? n - sub : lanes;
     for (ga_uint j = 0; j < m; j += LM_AHEAD) {
-      float y[LM_AHEAD][LM_E];
-      ga_uint k[LM_AHEAD];
-      ga_uint at[LM_AHEAD];
+      float y[LM_AHEAD][LM_W];
+      ga_uint k[LM_AHEAD], at[LM_AHEAD];
 #pragma unroll
-      for (int u = 0; u < LM_AHEAD; u++) at[u] = (ga_uint)__builtin_amdgcn_readlane((int)places, (int)(j + u));
+      for (int u = 0; u < LM_AHEAD; u++) {     /* (past m: the last one once more) */
+        const ga_uint w = j + u < m ? j + u : m - 1;
+        k[u] = LM_FROM(keys, w);
+        at[u] = LM_FROM(places, w);
+      }
       lm_fetch_rows(p, at, mine, y);
-#pragma unroll
-      for (int u = 0; u < LM_AHEAD; u++) k[u] = (ga_uint)__builtin_amdgcn_readlane((int)keys, (int)(j + u));
 #pragma unroll
       for (int u = 0; u < LM_AHEAD; u++) {
         if (j + u >= m) continue;
@@ -645,13 +663,13 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
           if (here) lm_write_run(p, run, mine, sum);
           else leave(0);
 #pragma unroll
-          for (int e = 0; e < LM_E; e++) sum[e] = 0.0f;
+          for (int e = 0; e < LM_W; e++) sum[e] = 0.0f;
           run = k[u];
           here = true;
         }
         if (k[u] != none) {
 #pragma unroll
-          for (int e = 0; e < LM_E; e++) sum[e] += y[u][e];
+          for (int e = 0; e < LM_W; e++) sum[e] += y[u][e];
         }
       }
     }
@@ -662,9 +680,16 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
 }
 
 /* The runs that cross chunks: the group of the chunk where a run begins adds
- * its parts.  A long run's parts are split over the group's wavefronts. */
+ * its parts.  A long run's parts are split over as many sets of lanes as the
+ * group has for the columns, which meet in the LDS in fixed order. */
 KERNEL void __launch_bounds__(256) lm_embed_grad_join(const lm_embed_grad p) {
-  const ga_uint chunk = GID_0 / p.tiles, tile = GID_0 % p.tiles, lane = LID_0 & 63, wave = LID_0 >> 6;
+  const ga_uint chunk = GID_0 / p.tiles, tile = GID_0 % p.tiles;
+#if LM_NARROW
+  const ga_uint lanes_log2 = p.lanes_log2;
+#else
+  const ga_uint lanes_log2 = 6;
+#endif
+  const ga_uint lane = LID_0 & ((1u << lanes_log2) - 1), set = LID_0 >> lanes_log2, sets = 256u >> lanes_log2;
   const ga_uint p0 = chunk * p.chunk;
   if (p0 + p.chunk >= p.n) return;             /* the last chunk: nothing goes on */
   const ga_uint run = p.key[p0 + p.chunk];
@@ -673,7 +698,7 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_join(const lm_embed_grad p) {
   /* the chunks after this one that begin inside the run */
   ga_uint parts = 0;
   for (;;) {
-    const ga_ulong at = (ga_ulong)(chunk + 1 + parts + lane) * p.chunk;
+    const ga_ulong at = (ga_ulong)(chunk + 1 + parts + (LID_0 & 63)) * p.chunk;
     const ga_ulong in = __builtin_amdgcn_ballot_w64(at < p.n && p.key[at < p.n ? at : 0] == run);
     if (~in == 0) {
       parts += 64;
@@ -682,33 +707,32 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_join(const lm_embed_grad p) {
     parts += (ga_uint)__builtin_ctzll(~in);
     break;
   }
-  const ga_long col = ((ga_long)tile * 64 + lane) * LM_E;
-  const ga_size pitch = (ga_size)p.tiles * 64 * LM_E;
+  const ga_long col = ((ga_long)tile * 64 + lane) * LM_W;
+  const ga_size pitch = (ga_size)p.tiles * 64 * LM_W;
   GLOBAL_MEM const float *next = p.partials + (ga_size)(chunk + 1) * 2 * pitch + col;
-  const ga_uint share = parts > 16 ? (parts + 3) / 4 : parts;
-  const ga_uint from = wave * share < parts ? wave * share : parts, to = from + share < parts ? from + share : parts;
-  float sum[LM_E];
+  const bool split = parts > 4;
+  const ga_uint share = split ? (parts + sets - 1) / sets : parts;
+  const ga_uint from = set * share < parts ? set * share : parts, to = from + share < parts ? from + share : parts;
+  float sum[LM_W];
 #pragma unroll
-  for (int e = 0; e < LM_E; e++) sum[e] = wave == 0 ? next[e - (ga_long)pitch] : 0.0f;
+  for (int e = 0; e < LM_W; e++) sum[e] = set == 0 ? next[e - (ga_long)pitch] : 0.0f;
 #pragma unroll 8
   for (ga_uint i = from; i < to; i++) {
 #pragma unroll
-    for (int e = 0; e < LM_E; e++) sum[e] += next[(ga_size)i * 2 * pitch + e];
+    for (int e = 0; e < LM_W; e++) sum[e] += next[(ga_size)i * 2 * pitch + e];
   }
-  if (parts > 16) {
-    LOCAL_MEM float meet[3][64][LM_E];
-    if (wave != 0) {
+  if (split) {
+    LOCAL_MEM float meet[256][LM_W];
 #pragma unroll
-      for (int e = 0; e < LM_E; e++) meet[wave - 1][lane][e] = sum[e];
-    }
+    for (int e = 0; e < LM_W; e++) meet[LID_0][e] = sum[e];
     local_barrier();
-    if (wave == 0) {
-      for (int w = 0; w < 3; w++)
+    if (set == 0) {
+      for (ga_uint w = 1; w < sets; w++)
 #pragma unroll
-        for (int e = 0; e < LM_E; e++) sum[e] += meet[w][lane][e];
+        for (int e = 0; e < LM_W; e++) sum[e] += meet[(w << lanes_log2) + lane][e];
     }
   }
-  if (wave == 0) lm_write_run(p, run, lm_columns_of(col, p.d), sum);
+  if (set == 0) lm_write_run(p, run, lm_columns_of(col, p.d), sum);
 }
 #endif
 
