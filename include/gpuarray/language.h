@@ -129,6 +129,22 @@ GPUARRAY_PUBLIC int GpuArray_clip_global_norm(GpuArray **rs,
                                               const GpuArray **as, size_t n,
                                               double max_norm, GpuArray *norm);
 
+/* The same for a list that is clipped again and again, of any length: an
+ * operator that holds the arrays' buffers (retained until it is freed) and a
+ * table of them in device memory.  The arrays count as they are when it is
+ * made; rs == NULL: for norms alone; rs may be `as`, or name `as` elements, to clip in place.
+ * Making one copies the table to the device, and is refused while the stream
+ * records a graph; calls may be recorded. */
+typedef struct _GpuGlobalNorm GpuGlobalNorm;
+GPUARRAY_PUBLIC int GpuGlobalNorm_new(GpuGlobalNorm **g, gpucontext *ctx,
+                                      const GpuArray **as, GpuArray **rs,
+                                      size_t n);
+GPUARRAY_PUBLIC void GpuGlobalNorm_free(GpuGlobalNorm *g);
+/* GpuArray_global_norm and GpuArray_clip_global_norm on its arrays. */
+GPUARRAY_PUBLIC int GpuGlobalNorm_norm(const GpuGlobalNorm *g, GpuArray *norm);
+GPUARRAY_PUBLIC int GpuGlobalNorm_clip(const GpuGlobalNorm *g, double max_norm,
+                                       GpuArray *norm);
+
 #ifdef __cplusplus
 }
 #endif

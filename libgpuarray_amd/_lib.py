@@ -239,6 +239,10 @@ SIGNATURES = {
     "GpuArray_token_logprobs": (C.c_int, [PA] * 7 + [C.c_double, c_ssize_t, C.c_int]),
     "GpuArray_token_logprobs_grad": (C.c_int, [PA] * 7 + [C.c_double, c_ssize_t, C.c_int]),
     "GpuArray_global_norm": (C.c_int, [PA, C.POINTER(PA), C.c_size_t]),
+    "GpuGlobalNorm_new": (C.c_int, [C.POINTER(C.c_void_p), C.c_void_p, C.POINTER(PA), C.POINTER(PA), C.c_size_t]),
+    "GpuGlobalNorm_free": (None, [C.c_void_p]),
+    "GpuGlobalNorm_norm": (C.c_int, [C.c_void_p, PA]),
+    "GpuGlobalNorm_clip": (C.c_int, [C.c_void_p, C.c_double, PA]),
     "GpuArray_clip_global_norm": (C.c_int, [C.POINTER(PA), C.POINTER(PA), C.c_size_t, C.c_double, PA]),
 }
 

@@ -267,6 +267,9 @@ def main():
     for x, o in [(GA_FLOAT, GA_FLOAT), (GA_BFLOAT16, GA_FLOAT), (GA_HALF, GA_HALF)]:
         check("gradient of short embedding rows, types %d, %d" % (x, o), gen_l(1 | x << 8 | o << 20 | GA_INT << 32 | 1 << 44))
         lm += 1
+    for kind in (4, 5):
+        check("norm operator %d on a table in device memory" % kind, gen_l(kind | GA_FLOAT << 8 | GA_FLOAT << 20 | GA_INT << 32 | 1 << 44))
+        lm += 1
     for ids, items in [(GA_INT, 1), (GA_LONG, 4), (GA_LONG, 16)]:
         check("tokens in the order of their ids, %d a lane" % items, gen_l(6 | GA_FLOAT << 8 | GA_FLOAT << 20 | ids << 32 | items << 44))
         lm += 1

@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <memory>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -90,22 +91,29 @@ struct logprobs_grad_args {
   float scale, by;
   uint32_t segments;
 };
-struct tensors_args {
-  void *partials, *result, *norm;
+struct tensor_arg {
+  const void *in;
+  void *out;
+  int64_t count;
+  uint32_t first, type;
+};
+struct norm_args {      // followed by the arrays themselves, or the address of their table
+  void *partials, *result, *norm, *counter;
   double max_norm;
-  uint32_t partial0, npartials;
-  int32_t n, norm_double;
-  uint32_t piece, in_place;
-  void *counter;
-  const void *in[LM_TENSORS];
-  void *out[LM_TENSORS];
-  int64_t count[LM_TENSORS];
-  uint32_t first[LM_TENSORS + 1];
-  unsigned char type[LM_TENSORS];
+  uint32_t partial0, npartials, n, pieces, piece;
+  int32_t norm_double, pad[2];
+};
+struct tensors_args {
+  norm_args a;
+  tensor_arg tensors[LM_TENSORS];
+};
+struct table_args {
+  norm_args a;
+  const void *tensors;
 };
 
 std::string lm_source(const lm_variant &v) {
-  std::string s = "#define LM_KIND " + std::to_string(v.kind) + "\n#define LM_TENSORS " + std::to_string(LM_TENSORS) + "\n";
+  std::string s = "#define LM_KIND " + std::to_string(v.kind) + "\n";
   auto name = [&](const char *what, unsigned tc) {
     const char *c = gpuarray_get_type((int)tc)->cluda_name;
     s += std::string("#define ") + what + " " + (c ? c : "ga_float") + "\n";
@@ -115,6 +123,7 @@ std::string lm_source(const lm_variant &v) {
   name("LM_ID", v.id);
   if (v.kind == LM_EMBED_GRAD) s += std::string("#define LM_NARROW ") + (v.extra ? "1\n" : "0\n");
   if (v.kind == LM_SORT) s += "#define LM_R " + std::to_string(v.extra ? v.extra : 4) + "\n";
+  if (v.kind == LM_NORM || v.kind == LM_CLIP) s += "#define LM_TENSORS " + std::to_string(v.extra ? 0 : LM_TENSORS) + "\n";
   if (v.kind == LM_LOGPROBS_GRAD) s += std::string("#define LM_ENT ") + (v.extra ? "1\n" : "0\n");
   if (v.kind == LM_LOGPROBS) {
     s += "#define LM_LANES " + std::to_string((v.extra & 31 ? v.extra & 31 : 1) * 64) + "\n";
@@ -670,27 +679,36 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
 
 // ---- global norm -------------------------------------------------------------------
 
-// Norm of the n arrays `as` into `norm` (may be NULL) and, if rs is not NULL, their clipping into rs.
-static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double max_norm, GpuArray *norm, const char *who) {
-  if (n == 0 && norm == nullptr) return GA_NO_ERROR;
-  gpucontext *ctx = GpuArray_context(norm != nullptr ? norm : as[0]);
-  checker c(ctx, who);
-  if (norm != nullptr) {
-    if (norm->nd > 1 || (norm->nd == 1 && norm->dimensions[0] != 1))
-      return c.fail(GA_INVALID_ERROR, "must be 0-d or have one element", "norm");
-    if (norm->typecode != GA_FLOAT && norm->typecode != GA_DOUBLE)
-      return c.fail(GA_VALUE_ERROR, "must be float or double", "norm");
-    c.aligned(norm, "norm");
-    c.result(norm, "norm");
-  }
-  if (std::isnan(max_norm) || max_norm < 0) return c.fail(GA_VALUE_ERROR, "max_norm must be 0 or above");
-  if (c.err != GA_NO_ERROR) return c.err;
-  size_t bytes = 0;
-  bool in_place = true;
+// What a call works on: arrays with at least one element, in pieces.
+struct norm_plan {
+  std::vector<tensor_arg> tensors;
+};
+
+// Pieces of 16 KiB: four chunks for each lane of a group, loaded at once.
+// Clipping 600 MB of bfloat16, by the piece: 16 KiB 186 us, 32 KiB 198, 64 KiB
+// 213.  The norm's groups take up to a 2048th of them each.
+static const size_t NORM_PIECE = 1024;        // chunks of 16 bytes
+static const size_t NORM_MAX_GROUPS = 2048;   // per table
+
+static int norm_check(checker &c, const GpuArray *norm) {
+  if (norm == nullptr) return c.err;
+  if (norm->nd > 1 || (norm->nd == 1 && norm->dimensions[0] != 1))
+    return c.fail(GA_INVALID_ERROR, "must be 0-d or have one element", "norm");
+  if (norm->typecode != GA_FLOAT && norm->typecode != GA_DOUBLE)
+    return c.fail(GA_VALUE_ERROR, "must be float or double", "norm");
+  if (GpuArray_context(norm) != c.ctx) return c.fail(GA_INVALID_ERROR, "the arrays belong to different contexts");
+  c.aligned(norm, "norm");
+  c.result(norm, "norm");
+  return c.err;
+}
+
+// The arrays `as` and, if rs is not NULL, what clipping writes, checked against each other.
+static int norm_arrays(checker &c, GpuArray **rs, const GpuArray **as, size_t n, norm_plan *plan) {
   std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
+  plan->tensors.reserve(n);
   for (size_t i = 0; i < n; i++) {
-    const GpuArray *a = as[i];
-    if (GpuArray_context(a) != ctx) return c.fail(GA_INVALID_ERROR, "the arrays belong to different contexts");
+    const GpuArray *a = as[i], *r = rs != nullptr ? rs[i] : a;
+    if (GpuArray_context(a) != c.ctx) return c.fail(GA_INVALID_ERROR, "the arrays belong to different contexts");
     if (!is_value(a->typecode) && a->typecode != GA_DOUBLE)
       return c.fail(GA_UNSUPPORTED_ERROR, "arrays must be float, half, bfloat16 or double");
     if (!GpuArray_ISONESEGMENT(a)) return c.fail(GA_INVALID_ERROR, "arrays must be contiguous");
@@ -698,119 +716,187 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
     if (c.err != GA_NO_ERROR) return c.err;
     size_t count = 1;
     for (unsigned j = 0; j < a->nd; j++) count *= a->dimensions[j];
-    bytes += count * GpuArray_ITEMSIZE(a);
-    if (norm != nullptr && overlap(norm, a)) return c.fail(GA_VALUE_ERROR, "overlaps an array", "norm");
-    if (rs == nullptr) continue;
-    const GpuArray *r = rs[i];
-    if (r != a && !same_place(r, a)) {
-      in_place = false;
-      if (GpuArray_context(r) != ctx) return c.fail(GA_INVALID_ERROR, "the arrays belong to different contexts");
-      if (r->nd != a->nd || r->typecode != a->typecode)
-        return c.fail(GA_INVALID_ERROR, "a result differs from its array in shape or type");
-      for (unsigned j = 0; j < a->nd; j++)
-        if (r->dimensions[j] != a->dimensions[j] || (a->dimensions[j] > 1 && count > 0 && r->strides[j] != a->strides[j]))
-          return c.fail(GA_INVALID_ERROR, "a result differs from its array in shape or strides");
-      c.aligned(r, "results");
-      if (norm != nullptr) c.apart(norm, r, "norm");
-      uintptr_t lo, hi;
-      span_of(a, &lo, &hi);
-      if (lo < hi) read.emplace_back(lo, hi);
+    const size_t size = GpuArray_ITEMSIZE(a);
+    if (rs != nullptr) {
+      if (r != a && !same_place(r, a)) {
+        if (GpuArray_context(r) != c.ctx) return c.fail(GA_INVALID_ERROR, "the arrays belong to different contexts");
+        if (r->nd != a->nd || r->typecode != a->typecode)
+          return c.fail(GA_INVALID_ERROR, "a result differs from its array in shape or type");
+        for (unsigned j = 0; j < a->nd; j++)
+          if (r->dimensions[j] != a->dimensions[j] || (a->dimensions[j] > 1 && count > 0 && r->strides[j] != a->strides[j]))
+            return c.fail(GA_INVALID_ERROR, "a result differs from its array in shape or strides");
+        c.aligned(r, "results");
+        if (count > 0) read.emplace_back((uintptr_t)at(a), (uintptr_t)at(a) + count * size);
+      }
+      if (!GpuArray_ISWRITEABLE(r)) return c.fail(GA_VALUE_ERROR, "a result is not writeable");
+      if (c.err != GA_NO_ERROR) return c.err;
+      if (count > 0) written.emplace_back((uintptr_t)at(r), (uintptr_t)at(r) + count * size);
     }
-    if (!GpuArray_ISWRITEABLE(r)) return c.fail(GA_VALUE_ERROR, "a result is not writeable");
-    if (c.err != GA_NO_ERROR) return c.err;
-    uintptr_t lo, hi;
-    span_of(r, &lo, &hi);
-    if (lo < hi) written.emplace_back(lo, hi);
+    if (count == 0) continue;
+    const uint64_t per = NORM_PIECE * (16 / size), p = (count + per - 1) / per;
+    if (p > 0x70000000) return c.fail(GA_XLARGE_ERROR, "an array is too large");
+    tensor_arg t = {at(a), at(r), (int64_t)count, (uint32_t)p,   // (`first` holds the count of pieces until a table is made)
+                    a->typecode == GA_FLOAT ? 0u : a->typecode == GA_HALF ? 1u : a->typecode == GA_BFLOAT16 ? 2u : 3u};
+    plan->tensors.push_back(t);
   }
-  if (rs != nullptr) {
-    // no two results overlap, and none overlaps an operand that is not itself
-    std::sort(written.begin(), written.end());
-    for (size_t i = 1; i < written.size(); i++)
-      if (written[i].first < written[i - 1].second) return c.fail(GA_VALUE_ERROR, "results overlap");
-    for (auto &x : read) {
-      auto it = std::lower_bound(written.begin(), written.end(), std::make_pair(x.second, (uintptr_t)0));
-      if (it != written.begin() && (it - 1)->second > x.first)
-        return c.fail(GA_VALUE_ERROR, "a result overlaps another array");
-    }
+  // no two results overlap, and none overlaps an operand that is not itself
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); i++)
+    if (written[i].first < written[i - 1].second) return c.fail(GA_VALUE_ERROR, "results overlap");
+  for (auto &x : read) {
+    auto it = std::lower_bound(written.begin(), written.end(), std::make_pair(x.second, (uintptr_t)0));
+    if (it != written.begin() && (it - 1)->second > x.first)
+      return c.fail(GA_VALUE_ERROR, "a result overlaps another array");
   }
+  return GA_NO_ERROR;
+}
 
-  // Pieces of 16 KiB: four chunks for each lane of a group, loaded at once.
-  // Clipping 600 MB of bfloat16, by the piece: 16 KiB 186 us, 32 KiB 198,
-  // 64 KiB 213.  The norm's groups take every 2048th piece (1024 groups: 88 us, 2048: 85, 4096: 84).
-  const size_t piece = 1024;        // chunks of 16 bytes
-  const size_t max_groups = 2048;   // of the norm, per table
-  const size_t tables = (n + LM_TENSORS - 1) / LM_TENSORS + bytes / 16 / piece / 0x70000000;
+// `norm` must lie outside all the arrays.
+static int norm_apart(checker &c, const norm_plan &plan, const GpuArray *norm) {
+  if (norm == nullptr) return GA_NO_ERROR;
+  const uintptr_t lo = (uintptr_t)at(norm), hi = lo + GpuArray_ITEMSIZE(norm);
+  static const size_t sizes[4] = {4, 2, 2, 8};
+  for (const tensor_arg &t : plan.tensors) {
+    const size_t bytes = (size_t)t.count * sizes[t.type];
+    if ((lo < (uintptr_t)t.in + bytes && (uintptr_t)t.in < hi) || (lo < (uintptr_t)t.out + bytes && (uintptr_t)t.out < hi))
+      return c.fail(GA_VALUE_ERROR, "overlaps an array", "norm");
+  }
+  return GA_NO_ERROR;
+}
+
+// Launches on tables: of a list of arrays cut into argument lists, or one in device memory.
+struct norm_table {
+  const tensor_arg *tensors;   // NULL: in device memory
+  const void *device;
+  uint32_t n, pieces;
+};
+static int norm_run(checker &c, const std::vector<norm_table> &tables, bool clip, double max_norm, const GpuArray *norm) {
+  gpucontext *ctx = c.ctx;
+  const bool by_table = tables.size() == 1 && tables[0].tensors == nullptr;
+  const size_t size = by_table ? sizeof(table_args) : sizeof(tensors_args);
+  const lm_variant vn(LM_NORM, GA_FLOAT, GA_FLOAT, GA_INT, by_table), vc(LM_CLIP, GA_FLOAT, GA_FLOAT, GA_INT, by_table);
   char *scratch = nullptr;
   GpuKernel *kpieces = nullptr, *kfinal = nullptr, *kclip = nullptr;
-  const lm_variant vn(LM_NORM, GA_FLOAT, GA_FLOAT, GA_INT, 0), vc(LM_CLIP, GA_FLOAT, GA_FLOAT, GA_INT, 0);
-  int err = lm_kernel(ctx, vn, "lm_norm_pieces", sizeof(tensors_args), &kpieces);
-  gpudata *counters = n != 0 ? ga_hip_redux_counters(ctx) : nullptr;
-  bool finished = false;
-  if (err == GA_NO_ERROR && rs != nullptr) err = lm_kernel(ctx, vc, "lm_clip_pieces", sizeof(tensors_args), &kclip);
-  if (err == GA_NO_ERROR) err = lm_scratch(ctx, 256 + (tables + 1) * max_groups * sizeof(double), &scratch);
+  int err = lm_kernel(ctx, vn, "lm_norm_pieces", size, &kpieces);
+  if (err == GA_NO_ERROR && clip) err = lm_kernel(ctx, vc, "lm_clip_pieces", size, &kclip);
+  if (err == GA_NO_ERROR)
+    err = lm_scratch(ctx, 256 + (tables.size() + 1) * NORM_MAX_GROUPS * sizeof(double), &scratch);
   if (err != GA_NO_ERROR) return err;
+  gpudata *counters = ga_hip_redux_counters(ctx);
 
-  tensors_args a;
-  memset(&a, 0, sizeof(a));
+  tensors_args args;
+  table_args *const short_args = (table_args *)&args;
+  memset(&args, 0, sizeof(args));
+  norm_args &a = args.a;
   a.result = scratch;
   a.partials = scratch + 256;
   a.norm = norm ? at(norm) : nullptr;
   a.norm_double = norm != nullptr && norm->typecode == GA_DOUBLE;
   a.max_norm = max_norm;
-  a.piece = (uint32_t)piece;
-  a.in_place = in_place;
-  // the arrays in tables of up to LM_TENSORS
-  auto for_tables = [&](auto &&launch) -> int {
-    size_t i = 0;
-    while (i < n) {
-      a.n = 0;
-      a.first[0] = 0;
-      for (; i < n && a.n < (int)LM_TENSORS; i++) {
-        const GpuArray *x = as[i];
-        int64_t count = 1;
-        for (unsigned j = 0; j < x->nd; j++) count *= (int64_t)x->dimensions[j];
-        const int64_t per = (int64_t)piece * (16 / (int64_t)GpuArray_ITEMSIZE(x)), p = (count + per - 1) / per;
-        if (p == 0) continue;
-        if (a.first[a.n] + p > 0x70000000) {
-          if (a.n == 0) return c.fail(GA_XLARGE_ERROR, "an array is too large");
-          break;
-        }
-        a.in[a.n] = at(x);
-        a.out[a.n] = rs != nullptr ? at(rs[i]) : nullptr;
-        a.count[a.n] = count;
-        a.type[a.n] = x->typecode == GA_FLOAT ? 0 : x->typecode == GA_HALF ? 1 : x->typecode == GA_BFLOAT16 ? 2 : 3;
-        a.first[a.n + 1] = a.first[a.n] + (uint32_t)p;
-        a.n++;
-      }
-      if (a.n == 0) break;
-      bool more = false;   // any element in the arrays that are left
-      for (size_t j = i; j < n && !more; j++) {
-        more = true;
-        for (unsigned d = 0; d < as[j]->nd; d++) more = more && as[j]->dimensions[d] != 0;
-      }
-      const int e = launch(a.first[a.n], !more);
-      if (e != GA_NO_ERROR) return e;
-    }
-    return GA_NO_ERROR;
+  a.piece = (uint32_t)NORM_PIECE;
+  auto take = [&](const norm_table &t) {
+    a.n = t.n;
+    a.pieces = t.pieces;
+    if (t.tensors != nullptr) memcpy(args.tensors, t.tensors, t.n * sizeof(tensor_arg));
+    else short_args->tensors = t.device;
   };
   // Up to two groups for each compute unit of the last table finish the norm
   // themselves; more of them would wait for one another's counting longer than
   // a launch takes.
-  err = for_tables([&](size_t pieces, bool last) -> int {
-    const size_t groups = std::min(pieces, max_groups);
+  bool finished = false;
+  for (size_t i = 0; i < tables.size() && err == GA_NO_ERROR; i++) {
+    take(tables[i]);
+    const size_t groups = std::min<size_t>(a.pieces, NORM_MAX_GROUPS);
     a.partial0 = a.npartials;
     a.npartials += (uint32_t)groups;
-    finished = last && counters != nullptr && groups <= 512;
+    finished = i + 1 == tables.size() && counters != nullptr && groups <= 512;
     a.counter = finished ? counters->devptr : nullptr;
-    return lm_launch(kpieces, groups, 256, &a);
-  });
-  if (err == GA_NO_ERROR && !finished) {
-    err = lm_kernel(ctx, vn, "lm_norm_final", sizeof(tensors_args), &kfinal);
-    if (err == GA_NO_ERROR) err = lm_launch(kfinal, 1, 1024, &a);
+    err = lm_launch(kpieces, groups, 256, &args);
   }
-  if (err == GA_NO_ERROR && rs != nullptr)
-    err = for_tables([&](size_t pieces, bool) { return lm_launch(kclip, pieces, 256, &a); });
+  if (err == GA_NO_ERROR && !finished) {
+    err = lm_kernel(ctx, vn, "lm_norm_final", size, &kfinal);
+    if (err == GA_NO_ERROR) err = lm_launch(kfinal, 1, 1024, &args);
+  }
+  for (size_t i = 0; i < tables.size() && err == GA_NO_ERROR && clip; i++) {
+    if (tables.size() > 1) take(tables[i]);
+    err = lm_launch(kclip, a.pieces, 256, &args);
+  }
   return err;
+}
+
+// One call on a list of arrays, which travel with the arguments of the launches.
+static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double max_norm, GpuArray *norm, const char *who) {
+  if (n == 0 && norm == nullptr) return GA_NO_ERROR;
+  checker c(GpuArray_context(norm != nullptr ? norm : as[0]), who);
+  norm_plan plan;
+  if (std::isnan(max_norm) || max_norm < 0) return c.fail(GA_VALUE_ERROR, "max_norm must be 0 or above");
+  if (norm_check(c, norm) != GA_NO_ERROR || norm_arrays(c, rs, as, n, &plan) != GA_NO_ERROR ||
+      norm_apart(c, plan, norm) != GA_NO_ERROR)
+    return c.err;
+  std::vector<norm_table> tables;
+  for (size_t i = 0; i < plan.tensors.size(); i++) {
+    const uint32_t p = plan.tensors[i].first;
+    if (tables.empty() || tables.back().n == LM_TENSORS || tables.back().pieces + (uint64_t)p > 0x7fffffff)
+      tables.push_back({&plan.tensors[i], nullptr, 0, 0});
+    plan.tensors[i].first = tables.back().pieces;
+    tables.back().n++;
+    tables.back().pieces += p;
+  }
+  return norm_run(c, tables, rs != nullptr, max_norm, norm);
+}
+
+struct _GpuGlobalNorm {
+  gpucontext *ctx;
+  norm_plan plan;
+  bool clips;
+  gpudata *table;
+  uint32_t pieces;
+  std::vector<gpudata *> held;   // the arrays' buffers
+};
+
+static int global_norm_new(GpuGlobalNorm **out, gpucontext *ctx, const GpuArray **as, GpuArray **rs, size_t n) {
+  checker c(ctx, "GpuGlobalNorm_new");
+  if (ga_hip_capturing(ctx))
+    return c.fail(GA_UNSUPPORTED_ERROR, "the stream records a graph: make the operator before recording");
+  std::unique_ptr<GpuGlobalNorm> g(new GpuGlobalNorm());
+  g->ctx = ctx;
+  g->clips = rs != nullptr;
+  g->table = nullptr;
+  if (norm_arrays(c, rs, as, n, &g->plan) != GA_NO_ERROR) return c.err;
+  uint64_t pieces = 0;
+  for (tensor_arg &t : g->plan.tensors) {
+    const uint32_t p = t.first;
+    t.first = (uint32_t)pieces;
+    pieces += p;
+    if (pieces > 0x7fffffff) return c.fail(GA_XLARGE_ERROR, "the arrays are too large together");
+  }
+  g->pieces = (uint32_t)pieces;
+  g->held.reserve(2 * n);
+  if (!g->plan.tensors.empty()) {
+    int err = GA_NO_ERROR;
+    g->table = gpudata_alloc(ctx, g->plan.tensors.size() * sizeof(tensor_arg), g->plan.tensors.data(), GA_BUFFER_INIT, &err);
+    if (g->table == nullptr) return err;
+  }
+  for (size_t i = 0; i < n; i++) {
+    g->held.push_back(as[i]->data);
+    if (rs != nullptr) g->held.push_back(rs[i]->data);
+  }
+  for (gpudata *b : g->held) gpudata_retain(b);
+  *out = g.release();
+  return GA_NO_ERROR;
+}
+
+static int global_norm_call(const GpuGlobalNorm *g, bool clip, double max_norm, GpuArray *norm, const char *who) {
+  checker c(g->ctx, who);
+  if (std::isnan(max_norm) || max_norm < 0) return c.fail(GA_VALUE_ERROR, "max_norm must be 0 or above");
+  if (clip && !g->clips) return c.fail(GA_INVALID_ERROR, "the operator was made without results");
+  if (norm_check(c, norm) != GA_NO_ERROR || norm_apart(c, g->plan, norm) != GA_NO_ERROR) return c.err;
+  std::vector<norm_table> tables;
+  if (g->table != nullptr)
+    tables.push_back({nullptr, g->table->devptr, (uint32_t)g->plan.tensors.size(), g->pieces});
+  else if (norm == nullptr)
+    return GA_NO_ERROR;
+  return norm_run(c, tables, clip, max_norm, norm);
 }
 
 // ---- the C entry points: nothing thrown leaves them ----------------------------------
@@ -852,6 +938,38 @@ int GpuArray_token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, cons
     return token_logprobs_grad(dlogits, logits, ids, stats, dlogp, entropy, dentropy, scale, ignore, check_error);
   } catch (const std::bad_alloc &) {
     return no_memory(GpuArray_context(logits));
+  }
+}
+
+int GpuGlobalNorm_new(GpuGlobalNorm **g, gpucontext *ctx, const GpuArray **as, GpuArray **rs, size_t n) {
+  *g = nullptr;
+  try {
+    return global_norm_new(g, ctx, as, rs, n);
+  } catch (const std::bad_alloc &) {
+    return no_memory(ctx);
+  }
+}
+
+void GpuGlobalNorm_free(GpuGlobalNorm *g) {
+  if (g == nullptr) return;
+  if (g->table != nullptr) gpudata_release(g->table);
+  for (gpudata *b : g->held) gpudata_release(b);
+  delete g;
+}
+
+int GpuGlobalNorm_norm(const GpuGlobalNorm *g, GpuArray *norm) {
+  try {
+    return global_norm_call(g, false, 0.0, norm, "GpuGlobalNorm_norm");
+  } catch (const std::bad_alloc &) {
+    return no_memory(g->ctx);
+  }
+}
+
+int GpuGlobalNorm_clip(const GpuGlobalNorm *g, double max_norm, GpuArray *norm) {
+  try {
+    return global_norm_call(g, true, max_norm, norm, "GpuGlobalNorm_clip");
+  } catch (const std::bad_alloc &) {
+    return no_memory(g->ctx);
   }
 }
 

@@ -1418,34 +1418,42 @@ KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad 
 #endif
 
 #if LM_KIND == LM_K_NORM || LM_KIND == LM_K_CLIP
-/* The arrays of a launch: up to LM_TENSORS of them, cut in pieces of `piece`
- * 16-byte chunks that are numbered through; first[i] is the number of array i's
- * first piece.  Arguments are read through a long way, so a piece finds its
- * array with one load a lane and a ballot, not by bisection. */
+/* The arrays of a launch, cut in pieces of `piece` 16-byte chunks that are
+ * numbered through; `first` is the number of an array's first piece.  They come
+ * with the arguments, up to LM_TENSORS of them, or lie in a table in device
+ * memory (LM_TENSORS 0).  A piece finds its array with one load a lane and a ballot, for each
+ * factor of 64 in their number. */
+struct lm_tensor {
+  GLOBAL_MEM const void *in;
+  GLOBAL_MEM void *out;
+  ga_long count;
+  ga_uint first, type;           /* type: 0 float, 1 half, 2 bfloat16, 3 double */
+};
 struct lm_tensors {
   GLOBAL_MEM double *partials;   /* sums of squares, one per group */
   GLOBAL_MEM double *result;     /* the factor */
   GLOBAL_MEM void *norm;
+  GLOBAL_MEM ga_uint *counter;   /* a zero that the last table's groups count on, or NULL: lm_norm_final follows */
   double max_norm;
   ga_uint partial0, npartials;
-  ga_int n, norm_double;
-  ga_uint piece, in_place;
-  GLOBAL_MEM ga_uint *counter;   /* a zero that the last table's groups count on, or NULL: lm_norm_final follows */
-  GLOBAL_MEM const void *in[LM_TENSORS];
-  GLOBAL_MEM void *out[LM_TENSORS];
-  ga_long count[LM_TENSORS];
-  ga_uint first[LM_TENSORS + 1];
-  unsigned char type[LM_TENSORS];   /* 0 float, 1 half, 2 bfloat16, 3 double */
+  ga_uint n, pieces, piece;
+  ga_int norm_double, pad[2];
+#if LM_TENSORS
+  lm_tensor tensors[LM_TENSORS];
+#else
+  GLOBAL_MEM const lm_tensor *tensors;
+#endif
 };
-LM_FN ga_int lm_find(const lm_tensors &p, ga_uint piece) {
-  ga_int before = 0;
-#pragma unroll
-  for (int k = 0; k < LM_TENSORS; k += 64) {
-    const ga_int i = k + (ga_int)(LID_0 & 63);
-    const bool begun = i < p.n && p.first[i] <= piece;
-    before += (ga_int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(begun));
+LM_FN ga_uint lm_find(const lm_tensors &p, ga_uint piece) {
+  ga_uint from = 0, n = p.n;
+  while (n > 1) {
+    const ga_uint step = (n + 63) / 64, i = (LID_0 & 63) * step;
+    const bool begun = i < n && p.tensors[from + (i < n ? i : 0)].first <= piece;
+    const ga_uint at = ((ga_uint)__builtin_popcountll(__builtin_amdgcn_ballot_w64(begun)) - 1) * step;
+    from += at;
+    n = n - at < step ? n - at : step;
   }
-  return before - 1;
+  return (ga_uint)__builtin_amdgcn_readfirstlane((int)from);
 }
 #define LM_BY_TYPE(type, F)       \
   switch (type) {                 \
@@ -1487,10 +1495,10 @@ template <> struct lm_wide<ga_double> { typedef double type; };
 #define LM_GROUP 256
 #define LM_U 8   /* chunks in flight per lane */
 
-/* The squares of piece elements [from, from + n) of type T, summed in 64 bits:
+/* The squares of n elements of type T, summed in 64 bits by the group:
  * a multiply-add of doubles costs what one of floats does, and neither the
  * largest nor the smallest float's square leaves their range. */
-template <class T> LM_FN double lm_squares(GLOBAL_MEM const T *x, ga_long n, ga_uint chunks) {
+template <class T> LM_FN double lm_squares(GLOBAL_MEM const T *x, ga_long n) {
   constexpr int E = 16 / (int)sizeof(T);
   double s[4] = {0.0, 0.0, 0.0, 0.0};
   ga_long head = (ga_long)((-(ga_size)x & 15) / sizeof(T));
@@ -1545,19 +1553,27 @@ template <int LANES> LM_FN void lm_norm_of_partials(const lm_tensors &p) {
     }
   }
 }
-/* A group adds every GDIM_0-th piece. */
+/* A group adds a range of pieces: what of it lies in one array in one go. */
 KERNEL void __launch_bounds__(LM_GROUP) lm_norm_pieces(const lm_tensors p) {
   double s = 0.0;
-  const ga_uint pieces = p.first[p.n];
-  for (ga_uint piece = GID_0; piece < pieces; piece += GDIM_0) {
-    const ga_int i = lm_find(p, piece);
-#define LM_SQUARES(T)                                                        \
-  {                                                                          \
-    const ga_long per = (ga_long)p.piece * (16 / (ga_long)sizeof(T));        \
-    const ga_long from = (ga_long)(piece - p.first[i]) * per, left = p.count[i] - from; \
-    s += lm_squares((GLOBAL_MEM const T *)p.in[i] + from, left < per ? left : per, p.piece); \
+  const ga_uint share = (p.pieces + GDIM_0 - 1) / GDIM_0;
+  ga_uint piece = GID_0 * share;
+  const ga_uint end = p.pieces - piece < share ? p.pieces : piece + share;
+  if (piece < p.pieces) {
+    for (ga_uint i = lm_find(p, piece); piece < end; i++) {
+      const lm_tensor t = p.tensors[i];
+      const ga_uint next = i + 1 < p.n ? p.tensors[i + 1].first : p.pieces;
+      const ga_uint stop = next < end ? next : end;
+#define LM_SQUARES(T)                                                             \
+  {                                                                               \
+    const ga_long per = (ga_long)p.piece * (16 / (ga_long)sizeof(T));             \
+    const ga_long from = (ga_long)(piece - t.first) * per, left = t.count - from; \
+    const ga_long n = (ga_long)(stop - piece) * per;                              \
+    s += lm_squares((GLOBAL_MEM const T *)t.in + from, left < n ? left : n);      \
   }
-    LM_BY_TYPE(p.type[i], LM_SQUARES)
+      LM_BY_TYPE(t.type, LM_SQUARES)
+      piece = stop;
+    }
   }
   s = lm_group_sum<LM_GROUP / 64>(s);
   LOCAL_MEM ga_uint last;
@@ -1618,16 +1634,15 @@ template <class T> LM_FN void lm_scale(GLOBAL_MEM const T *x, GLOBAL_MEM T *o, g
 }
 KERNEL void __launch_bounds__(LM_GROUP) lm_clip_pieces(const lm_tensors p) {
   const ga_uint piece = GID_0;
-  const ga_int i = lm_find(p, piece);
+  const lm_tensor t = p.tensors[lm_find(p, piece)];
   const double by = p.result[0];
-  if (by == 1.0 && p.in_place) return;
-  if (by == 1.0 && p.in[i] == p.out[i]) return;
+  if (by == 1.0 && t.in == t.out) return;
 #define LM_SCALE(T)                                                          \
   {                                                                          \
     const ga_long per = (ga_long)p.piece * (16 / (ga_long)sizeof(T));        \
-    const ga_long from = (ga_long)(piece - p.first[i]) * per, left = p.count[i] - from; \
-    lm_scale((GLOBAL_MEM const T *)p.in[i] + from, (GLOBAL_MEM T *)p.out[i] + from, left < per ? left : per, by); \
+    const ga_long from = (ga_long)(piece - t.first) * per, left = t.count - from; \
+    lm_scale((GLOBAL_MEM const T *)t.in + from, (GLOBAL_MEM T *)t.out + from, left < per ? left : per, by); \
   }
-  LM_BY_TYPE(p.type[i], LM_SCALE)
+  LM_BY_TYPE(t.type, LM_SCALE)
 }
 #endif

@@ -105,31 +105,46 @@ def token_logprobs_grad(logits, ids, stats, dlogp, entropy=None, dentropy=None, 
     return out
 
 
+def _pointers(arrays):
+    for a in arrays:
+        if not isinstance(a, GpuArray):
+            raise TypeError("expected GpuArrays")
+    return (_lib.PA * max(len(arrays), 1))(*[C.pointer(a.ga) for a in arrays])
+
+
+def _lists(arrays, out, context):
+    arrays = list(arrays)
+    out = None if out is None else list(out)
+    if out is not None and len(out) != len(arrays):
+        raise ValueError("%d arrays to clip into for %d" % (len(out), len(arrays)))
+    pointers = _pointers(arrays), None if out is None else _pointers(out)
+    return arrays, out, arrays[0].context if arrays else gpuarray._ensure_context(context), pointers
+
+
 class GlobalNorm(object):
     """The 2-norm over all elements of a list of contiguous arrays, and
-    clipping by it: `out` is the list of arrays that clipping writes (None:
-    the arrays themselves).  Holds the arrays and their C argument lists, for
-    callers that clip the same gradients every step."""
+    clipping by it, for callers that clip the same gradients every step: `out`
+    is the list of arrays that clipping writes (None: the arrays themselves).
+    Holds the arrays, as they are now, and a table of them on the device."""
 
     def __init__(self, arrays, out=None, context=None):
-        self.arrays = list(arrays)
-        self.out = None if out is None else list(out)
-        if self.out is not None and len(self.out) != len(self.arrays):
-            raise ValueError("%d arrays to clip into for %d" % (len(self.out), len(self.arrays)))
-        for a in self.arrays + (self.out or []):
-            if not isinstance(a, GpuArray):
-                raise TypeError("expected GpuArrays")
-        self.context = self.arrays[0].context if self.arrays else gpuarray._ensure_context(context)
-        self._as = (_lib.PA * max(len(self.arrays), 1))(*[C.pointer(a.ga) for a in self.arrays])
-        self._rs = None if self.out is None else (_lib.PA * max(len(self.out), 1))(*[C.pointer(a.ga) for a in self.out])
+        self.arrays, self.out, self.context, (a, r) = _lists(arrays, out, context)
+        if r is None and all(x.flags.writeable for x in self.arrays):
+            r = a                  # (read-only arrays have a norm, but are not clipped in place)
+        self.g = C.c_void_p()
+        _check(lib.GpuGlobalNorm_new(C.byref(self.g), self.context.ctx, a, r, len(self.arrays)), self.context.ctx)
 
-    def _norm(self, norm):
-        return gpuarray.empty((), "float32", context=self.context) if norm is None else norm
+    def __del__(self):
+        g = getattr(self, "g", None)
+        if g:
+            lib.GpuGlobalNorm_free(g)
+            self.g = None
 
     def norm(self, norm=None):
         """The norm, in a 0-d float32 array or in `norm`."""
-        norm = self._norm(norm)
-        err = lib.GpuArray_global_norm(norm._ref, self._as, len(self.arrays))
+        if norm is None:
+            norm = gpuarray.empty((), "float32", context=self.context)
+        err = lib.GpuGlobalNorm_norm(self.g, norm._ref)
         if err:
             _check(err, self.context.ctx)
         return norm
@@ -137,18 +152,27 @@ class GlobalNorm(object):
     def clip(self, max_norm, norm=None):
         """Scales the arrays by max_norm / norm where the norm is finite and
         above max_norm; returns the norm before that.  Does not wait."""
-        norm = self._norm(norm)
-        err = lib.GpuArray_clip_global_norm(self._rs, self._as, len(self.arrays), max_norm, norm._ref)
+        if norm is None:
+            norm = gpuarray.empty((), "float32", context=self.context)
+        err = lib.GpuGlobalNorm_clip(self.g, max_norm, norm._ref)
         if err:
             _check(err, self.context.ctx)
         return norm
 
 
 def global_norm(arrays, norm=None, context=None):
-    """GlobalNorm(arrays).norm()"""
-    return GlobalNorm(arrays, context=context).norm(norm)
+    """GlobalNorm(arrays).norm() in one call, for a list that is used once."""
+    arrays, _, ctx, (a, _) = _lists(arrays, None, context)
+    if norm is None:
+        norm = gpuarray.empty((), "float32", context=ctx)
+    _check(lib.GpuArray_global_norm(norm._ref, a, len(arrays)), ctx.ctx)
+    return norm
 
 
 def clip_by_global_norm(arrays, max_norm, out=None, norm=None, context=None):
-    """GlobalNorm(arrays, out).clip(max_norm)"""
-    return GlobalNorm(arrays, out, context=context).clip(max_norm, norm)
+    """GlobalNorm(arrays, out).clip(max_norm) in one call, for a list that is used once."""
+    arrays, out, ctx, (a, r) = _lists(arrays, out, context)
+    if norm is None:
+        norm = gpuarray.empty((), "float32", context=ctx)
+    _check(lib.GpuArray_clip_global_norm(r, a, len(arrays), max_norm, norm._ref), ctx.ctx)
+    return norm

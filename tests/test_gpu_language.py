@@ -672,6 +672,42 @@ def test_clipping_special_norms_and_layouts(ctx):
     assert abs(want) > 0
 
 
+@pytest.mark.parametrize("count", [1, 64, 65, 300, 4097])
+def test_global_norm_operator(ctx, count):
+    """The operator that holds its arrays against the call that does not, over lists of any length."""
+    rng = np.random.default_rng(count)
+    kinds = ["bfloat16", "float32", "float16", "float64"]
+    sizes = [(i % 7,) if count > 1 else (5,) for i in range(count)]
+    sizes[count // 2] = (40003,)
+    hosts, devs = arrays_of(ctx, sizes, kinds, rng)
+    into = [gpuarray.empty(h.shape, h.dtype, context=ctx) for h in hosts]
+    op = ga.GlobalNorm(devs, out=into)
+    norm = np.asarray(op.norm())
+    want = np.sqrt(sum((decode(h) ** 2).sum() for h in hosts))
+    assert abs(norm - want) <= want * 2 * U
+    assert np.array_equal(np.asarray(op.clip(want / 2)), norm)
+    again = [gpuarray.empty(h.shape, h.dtype, context=ctx) for h in hosts]
+    ga.clip_by_global_norm(devs, want / 2, out=again)
+    for a, b, h, d in zip(into, again, hosts, devs):
+        assert np.array_equal(decode(a), decode(b)) and np.array_equal(decode(d), decode(h))
+    big = count // 2
+    assert np.max(np.abs(decode(into[big]) - decode(hosts[big]) / 2)) < 0.02
+    assert np.array_equal(np.asarray(ga.global_norm(devs)), norm)
+
+
+def test_global_norm_operator_holds_its_arrays(ctx):
+    a = gpuarray.array(np.full(1000, 3, np.float32), context=ctx)
+    op = ga.GlobalNorm([a])
+    op.arrays = None
+    view = a[:2]
+    del a
+    gpuarray.array(np.zeros(1000, np.float32), context=ctx)      # would take the freed block
+    assert abs(float(np.asarray(op.clip(1.0))) - 3 * np.sqrt(1000)) < 1e-3
+    assert np.max(np.abs(np.asarray(view) - 1 / np.sqrt(1000))) < 1e-6
+    nothing = ga.GlobalNorm([], context=ctx)
+    assert float(np.asarray(nothing.norm())) == 0.0 and float(np.asarray(nothing.clip(1.0))) == 0.0
+
+
 # ---- long offsets, graphs, the whole together -------------------------------------------------------
 
 def test_offsets_past_32_bits(ctx):
@@ -727,6 +763,15 @@ def test_language_operators_replay_from_a_graph(ctx):
         ga.clip_by_global_norm([o["g"]], 1e-3, out=[o["clipped"]], norm=o["norm"])
 
     eager, replayed = outputs(), outputs()
+    for o in (eager, replayed):
+        o["all"] = gpuarray.zeros((), context=ctx)
+    ops = {id(o): ga.GlobalNorm([o["d"], o["g"], o["h"]]) for o in (eager, replayed)}
+    step = issue
+
+    def issue(o):
+        step(o)
+        ops[id(o)].clip(5.0, norm=o["all"])
+
     issue(eager)
     issue(replayed)
     ctx.sync()
@@ -734,6 +779,8 @@ def test_language_operators_replay_from_a_graph(ctx):
     assert hip.hipStreamBeginCapture(stream, 0) == 0
     try:
         issue(replayed)
+        with pytest.raises(_lib.UnsupportedException):
+            ga.GlobalNorm([eager["d"]])                          # its table cannot be copied now
     finally:
         rc = hip.hipStreamEndCapture(stream, C.byref(graph))
     assert rc == 0
@@ -905,6 +952,14 @@ def test_refusal_of_arrays_of_two_contexts(ctx):
         with pytest.raises(_lib.GpuArrayException) as e:
             call()
         assert e.value.code == _lib.GA_INVALID_ERROR
+    fixed = gpuarray.from_strided(table, 0, (9, 8), (32, 4), writeable=False)
+    with pytest.raises(_lib.GpuArrayException):
+        ga.GlobalNorm([fixed]).clip(1.0)
+    for call in (lambda: ga.GlobalNorm([table]).clip(-1.0), lambda: ga.GlobalNorm([table]).clip(float("nan")),
+                 lambda: ga.GlobalNorm([table]).norm(table[0, :1]), lambda: ga.GlobalNorm([table, table]),
+                 lambda: ga.GlobalNorm([ids], context=second), lambda: ga.GlobalNorm([table[:, :3]])):
+        with pytest.raises(_lib.GpuArrayException):
+            call()
     with pytest.raises(ValueError):
         ga.GlobalNorm([table], out=[])
     with pytest.raises(TypeError):
