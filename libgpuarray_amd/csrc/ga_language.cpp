@@ -686,9 +686,11 @@ struct norm_plan {
 
 // Pieces of 16 KiB: four chunks for each lane of a group, loaded at once.
 // Clipping 600 MB of bfloat16, by the piece: 16 KiB 186 us, 32 KiB 198, 64 KiB
-// 213.  The norm's groups take up to a 2048th of them each.
-static const size_t NORM_PIECE = 1024;        // chunks of 16 bytes
-static const size_t NORM_MAX_GROUPS = 2048;   // per table
+// 213.  The norm's groups, two for each compute unit, take a range of them each
+// (600 MB in 256 to 2048 groups: 107 to 109 us), so that the last one of them can
+// finish the norm.
+static const size_t NORM_PIECE = 1024;       // chunks of 16 bytes
+static const size_t NORM_MAX_GROUPS = 512;   // per table
 
 static int norm_check(checker &c, const GpuArray *norm) {
   if (norm == nullptr) return c.err;
@@ -800,16 +802,15 @@ static int norm_run(checker &c, const std::vector<norm_table> &tables, bool clip
     if (t.tensors != nullptr) memcpy(args.tensors, t.tensors, t.n * sizeof(tensor_arg));
     else short_args->tensors = t.device;
   };
-  // Up to two groups for each compute unit of the last table finish the norm
-  // themselves; more of them would wait for one another's counting longer than
-  // a launch takes.
+  // (without counters, while a graph is recorded before they are made, a launch
+  // of its own finishes the norm)
   bool finished = false;
   for (size_t i = 0; i < tables.size() && err == GA_NO_ERROR; i++) {
     take(tables[i]);
     const size_t groups = std::min<size_t>(a.pieces, NORM_MAX_GROUPS);
     a.partial0 = a.npartials;
     a.npartials += (uint32_t)groups;
-    finished = i + 1 == tables.size() && counters != nullptr && groups <= 512;
+    finished = i + 1 == tables.size() && counters != nullptr;
     a.counter = finished ? counters->devptr : nullptr;
     err = lm_launch(kpieces, groups, 256, &args);
   }
