@@ -686,11 +686,11 @@ struct norm_plan {
 
 // Pieces of 16 KiB: four chunks for each lane of a group, loaded at once.
 // Clipping 600 MB of bfloat16, by the piece: 16 KiB 186 us, 32 KiB 198, 64 KiB
-// 213.  The norm's groups, two for each compute unit, take a range of them each
+// 213.  The norm's groups, one for each compute unit, take a range of them each
 // (600 MB in 256 to 2048 groups: 107 to 109 us), so that the last one of them can
 // finish the norm.
 static const size_t NORM_PIECE = 1024;       // chunks of 16 bytes
-static const size_t NORM_MAX_GROUPS = 512;   // per table
+static const size_t NORM_MAX_GROUPS = 256;   // per table
 
 static int norm_check(checker &c, const GpuArray *norm) {
   if (norm == nullptr) return c.err;
