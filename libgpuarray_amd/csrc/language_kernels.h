@@ -197,21 +197,21 @@ KERNEL void __launch_bounds__(256) lm_embed_rows(const lm_embed p) {
     id[u] = row < p.n ? lm_id((ga_long)*lm_at(p.ids, row * p.id_step), p.ignore, LM_NONE, p.v) : -3;
     if (id[u] == -2) *p.err = -1;
   }
-  if (col >= p.d || p.v == 0) return;
+  if (col >= p.d) return;
   /* Loads are unconditional, so that all of them are in flight at once: rows
    * of no token fetch row 0, and the lane at a row's end fetches the row's
    * last LM_C columns, of which it writes its own. */
   const ga_long from = p.d >= LM_C && p.d - col < LM_C ? p.d - LM_C : col;
   const ga_int skip = (ga_int)(col - from);
   float y[LM_ROWS][LM_C];
-  if (p.d >= LM_C) {
+  if (p.d >= LM_C && p.v != 0) {
 #pragma unroll
     for (int u = 0; u < LM_ROWS; u++) lm_load(lm_at(p.table, (id[u] > 0 ? id[u] : 0) * p.table_row) + from, y[u]);
   } else {
 #pragma unroll
     for (int u = 0; u < LM_ROWS; u++)
 #pragma unroll
-      for (int e = 0; e < LM_C; e++) y[u][e] = e < p.d ? (float)lm_get(lm_at(p.table, (id[u] > 0 ? id[u] : 0) * p.table_row)[e]) : 0.0f;
+      for (int e = 0; e < LM_C; e++) y[u][e] = e < p.d && p.v != 0 ? (float)lm_get(lm_at(p.table, (id[u] > 0 ? id[u] : 0) * p.table_row)[e]) : 0.0f;
   }
 #pragma unroll
   for (int u = 0; u < LM_ROWS; u++) {

@@ -143,6 +143,14 @@ def test_embedding_of_nothing(ctx):
         ga.embedding(gpuarray.zeros((0, 3), context=ctx), gpuarray.zeros((2,), "int64", context=ctx))
 
 
+@pytest.mark.parametrize("d", [3, 40])
+def test_embedding_of_no_token_in_an_empty_table(ctx, d):
+    out = gpuarray.array(np.full((5, d), 7, np.float32), context=ctx)
+    ids = gpuarray.array(np.full(5, -100), context=ctx)
+    ga.embedding(gpuarray.zeros((0, d), context=ctx), ids, ignore=-100, out=out)
+    assert np.all(np.asarray(out) == 0)
+
+
 # ---- its gradient -----------------------------------------------------------------------------------
 
 def check_embedding_grad(got, dout, ids, v, scale, ignore, grad, base=None):
