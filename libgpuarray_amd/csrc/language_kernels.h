@@ -37,7 +37,9 @@ template <class T> LM_FN T *lm_at(T *base, ga_long bytes) {
 }
 
 /* An id in [0, v); -1: no token; -2: out of range. */
-LM_FN ga_long lm_id(ga_long id, ga_long ignore, ga_long none, ga_long v) {
+template <class T> LM_FN ga_long lm_id(T raw, ga_long ignore, ga_long none, ga_long v) {
+  ga_long id = (ga_long)raw;
+  if ((T)-1 > (T)0 && id < 0) return -2;   /* an unsigned id of 2^63 or more does not count from the end */
   if (ignore != none && id == ignore) return -1;
   if (id < 0) id += v;
   return id >= 0 && id < v ? id : -2;
@@ -194,7 +196,7 @@ KERNEL void __launch_bounds__(256) lm_embed_rows(const lm_embed p) {
 #pragma unroll
   for (int u = 0; u < LM_ROWS; u++) {
     const ga_long row = row0 + u * side;
-    id[u] = row < p.n ? lm_id((ga_long)*lm_at(p.ids, row * p.id_step), p.ignore, LM_NONE, p.v) : -3;
+    id[u] = row < p.n ? lm_id(*lm_at(p.ids, row * p.id_step), p.ignore, LM_NONE, p.v) : -3;
     if (id[u] == -2) *p.err = -1;
   }
   if (col >= p.d) return;
@@ -278,7 +280,7 @@ LM_FN void lm_clear(const lm_sorting &p, ga_uint first) {
 }
 
 LM_FN ga_uint lm_first_key(const lm_sorting &p, ga_uint i) {
-  const ga_long id = lm_id((ga_long)*lm_at(p.ids, (ga_long)i * p.id_step), p.ignore, LM_NONE, p.v);
+  const ga_long id = lm_id(*lm_at(p.ids, (ga_long)i * p.id_step), p.ignore, LM_NONE, p.v);
   if (id == -2) *p.err = -1;
   return id < 0 ? (ga_uint)p.v : (ga_uint)id;
 }
@@ -550,7 +552,7 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
   const ga_uint parts = (p.tiles + 3) / 4, part = GID_0 % parts;
   const ga_uint tiles = p.tiles - part * 4 < 4 ? p.tiles - part * 4 : 4;
   const ga_long r0 = (ga_long)(GID_0 / parts) * p.rows;
-  const ga_long id = LID_0 < p.n ? lm_id((ga_long)*lm_at(p.ids, (ga_long)LID_0 * p.id_step), p.ignore, LM_NONE, p.v) : -1;
+  const ga_long id = LID_0 < p.n ? lm_id(*lm_at(p.ids, (ga_long)LID_0 * p.id_step), p.ignore, LM_NONE, p.v) : -1;
   if (id == -2) *p.err = -1;
   const ga_uint row = id >= r0 && id < r0 + p.rows ? (ga_uint)(id - r0) : LM_FEW_ROWS;
   for (ga_uint k = 0; k < p.rows; k++) {
@@ -1043,10 +1045,10 @@ struct lm_token {
   ga_long id;   /* -1: no token, -2: out of range */
   float x;
 };
-LM_FN ga_long lm_token_id(const lm_logprobs &p, ga_long r) {
-  return p.ids != nullptr ? (ga_long)*lm_at(p.ids, r * p.id_step) : 0;
+LM_FN LM_ID lm_token_id(const lm_logprobs &p, ga_long r) {
+  return p.ids != nullptr ? *lm_at(p.ids, r * p.id_step) : 0;
 }
-LM_FN lm_token lm_token_of(const lm_logprobs &p, ga_long r, ga_long id) {
+LM_FN lm_token lm_token_of(const lm_logprobs &p, ga_long r, LM_ID id) {
   lm_token k = {-1, 0.0f};
   if (p.ids != nullptr) {
     k.id = lm_id(id, p.ignore, LM_NONE, p.v);
@@ -1155,7 +1157,7 @@ LM_FN void lm_join_pieces(const lm_logprobs &p, ga_long r) {
   lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
   ga_ulong list = 0;
   /* Every load has a long way: all of them go out before the first is used. */
-  const ga_long token_id = lm_token_id(p, r);
+  const LM_ID token_id = lm_token_id(p, r);
   const auto word = [&](ga_uint i, ga_uint place) {
     return lm_fetch((GLOBAL_MEM const ga_ulong *)(from + (ga_size)(i < p.pieces ? i : 0) * p.partial_bytes) + place);
   };
@@ -1235,7 +1237,7 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
   lm_state a = {LM_LOWEST, 0.0f, 0.0f, 0.0f};
   lm_best best = {0, 0, 0, 0, -INFINITY};
 #if !LM_SPLIT
-  const ga_long token_id = lm_token_id(p, r);
+  const LM_ID token_id = lm_token_id(p, r);
 #endif
   lm_u4 raw[LM_U];
   const auto fetch = [&](ga_uint base) {   /* unconditional loads: all of them in flight */
@@ -1366,7 +1368,7 @@ KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad 
   float g = 0.0f, gh = 0.0f, h = 0.0f;
   ga_long id = -1;
   if (p.ids != nullptr) {
-    id = lm_id((ga_long)*lm_at(p.ids, r * p.id_step), p.ignore, LM_NONE, p.v);
+    id = lm_id(*lm_at(p.ids, r * p.id_step), p.ignore, LM_NONE, p.v);
     if (id == -2 && segment == 0 && lane == 0) *p.err = -1;
     if (id >= 0) g = *lm_at(p.dlogp, r * p.dlogp_step);
   }

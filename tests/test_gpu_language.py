@@ -100,6 +100,26 @@ def test_embedding_id_types(ctx, id_type):
     assert np.array_equal(got, w[ids.astype(int)])
 
 
+def test_unsigned_ids_do_not_count_from_the_end(ctx):
+    """2^64 - 1 is out of range, and is not `ignore` = -1 either."""
+    w = np.arange(12, dtype=np.float32).reshape(4, 3)
+    table, ids = gpuarray.array(w, context=ctx), gpuarray.array(np.array([1, 2 ** 64 - 1], np.uint64), context=ctx)
+    for ignore in (None, -1):
+        out = gpuarray.array(np.full((2, 3), 7, np.float32), context=ctx)
+        with pytest.raises(IndexError):
+            ga.embedding(table, ids, out=out, ignore=ignore)
+        assert np.array_equal(np.asarray(out), [w[1], [7, 7, 7]])
+        with pytest.raises(IndexError):
+            ga.token_logprobs(table[:2], ids, ignore=ignore)
+        grad = gpuarray.zeros((4, 3), context=ctx)
+        with pytest.raises(IndexError):
+            ga.embedding_grad(table[:2], ids, grad, ignore=ignore)
+        assert np.array_equal(np.asarray(grad), [[0, 0, 0], w[0], [0, 0, 0], [0, 0, 0]])
+        stats, one = gpuarray.zeros((2, 2), context=ctx), gpuarray.array(np.ones(2, np.float32), context=ctx)
+        with pytest.raises(IndexError):
+            ga.token_logprobs_grad(table[:2], ids, stats, one, ignore=ignore)
+
+
 @pytest.mark.parametrize("pitch,flip,step", [(3, False, 2), (0, True, -1), (13, True, 1), (1, False, 0)])
 def test_embedding_layouts(ctx, pitch, flip, step):
     rng = np.random.default_rng(5)
