@@ -313,7 +313,9 @@ int lm_check_error(gpucontext *ctx, gpudata *errbuf) {
 
 int no_memory(gpucontext *ctx) { return ga_err_set(ctx->err, GA_MEMORY_ERROR, "Out of memory"); }
 
-const size_t MAX_GROUPS = 0x7fffffff;
+const size_t MAX_ROWS = 0x7fffffff;   // rows or tokens that 32-bit numbers of them allow
+// a launch has fewer than 2^32 lanes
+inline size_t max_groups(size_t lanes) { return 0xffffffffu / lanes; }
 
 }  // namespace
 
@@ -359,7 +361,7 @@ static int embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, 
   unsigned lanes_log2 = 0;
   while (lanes_log2 < 8 && ((size_t)1 << lanes_log2) < row_lanes) lanes_log2++;
   const size_t row_groups = (n + ((size_t)1024 >> lanes_log2) - 1) / ((size_t)1024 >> lanes_log2);
-  if (row_groups > MAX_GROUPS || segments > MAX_GROUPS / row_groups) return c.fail(GA_XLARGE_ERROR, "too many elements");
+  if (row_groups > max_groups(256) || segments > max_groups(256) / row_groups) return c.fail(GA_XLARGE_ERROR, "too many elements");
   GpuKernel *k;
   gpudata *errbuf = nullptr;
   int err = lm_kernel(ctx, lm_variant(LM_EMBED, table->typecode, out->typecode, ids->typecode, 0), "lm_embed_rows",
@@ -393,7 +395,7 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   c.scale(scale, false);
   if (c.err != GA_NO_ERROR) return c.err;
   if (d == 0 || (v == 0 && n == 0)) return GA_NO_ERROR;
-  if (v > MAX_GROUPS || n > MAX_GROUPS) return c.fail(GA_XLARGE_ERROR, "too many rows");
+  if (v > MAX_ROWS || n > MAX_ROWS) return c.fail(GA_XLARGE_ERROR, "too many rows");
 
   const size_t osize = gpuarray_get_elsize(grad->typecode);
   const size_t cols = 64 * 16 / std::max(osize, gpuarray_get_elsize(dout->typecode));   // of a wavefront
@@ -414,7 +416,7 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
     GpuKernel *kfew = nullptr;
     err = lm_kernel(ctx, vg, "lm_embed_grad_few", sizeof(embed_grad_args), &kfew);
     const size_t parts = (tiles + 3) / 4, row_groups = v ? (v + a.rows - 1) / a.rows : 1;
-    if (parts > MAX_GROUPS / row_groups) return c.fail(GA_XLARGE_ERROR, "too many elements");
+    if (parts > max_groups(256) / row_groups) return c.fail(GA_XLARGE_ERROR, "too many elements");
     if (err == GA_NO_ERROR) err = lm_launch(kfew, row_groups * parts, 256, &a);
     return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
   }
@@ -425,7 +427,7 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   size_t chunk = 8;
   while (chunk < 256 && n / (chunk * 2) / per_wave * tiles >= (narrow ? 2048u : 8192u)) chunk *= 2;
   const size_t chunks = (n + chunk - 1) / chunk;
-  if (chunks * tiles > MAX_GROUPS) return c.fail(GA_XLARGE_ERROR, "too many elements");
+  if (tiles > max_groups(256) / chunks) return c.fail(GA_XLARGE_ERROR, "too many elements");
   // The digits: as few passes as ten bits a digit allow.
   unsigned bits = 1;
   while (v >> bits != 0) bits++;
@@ -566,7 +568,7 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
     return c.fail(GA_VALUE_ERROR, "more alternatives than the vocabulary or GA_TOKEN_LOGPROBS_MAX_TOP has");
   if (t == 0 || (logp == nullptr && entropy == nullptr && stats == nullptr && top == 0)) return GA_NO_ERROR;
   if (v == 0) return c.fail(GA_VALUE_ERROR, "empty vocabulary");
-  if (t > MAX_GROUPS || v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many rows or columns");
+  if (v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many columns");
   // A row that a wavefront covers in two rounds of loads belongs to one
   // wavefront, longer ones to a group, which grows while there are too few
   // rows to fill the chip; below that, rows are cut in pieces of at least two
@@ -586,6 +588,8 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
     pieces = (row_chunks + piece_chunks - 1) / piece_chunks;
   }
   const bool split = pieces > 1;
+  const size_t groups = split ? t * pieces : lanes < 256 ? (t + 3) / 4 : t;
+  if (groups > max_groups(std::max(lanes, 256u))) return c.fail(GA_XLARGE_ERROR, "too many rows");
   const size_t partial_bytes = 16 + 8 * top;
   const lm_variant var(LM_LOGPROBS, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT,
                        logprobs_extra(lanes, entropy != nullptr, top != 0, split));
@@ -655,11 +659,11 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
   c.scale(scale, true);
   if (c.err != GA_NO_ERROR) return c.err;
   if (t == 0 || v == 0) return GA_NO_ERROR;
-  if (t > MAX_GROUPS || v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many rows or columns");
+  if (v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many columns");
   // a wavefront's share of a row: 32 elements a lane (and one chunk more, for rows that start inside one)
   const size_t esize = gpuarray_get_elsize(logits->typecode);
   const size_t segments = (v * esize / 16 + 2 + 128 * esize - 1) / (128 * esize);
-  if (segments > 2 * MAX_GROUPS / t) return c.fail(GA_XLARGE_ERROR, "too many elements");
+  if (segments > 4 * max_groups(256) / t) return c.fail(GA_XLARGE_ERROR, "too many elements");
   GpuKernel *k;
   gpudata *errbuf = nullptr;
   int err = lm_kernel(ctx, lm_variant(LM_LOGPROBS_GRAD, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT, entropy != nullptr),
@@ -736,7 +740,7 @@ static int norm_arrays(checker &c, GpuArray **rs, const GpuArray **as, size_t n,
     }
     if (count == 0) continue;
     const uint64_t per = NORM_PIECE * (16 / size), p = (count + per - 1) / per;
-    if (p > 0x70000000) return c.fail(GA_XLARGE_ERROR, "an array is too large");
+    if (p > max_groups(256)) return c.fail(GA_XLARGE_ERROR, "an array is too large");
     tensor_arg t = {at(a), at(r), (int64_t)count, (uint32_t)p,   // (`first` holds the count of pieces until a table is made)
                     a->typecode == GA_FLOAT ? 0u : a->typecode == GA_HALF ? 1u : a->typecode == GA_BFLOAT16 ? 2u : 3u};
     plan->tensors.push_back(t);
@@ -837,7 +841,7 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
   std::vector<norm_table> tables;
   for (size_t i = 0; i < plan.tensors.size(); i++) {
     const uint32_t p = plan.tensors[i].first;
-    if (tables.empty() || tables.back().n == LM_TENSORS || tables.back().pieces + (uint64_t)p > 0x7fffffff)
+    if (tables.empty() || tables.back().n == LM_TENSORS || tables.back().pieces + (uint64_t)p > max_groups(256))
       tables.push_back({&plan.tensors[i], nullptr, 0, 0});
     plan.tensors[i].first = tables.back().pieces;
     tables.back().n++;
@@ -869,7 +873,7 @@ static int global_norm_new(GpuGlobalNorm **out, gpucontext *ctx, const GpuArray 
     const uint32_t p = t.first;
     t.first = (uint32_t)pieces;
     pieces += p;
-    if (pieces > 0x7fffffff) return c.fail(GA_XLARGE_ERROR, "the arrays are too large together");
+    if (pieces > max_groups(256)) return c.fail(GA_XLARGE_ERROR, "the arrays are too large together");
   }
   g->pieces = (uint32_t)pieces;
   g->held.reserve(2 * n);

@@ -973,6 +973,25 @@ def test_refusals(ctx):
         assert ctx.last_launch_hash() == before, what
 
 
+def test_refusals_of_more_lanes_than_a_launch_has(ctx):
+    """2^26 rows of one column each have a wavefront, 2^28 rows of a gradient of few tokens 16 a group."""
+    t = 1 << 26
+    logits = gpuarray.from_strided(gpuarray.zeros((1,), "float16", context=ctx), 0, (t, 1), (0, 2))
+    stats = gpuarray.from_strided(gpuarray.zeros((2,), context=ctx), 0, (t, 2), (0, 4))
+    ids = gpuarray.from_strided(gpuarray.zeros((1,), "int32", context=ctx), 0, (t,), (0,))
+    dlogp = gpuarray.from_strided(gpuarray.zeros((1,), context=ctx), 0, (t,), (0,))
+    logp, dlogits = gpuarray.empty((t,), context=ctx), gpuarray.empty((t, 1), "float16", context=ctx)
+    grad = gpuarray.empty((1 << 28, 1), "float16", context=ctx)
+    before = ctx.last_launch_hash()
+    for call in (lambda: ga.token_logprobs(logits, ids, out=ga.TokenLogprobs(logp, None, None, None, None)),
+                 lambda: ga.token_logprobs_grad(logits, ids, stats, dlogp, out=dlogits),
+                 lambda: ga.embedding_grad(logits[:3], ids[:3], grad)):
+        with pytest.raises(_lib.GpuArrayException) as e:
+            call()
+        assert e.value.code == _lib.GA_XLARGE_ERROR
+        assert ctx.last_launch_hash() == before
+
+
 def test_refusal_of_arrays_of_two_contexts(ctx):
     second = ga.init("hip0")
     table, ids = gpuarray.zeros((9, 8), context=ctx), gpuarray.zeros((4,), "int64", context=second)

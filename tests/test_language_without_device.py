@@ -10,6 +10,7 @@ import pytest
 from test_host_logic_without_device import ROOT, build, mock_runtime  # noqa: F401  (fixtures)
 
 HOST_ONLY = ["tests/test_gpu_language.py::test_refusals",
+             "tests/test_gpu_language.py::test_refusals_of_more_lanes_than_a_launch_has",
              "tests/test_gpu_language.py::test_refusal_of_arrays_of_two_contexts"]
 
 
