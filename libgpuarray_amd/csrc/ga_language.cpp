@@ -179,6 +179,17 @@ int lm_scratch(gpucontext *ctx, size_t bytes, char **out) {
   return GA_NO_ERROR;
 }
 
+// The context's counters, zeros that the groups of a launch count on and that the last one zeroes.
+int lm_counters(gpucontext *ctx, void **out) {
+  gpudata *b = ga_hip_redux_counters(ctx);
+  if (b == nullptr)
+    return ga_hip_capturing(ctx) ? ga_err_set(ctx->err, GA_UNSUPPORTED_ERROR,
+                                              "The counters are not made yet and the stream records a graph: call once before recording")
+                                 : ctx->err->code;
+  *out = b->devptr;
+  return GA_NO_ERROR;
+}
+
 // ---- checks of arguments -------------------------------------------------------
 
 inline char *at(const GpuArray *a) { return (char *)a->data->devptr + a->offset; }
@@ -288,6 +299,11 @@ struct checker {
     if (err == GA_NO_ERROR && a != nullptr && b != nullptr && overlap(a, b))
       fail(GA_VALUE_ERROR, "overlaps another argument", arg);
   }
+  // reading the error word waits, which a stream that records a graph does not allow
+  void waits(int check_error) {
+    if (err == GA_NO_ERROR && check_error && ga_hip_capturing(ctx))
+      fail(GA_UNSUPPORTED_ERROR, "check_error waits, and the stream records a graph");
+  }
   // a scale that a float holds
   void scale(double s, bool positive) {
     if (err == GA_NO_ERROR && (!std::isfinite((float)s) || (positive && !((float)s > 0.0f))))
@@ -353,6 +369,7 @@ static int embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, 
   c.apart(out, table, "out");
   c.apart(out, ids, "out");
   c.scale(scale, false);
+  c.waits(check_error);
   if (c.err != GA_NO_ERROR) return c.err;
   if (n == 0 || d == 0) return GA_NO_ERROR;
   // lanes of a row: a power of two, each with 16 bytes of the narrower side; a lane moves four rows
@@ -393,6 +410,7 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   c.apart(grad, dout, "grad");
   c.apart(grad, ids, "grad");
   c.scale(scale, false);
+  c.waits(check_error);
   if (c.err != GA_NO_ERROR) return c.err;
   if (d == 0 || (v == 0 && n == 0)) return GA_NO_ERROR;
   if (v > MAX_ROWS || n > MAX_ROWS) return c.fail(GA_XLARGE_ERROR, "too many rows");
@@ -562,6 +580,7 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
     for (int j = 0; j < i; j++) c.apart(results[i], results[j], names[i]);
   }
   c.scale(scale, true);
+  c.waits(check_error);
   if (c.err != GA_NO_ERROR) return c.err;
   const size_t top = top_ids ? top_ids->dimensions[1] : 0;
   if (top > GA_TOKEN_LOGPROBS_MAX_TOP || top > v)
@@ -572,7 +591,7 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
   // A row that a wavefront covers in two rounds of loads belongs to one
   // wavefront, longer ones to a group, which grows while there are too few
   // rows to fill the chip; below that, rows are cut in pieces of at least two
-  // chunks per lane and joined by a second launch.
+  // chunks per lane, of which the last one to end joins them all.
   const size_t row_chunks = v * gpuarray_get_elsize(logits->typecode) / 16 + 1;
   const size_t cus = ga_hip_numprocs(ctx) ? ga_hip_numprocs(ctx) : 256;
   unsigned lanes = 64;
@@ -581,7 +600,7 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
     while (lanes < 1024 && t * lanes < cus * 1024 && row_chunks > 8 * lanes) lanes *= 2;
   }
   size_t pieces = 1, piece_chunks = row_chunks;
-  if (row_chunks > 512 && t * 2 <= cus) {
+  if (row_chunks > 512 && t * 2 <= cus && t <= ga_hip_redux_counters_max) {
     lanes = 256;
     pieces = std::min((2 * cus + t - 1) / t, (row_chunks + 511) / 512);
     piece_chunks = (row_chunks + pieces - 1) / pieces;
@@ -593,14 +612,12 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
   const size_t partial_bytes = 16 + 8 * top;
   const lm_variant var(LM_LOGPROBS, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT,
                        logprobs_extra(lanes, entropy != nullptr, top != 0, split));
-  GpuKernel *k, *kjoin = nullptr;
+  GpuKernel *k;
   gpudata *errbuf = nullptr;
   char *scratch = nullptr;
+  void *counters = nullptr;   // the last piece of a row joins them
   int err = lm_kernel(ctx, var, "lm_logprobs_rows", sizeof(logprobs_args), &k);
-  // the last piece of a row joins them, or, where there are no counters, a second launch does
-  gpudata *counters = split && t <= ga_hip_redux_counters_max ? ga_hip_redux_counters(ctx) : nullptr;
-  if (err == GA_NO_ERROR && split && counters == nullptr)
-    err = lm_kernel(ctx, var, "lm_logprobs_join", sizeof(logprobs_args), &kjoin);
+  if (err == GA_NO_ERROR && split) err = lm_counters(ctx, &counters);
   if (err == GA_NO_ERROR && split) err = lm_scratch(ctx, t * pieces * partial_bytes, &scratch);
   if (err == GA_NO_ERROR) err = lm_errbuf(ctx, logits, &errbuf);
   if (err != GA_NO_ERROR) return err;
@@ -612,13 +629,8 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
                      step(top_ids, 1), (int64_t)t, (int64_t)v, ignore, (float)scale,
                      (float)((double)(float)scale * 1.4426950408889634), (int32_t)top,
                      top_ids != nullptr && top_ids->typecode == GA_LONG, (uint32_t)pieces, (uint32_t)piece_chunks,
-                     (uint32_t)partial_bytes, 0, counters ? counters->devptr : nullptr};
-  if (split) {
-    err = lm_launch(k, t * pieces, lanes, &a);
-    if (err == GA_NO_ERROR && counters == nullptr) err = lm_launch(kjoin, t, lanes, &a);
-  } else {
-    err = lanes < 256 ? lm_launch(k, (t + 3) / 4, 256, &a) : lm_launch(k, t, lanes, &a);
-  }
+                     (uint32_t)partial_bytes, 0, counters};
+  err = lm_launch(k, groups, std::max(lanes, 256u), &a);
   return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;
 }
 
@@ -657,6 +669,7 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
   c.apart(dlogits, stats, "dlogits");
   if (c.err == GA_NO_ERROR && !same_place(dlogits, logits)) c.apart(dlogits, logits, "dlogits");
   c.scale(scale, true);
+  c.waits(check_error);
   if (c.err != GA_NO_ERROR) return c.err;
   if (t == 0 || v == 0) return GA_NO_ERROR;
   if (v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many columns");
@@ -770,7 +783,8 @@ static int norm_apart(checker &c, const norm_plan &plan, const GpuArray *norm) {
   return GA_NO_ERROR;
 }
 
-// Launches on tables: of a list of arrays cut into argument lists, or one in device memory.
+// Launches on tables: of a list of arrays cut into argument lists, or one in
+// device memory.  There is one at least, with no arrays if need be.
 struct norm_table {
   const tensor_arg *tensors;   // NULL: in device memory
   const void *device;
@@ -782,13 +796,13 @@ static int norm_run(checker &c, const std::vector<norm_table> &tables, bool clip
   const size_t size = by_table ? sizeof(table_args) : sizeof(tensors_args);
   const lm_variant vn(LM_NORM, GA_FLOAT, GA_FLOAT, GA_INT, by_table), vc(LM_CLIP, GA_FLOAT, GA_FLOAT, GA_INT, by_table);
   char *scratch = nullptr;
-  GpuKernel *kpieces = nullptr, *kfinal = nullptr, *kclip = nullptr;
+  void *counters = nullptr;
+  GpuKernel *kpieces = nullptr, *kclip = nullptr;
   int err = lm_kernel(ctx, vn, "lm_norm_pieces", size, &kpieces);
   if (err == GA_NO_ERROR && clip) err = lm_kernel(ctx, vc, "lm_clip_pieces", size, &kclip);
-  if (err == GA_NO_ERROR)
-    err = lm_scratch(ctx, 256 + (tables.size() + 1) * NORM_MAX_GROUPS * sizeof(double), &scratch);
+  if (err == GA_NO_ERROR) err = lm_counters(ctx, &counters);
+  if (err == GA_NO_ERROR) err = lm_scratch(ctx, 256 + tables.size() * NORM_MAX_GROUPS * sizeof(double), &scratch);
   if (err != GA_NO_ERROR) return err;
-  gpudata *counters = ga_hip_redux_counters(ctx);
 
   tensors_args args;
   table_args *const short_args = (table_args *)&args;
@@ -806,25 +820,18 @@ static int norm_run(checker &c, const std::vector<norm_table> &tables, bool clip
     if (t.tensors != nullptr) memcpy(args.tensors, t.tensors, t.n * sizeof(tensor_arg));
     else short_args->tensors = t.device;
   };
-  // (without counters, while a graph is recorded before they are made, a launch
-  // of its own finishes the norm)
-  bool finished = false;
+  // the last table's groups count themselves in, and the last of those finishes the norm
   for (size_t i = 0; i < tables.size() && err == GA_NO_ERROR; i++) {
     take(tables[i]);
-    const size_t groups = std::min<size_t>(a.pieces, NORM_MAX_GROUPS);
+    const size_t groups = std::min<size_t>(std::max(a.pieces, 1u), NORM_MAX_GROUPS);
     a.partial0 = a.npartials;
     a.npartials += (uint32_t)groups;
-    finished = i + 1 == tables.size() && counters != nullptr;
-    a.counter = finished ? counters->devptr : nullptr;
+    a.counter = i + 1 == tables.size() ? counters : nullptr;
     err = lm_launch(kpieces, groups, 256, &args);
-  }
-  if (err == GA_NO_ERROR && !finished) {
-    err = lm_kernel(ctx, vn, "lm_norm_final", size, &kfinal);
-    if (err == GA_NO_ERROR) err = lm_launch(kfinal, 1, 1024, &args);
   }
   for (size_t i = 0; i < tables.size() && err == GA_NO_ERROR && clip; i++) {
     if (tables.size() > 1) take(tables[i]);
-    err = lm_launch(kclip, a.pieces, 256, &args);
+    if (a.pieces != 0) err = lm_launch(kclip, a.pieces, 256, &args);
   }
   return err;
 }
@@ -847,6 +854,7 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
     tables.back().n++;
     tables.back().pieces += p;
   }
+  if (tables.empty()) tables.push_back({nullptr, nullptr, 0, 0});
   return norm_run(c, tables, rs != nullptr, max_norm, norm);
 }
 
@@ -896,11 +904,9 @@ static int global_norm_call(const GpuGlobalNorm *g, bool clip, double max_norm, 
   if (std::isnan(max_norm) || max_norm < 0) return c.fail(GA_VALUE_ERROR, "max_norm must be 0 or above");
   if (clip && !g->clips) return c.fail(GA_INVALID_ERROR, "the operator was made without results");
   if (norm_check(c, norm) != GA_NO_ERROR || norm_apart(c, g->plan, norm) != GA_NO_ERROR) return c.err;
-  std::vector<norm_table> tables;
-  if (g->table != nullptr)
-    tables.push_back({nullptr, g->table->devptr, (uint32_t)g->plan.tensors.size(), g->pieces});
-  else if (norm == nullptr)
-    return GA_NO_ERROR;
+  if (g->table == nullptr && norm == nullptr) return GA_NO_ERROR;
+  const std::vector<norm_table> tables = {
+      {nullptr, g->table ? g->table->devptr : nullptr, (uint32_t)g->plan.tensors.size(), g->pieces}};
   return norm_run(c, tables, clip, max_norm, norm);
 }
 

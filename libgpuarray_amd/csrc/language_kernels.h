@@ -753,7 +753,7 @@ struct lm_logprobs {
   ga_int top, top_long;
   ga_uint pieces, piece_chunks, partial_bytes;
   ga_uint pad;
-  GLOBAL_MEM ga_uint *counters;  /* one zero per row, or NULL: lm_logprobs_join follows */
+  GLOBAL_MEM ga_uint *counters;  /* one zero per row in pieces */
 };
 
 /* Softmax statistics of some elements x of a row.  With R(m) = by * m, rounded,
@@ -1300,7 +1300,6 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
     if (lane < p.top) lm_publish(words + 2 + lane, list);
 #endif
   }
-  if (p.counters == nullptr) return;
   LOCAL_MEM ga_uint last;
   if (LID_0 < 64) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   /* (of every lane of the wavefront) */
@@ -1313,9 +1312,6 @@ KERNEL void __launch_bounds__(LM_LANES < 256 ? 256 : LM_LANES) lm_logprobs_rows(
 #endif
 }
 
-#if LM_SPLIT
-KERNEL void __launch_bounds__(LM_LANES) lm_logprobs_join(const lm_logprobs p) { lm_join_pieces(p, GID_0); }
-#endif
 #endif
 
 #if LM_KIND == LM_K_LOGPROBS_GRAD
@@ -1435,7 +1431,7 @@ struct lm_tensors {
   GLOBAL_MEM double *partials;   /* sums of squares, one per group */
   GLOBAL_MEM double *result;     /* the factor */
   GLOBAL_MEM void *norm;
-  GLOBAL_MEM ga_uint *counter;   /* a zero that the last table's groups count on, or NULL: lm_norm_final follows */
+  GLOBAL_MEM ga_uint *counter;   /* a zero that the last table's groups count on; NULL for the others */
   double max_norm;
   ga_uint partial0, npartials;
   ga_uint n, pieces, piece;
@@ -1457,6 +1453,7 @@ LM_FN ga_uint lm_find(const lm_tensors &p, ga_uint piece) {
   }
   return (ga_uint)__builtin_amdgcn_readfirstlane((int)from);
 }
+#define LM_GROUP 256
 #define LM_BY_TYPE(type, F)       \
   switch (type) {                 \
     case 0: F(ga_float); break;   \
@@ -1471,16 +1468,16 @@ LM_FN double lm_lane_xor(double v, int mask) {
   const ga_uint hi = (ga_uint)__builtin_amdgcn_ds_bpermute(from, (int)(ga_uint)(b >> 32));
   return __builtin_bit_cast(double, (ga_ulong)hi << 32 | lo);
 }
-/* the sum over a group of WAVES wavefronts, in lane 0 */
-template <int WAVES> LM_FN double lm_group_sum(double v) {
-  LOCAL_MEM double part[WAVES];
+/* the sum over a group */
+LM_FN double lm_group_sum(double v) {
+  LOCAL_MEM double part[LM_GROUP / 64];
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v += lm_lane_xor(v, d);
   if ((LID_0 & 63) == 0) part[LID_0 >> 6] = v;
   local_barrier();
   v = part[0];
 #pragma unroll
-  for (int w = 1; w < WAVES; w++) v += part[w];
+  for (int w = 1; w < LM_GROUP / 64; w++) v += part[w];
   return v;
 }
 LM_FN void lm_unpack(const lm_u4 &q, double *y, ga_double) {
@@ -1494,7 +1491,6 @@ template <> struct lm_wide<ga_double> { typedef double type; };
 #endif
 
 #if LM_KIND == LM_K_NORM
-#define LM_GROUP 256
 #define LM_U 8   /* chunks in flight per lane */
 
 /* The squares of n elements of type T, summed in 64 bits by the group:
@@ -1540,12 +1536,12 @@ template <class T> LM_FN double lm_squares(GLOBAL_MEM const T *x, ga_long n) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 /* The norm and the factor from all partial sums, by one group. */
-template <int LANES> LM_FN void lm_norm_of_partials(const lm_tensors &p) {
+LM_FN void lm_norm_of_partials(const lm_tensors &p) {
   double s = 0.0;
-  for (ga_uint k = LID_0; k < p.npartials; k += LANES)
+  for (ga_uint k = LID_0; k < p.npartials; k += LM_GROUP)
     s += __builtin_bit_cast(double, lm_fetch((GLOBAL_MEM const ga_ulong *)p.partials + k));
   local_barrier();   /* (the LDS of an earlier sum is free again) */
-  s = lm_group_sum<LANES / 64>(s);
+  s = lm_group_sum(s);
   if (LID_0 == 0) {
     const double norm = __builtin_sqrt(s);
     p.result[0] = norm > p.max_norm && norm < (double)INFINITY ? p.max_norm / norm : 1.0;
@@ -1577,20 +1573,18 @@ KERNEL void __launch_bounds__(LM_GROUP) lm_norm_pieces(const lm_tensors p) {
       piece = stop;
     }
   }
-  s = lm_group_sum<LM_GROUP / 64>(s);
+  s = lm_group_sum(s);
   LOCAL_MEM ga_uint last;
   if (LID_0 == 0) {
     lm_publish((GLOBAL_MEM ga_ulong *)p.partials + p.partial0 + GID_0, __builtin_bit_cast(ga_ulong, s));
     last = p.counter != nullptr && lm_count_in(p.counter, GDIM_0);
   }
   local_barrier();
-  if (last) lm_norm_of_partials<LM_GROUP>(p);
+  if (last) lm_norm_of_partials(p);
 }
-KERNEL void __launch_bounds__(1024) lm_norm_final(const lm_tensors p) { lm_norm_of_partials<1024>(p); }
 #endif
 
 #if LM_KIND == LM_K_CLIP
-#define LM_GROUP 256
 #define LM_U 4
 
 LM_FN void lm_scaled(const lm_u4 &q, lm_u4a &r, double by, ga_double) {

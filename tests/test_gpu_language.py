@@ -812,6 +812,12 @@ def test_language_operators_replay_from_a_graph(ctx):
         issue(replayed)
         with pytest.raises(_lib.UnsupportedException):
             ga.GlobalNorm([eager["d"]])                          # its table cannot be copied now
+        for call in (lambda: ga.embedding(table, ids, out=replayed["h"]),        # what waits is refused, and breaks nothing
+                     lambda: ga.embedding_grad(replayed["d"], ids, replayed["g"]),
+                     lambda: ga.token_logprobs(replayed["h"], targets, out=ga.TokenLogprobs(replayed["logp"], None, None, None, None)),
+                     lambda: ga.token_logprobs_grad(replayed["h"], targets, replayed["stats"], dlogp, out=replayed["d"])):
+            with pytest.raises(_lib.UnsupportedException):
+                call()
     finally:
         rc = hip.hipStreamEndCapture(stream, C.byref(graph))
     assert rc == 0
