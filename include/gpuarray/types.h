@@ -49,9 +49,9 @@ enum GPUARRAY_TYPES {
   GA_HALF2 = 304, GA_HALF4 = 305, GA_HALF8 = 306, GA_HALF16 = 307,
   GA_NVEC = 308,
 
-  /* bfloat16: the upper half of a float.  Not in the reference; the last code
-   * below the user-registered types. */
-  GA_BFLOAT16 = 511,
+  /* bfloat16: the upper half of a float.  Not in the reference, which leaves
+   * the codes from here to the user-registered types without a type. */
+  GA_BFLOAT16 = 320,
 
   GA_ENDVEC = 512   /* user-registered types start here */
 };

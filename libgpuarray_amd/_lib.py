@@ -39,7 +39,7 @@ GA_BOOL, GA_BYTE, GA_UBYTE, GA_SHORT, GA_USHORT = 0, 1, 2, 3, 4
 GA_INT, GA_UINT, GA_LONG, GA_ULONG = 5, 6, 7, 8
 GA_FLOAT, GA_DOUBLE, GA_CFLOAT, GA_CDOUBLE = 11, 12, 14, 15
 GA_HALF, GA_SIZE, GA_SSIZE = 23, 24, 25
-GA_BFLOAT16 = 511
+GA_BFLOAT16 = 320
 
 GA_C_CONTIGUOUS = 0x0001
 GA_F_CONTIGUOUS = 0x0002

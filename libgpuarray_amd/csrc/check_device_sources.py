@@ -252,7 +252,7 @@ def main():
         t += 1
     # operators of language models: (operator, operand, result, ids) as the library packs them
     gen_l = ext(b"hip_language_source", C.c_void_p, [C.c_ulonglong])
-    GA_BFLOAT16 = 511
+    GA_BFLOAT16 = 320
     lm = 0
     for kind in range(6):
         for x, o in [(GA_FLOAT, GA_FLOAT), (GA_BFLOAT16, GA_FLOAT), (GA_HALF, GA_BFLOAT16)]:
