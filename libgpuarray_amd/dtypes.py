@@ -22,7 +22,17 @@ def to_bfloat16(a):
 
 def from_bfloat16(a):
     """float32 values of a host array of bfloat16 records."""
-    return (np.ascontiguousarray(a).view(np.uint16).astype(np.uint32) << 16).view(np.float32)
+    a = np.asarray(a)
+    return (np.ascontiguousarray(a).view(np.uint16).astype(np.uint32) << 16).view(np.float32).reshape(a.shape)
+
+
+def as_numbers(obj, dtype):
+    """What NumPy has to be given to convert `obj` to `dtype`: of bfloat16 it
+    knows the bits only, and would convert those."""
+    if dtype is None:
+        return obj
+    to, of = np.dtype(dtype) == bfloat16, getattr(obj, "dtype", None) == bfloat16
+    return to_bfloat16(obj) if to and not of else from_bfloat16(obj) if of and not to else obj
 
 
 _REGISTERED = {}     # dtype -> C name, for element types added with register_dtype
@@ -84,6 +94,7 @@ def _fill_dtype_registry():
             (np.uint64, ["ga_ulong", "unsigned long", "unsigned long int", "long unsigned int",
                          "unsigned long long", "ga_size", "size_t"]),
             (np.float16, ["ga_half", "half"]),
+            (bfloat16, ["ga_bfloat16", "bfloat16"]),
             (np.float32, ["ga_float", "float"]),
             (np.float64, ["ga_double", "double"])):
         register_dtype(dt, names)
@@ -121,6 +132,8 @@ def get_np_obj(obj):
 
 def get_common_dtype(obj1, obj2, allow_double):
     """reference pygpu/dtypes.py:169-192"""
+    if getattr(obj1, "dtype", None) == bfloat16 and getattr(obj2, "dtype", None) == bfloat16:
+        return bfloat16        # (with another type NumPy knows no common one: TypeError)
     result = np.asarray(get_np_obj(obj1) + get_np_obj(obj2)).dtype
     if not allow_double:
         if result == np.float64:

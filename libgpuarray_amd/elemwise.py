@@ -11,7 +11,7 @@ from . import _lib
 from ._lib import lib, check, ElemwiseArg
 from . import gpuarray
 from .gpuarray import GpuArray, dtype_to_typecode
-from .dtypes import dtype_to_ctype, get_common_dtype
+from .dtypes import as_numbers, bfloat16, dtype_to_ctype, get_common_dtype
 
 
 class arg(object):
@@ -63,7 +63,7 @@ class GpuElemwise(object):
                 buf = np.zeros((), dtype=a.dtype)
                 self._scalars[i] = buf
                 self._ptrs[i] = buf.ctypes.data
-        self._slots = [(i, a.scalar, a.name) for i, a in enumerate(self.args)]
+        self._slots = [(i, a.scalar and (2 if a.dtype == bfloat16 else 1), a.name) for i, a in enumerate(self.args)]
         if not self.ge:
             # the code is in the context's record; surface it like any other failure
             msg = context.error()
@@ -93,7 +93,7 @@ class GpuElemwise(object):
         for i, scalar, name in self._slots:
             v = values[i]
             if scalar:
-                self._scalars[i][...] = v
+                self._scalars[i][...] = v if scalar == 1 else as_numbers(v, bfloat16)
             else:
                 try:
                     ptrs[i] = v._addr

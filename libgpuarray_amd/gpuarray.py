@@ -13,7 +13,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import lib, check, GpuArrayException, UnsupportedException, GpuArrayStruct, c_ssize_t
-from .dtypes import bfloat16
+from .dtypes import bfloat16, as_numbers
 from .dtypes import dtype_to_ctype  # noqa: F401  (part of this module's interface, as in the reference)
 
 # numpy dtype.num equals the typecode on LP64 Linux
@@ -440,7 +440,7 @@ class GpuArray(object):
         if self.size == 0:
             return False
         if self.size == 1:
-            return bool(np.asarray(self))
+            return bool(as_numbers(np.asarray(self), "float32") if self.dtype == bfloat16 else np.asarray(self))
         raise ValueError("Truth value of array with more than one element is ambiguous")
 
     __hash__ = None
@@ -509,7 +509,7 @@ class GpuArray(object):
         if out.nbytes:
             a._check(lib.GpuArray_read(out.ctypes.data_as(C.c_void_p), out.nbytes, a._ptr()))
         if dtype is not None and np.dtype(dtype) != out.dtype:
-            out = out.astype(dtype)
+            out = as_numbers(out, dtype).astype(dtype)
         return out
 
     def copy(self, order="C"):
@@ -682,7 +682,7 @@ class GpuArray(object):
         """a[key] = value through GpuArray_setarray (reference gpuarray.pyx:2071-2096)."""
         target = self if key is Ellipsis or key == slice(None) else self.__getitem__(key)
         if not isinstance(value, GpuArray):
-            value = array(np.asarray(value, dtype=self.dtype), context=self.context)
+            value = array(np.asarray(as_numbers(value, self.dtype), dtype=self.dtype), context=self.context)
         target._check(lib.GpuArray_setarray(target._ptr(), value._ptr()))
 
     def __repr__(self):
@@ -724,7 +724,7 @@ def array(obj, dtype=None, order="A", context=None, cls=None):
     """Device copy of anything numpy can turn into an array."""
     if isinstance(obj, GpuArray):
         return obj.copy("C" if order == "A" else order)
-    a = np.array(obj, dtype=dtype, copy=True)
+    a = np.array(as_numbers(obj, dtype), dtype=dtype, copy=True)
     # (np.ascontiguousarray would turn a 0-d array into a 1-d one)
     if order.upper() == "F" or (order.upper() == "A" and a.flags.f_contiguous
                                 and not a.flags.c_contiguous):
@@ -940,7 +940,7 @@ class GpuKernel(object):
                     raise TypeError("expected a GpuArray")
                 ptrs[i] = a.ga.data
             else:
-                v = np.asarray(a, dtype=dt).reshape(1).copy()
+                v = np.asarray(as_numbers(a, dt), dtype=dt).reshape(1).copy()
                 keep.append(v)
                 ptrs[i] = v.ctypes.data
         if n is not None:

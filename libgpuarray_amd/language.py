@@ -32,6 +32,20 @@ def _finish(err, ctx):
     _check(err, ctx.ctx)
 
 
+def _ignore(ignore):
+    """The argument of the C calls, which would take a larger number modulo 2^64."""
+    if ignore is None:
+        return NO_IGNORE
+    if not -1 << 63 <= ignore < 1 << 63:
+        raise ValueError("ignore does not fit 64 bits")
+    return int(ignore)
+
+
+def _dims(a, nd, what):
+    if a.ndim != nd:
+        raise ValueError("%s must have %d dim%s" % (what, nd, "s" if nd > 1 else ""))
+
+
 def _ref(a):
     return None if a is None else a._ref
 
@@ -42,10 +56,11 @@ def embedding(table, ids, scale=1.0, ignore=None, out=None, dtype=None, check=Tr
     rows of the id `ignore` are zeros.  check=False does not wait for the
     bounds flag, as in GpuArray.take1."""
     if out is None:
+        _dims(table, 2, "table")
+        _dims(ids, 1, "ids")
         out = gpuarray.empty((ids.shape[0], table.shape[1]), table.dtype if dtype is None else dtype,
                              context=table.context, cls=type(table))
-    err = lib.GpuArray_embedding(out._ref, table._ref, ids._ref, scale, NO_IGNORE if ignore is None else ignore,
-                                 1 if check else 0)
+    err = lib.GpuArray_embedding(out._ref, table._ref, ids._ref, scale, _ignore(ignore), 1 if check else 0)
     if err:
         _finish(err, out.context)
     return out
@@ -55,8 +70,8 @@ def embedding_grad(dout, ids, grad, scale=1.0, ignore=None, accumulate=False, ch
     """Gradient of embedding() with respect to its table, into `grad` (v, d):
     every row is scale times the sum of the rows of `dout` that have its id,
     in a fixed order; with `accumulate` that is added to what `grad` holds."""
-    err = lib.GpuArray_embedding_grad(grad._ref, dout._ref, ids._ref, scale, NO_IGNORE if ignore is None else ignore,
-                                      1 if accumulate else 0, 1 if check else 0)
+    err = lib.GpuArray_embedding_grad(grad._ref, dout._ref, ids._ref, scale, _ignore(ignore), 1 if accumulate else 0,
+                                      1 if check else 0)
     if err:
         _finish(err, grad.context)
     return grad
@@ -74,6 +89,9 @@ def token_logprobs(logits, ids=None, scale=1.0, top=0, entropy=False, ignore=Non
     write; those it leaves out (None) are not computed.  All values are
     float32."""
     if out is None:
+        _dims(logits, 2, "logits")
+        if top < 0:
+            raise ValueError("top must be 0 or above")
         t, ctx = logits.shape[0], logits.context
 
         def new(shape, dtype="float32"):
@@ -83,7 +101,7 @@ def token_logprobs(logits, ids=None, scale=1.0, top=0, entropy=False, ignore=Non
                             new((t, top)) if top else None, new((t, top), "int64") if top else None)
     logp, h, stats, top_logp, top_ids = out
     err = lib.GpuArray_token_logprobs(_ref(logp), _ref(h), _ref(stats), _ref(top_logp), _ref(top_ids), logits._ref,
-                                      _ref(ids), scale, NO_IGNORE if ignore is None else ignore, 1 if check else 0)
+                                      _ref(ids), scale, _ignore(ignore), 1 if check else 0)
     if err:
         _finish(err, logits.context)
     return out
@@ -98,8 +116,7 @@ def token_logprobs_grad(logits, ids, stats, dlogp, entropy=None, dentropy=None, 
     if out is None:
         out = logits._empty_like_me()
     err = lib.GpuArray_token_logprobs_grad(out._ref, logits._ref, _ref(ids), stats._ref, _ref(dlogp), _ref(entropy),
-                                           _ref(dentropy), scale, NO_IGNORE if ignore is None else ignore,
-                                           1 if check else 0)
+                                           _ref(dentropy), scale, _ignore(ignore), 1 if check else 0)
     if err:
         _finish(err, out.context)
     return out
@@ -124,8 +141,9 @@ def _lists(arrays, out, context):
 class GlobalNorm(object):
     """The 2-norm over all elements of a list of contiguous arrays, and
     clipping by it, for callers that clip the same gradients every step: `out`
-    is the list of arrays that clipping writes (None: the arrays themselves).
-    Holds the arrays, as they are now, and a table of them on the device."""
+    is the list of arrays that clipping writes (None: the arrays themselves,
+    no two of which may overlap then).  Holds the arrays, as they are now, and
+    a table of them on the device."""
 
     def __init__(self, arrays, out=None, context=None):
         self.arrays, self.out, self.context, (a, r) = _lists(arrays, out, context)

@@ -66,7 +66,7 @@ class GpuReduction(object):
 
 
 from .tools import Argument, ArrayArg, ScalarArg, as_argument  # noqa: E402,F401
-from .dtypes import parse_c_arg_backend  # noqa: E402
+from .dtypes import as_numbers, parse_c_arg_backend  # noqa: E402
 
 
 _INDEX_RE = re.compile(r"([a-zA-Z_][a-zA-Z0-9_]*)\[i\]")
@@ -213,7 +213,7 @@ class MapReduction(object):
             if d.isarray():
                 ptrs[i] = C.cast(a._ptr(), C.c_void_p)
             else:
-                v = np.asarray(a, dtype=d.dtype).reshape(1).copy()
+                v = np.asarray(as_numbers(a, d.dtype), dtype=d.dtype).reshape(1).copy()
                 keep.append(v)
                 ptrs[i] = v.ctypes.data
         axes = list(axes)

@@ -893,6 +893,46 @@ def test_bfloat16_arrays(ctx):
     assert np.array_equal(decode(dev), decode(ga.to_bfloat16(special)), equal_nan=True)
 
 
+def test_numbers_become_bfloat16_and_back(ctx):
+    """Lists, scalars and arrays of other types, wherever a host value meets an array of bfloat16."""
+    x = [[1.5, -2.25], [3.0, 1e30]]
+    a = gpuarray.array(x, dtype=ga.bfloat16, context=ctx)
+    want = decode(ga.to_bfloat16(x))
+    assert a.shape == (2, 2) and np.array_equal(decode(a), want)
+    assert np.array_equal(np.asarray(a, dtype="float64"), want)
+    assert np.array_equal(np.asarray(gpuarray.array(ga.to_bfloat16(x), dtype="float32", context=ctx)), want)
+    assert gpuarray.array(2.5, dtype=ga.bfloat16, context=ctx).shape == ()
+    assert ga.from_bfloat16(ga.to_bfloat16(2.5)).shape == ()
+    a[0] = 7
+    a[1, 1] = -0.5
+    assert np.array_equal(decode(a), [[7, 7], [3, -0.5]])
+    assert a[1, 1] and not gpuarray.array(-0.0, dtype=ga.bfloat16, context=ctx)
+    from libgpuarray_amd.elemwise import GpuElemwise, arg as e_arg
+    from libgpuarray_amd import ndgpuarray
+    k = GpuElemwise(ctx, "r = a * s", [e_arg("r", ga.bfloat16, write=True), e_arg("a", ga.bfloat16, read=True),
+                                       e_arg("s", ga.bfloat16, scalar=True)])
+    r = gpuarray.empty((2, 2), ga.bfloat16, context=ctx)
+    k(r, a, 1.5)
+    assert np.array_equal(decode(r), [[10.5, 10.5], [4.5, -0.75]])
+    b = gpuarray.array(ga.to_bfloat16(x), context=ctx, cls=ndgpuarray)
+    assert np.array_equal(decode(b + b), 2 * want)
+    assert np.array_equal(np.asarray(b > 2.0), want > 2)
+    with pytest.raises(TypeError):
+        b + 1.0                                              # no common type: convert one of them
+    with pytest.raises(_lib.GpuArrayException):
+        b.sum()
+
+
+def test_refusals_of_python_values(ctx):
+    z = lambda shape, dt="float32": gpuarray.zeros(shape, dt, context=ctx)  # noqa: E731
+    table, ids = z((9, 8)), z((4,), "int64")
+    for call in (lambda: ga.embedding(z((9,)), ids), lambda: ga.embedding(table, z((), "int64")),
+                 lambda: ga.embedding(table, ids, ignore=1 << 63), lambda: ga.token_logprobs(z(())),
+                 lambda: ga.token_logprobs(table, top=-1), lambda: ga.embedding_grad(z((4, 8)), ids, table, ignore=-(1 << 63) - 1)):
+        with pytest.raises(ValueError):
+            call()
+
+
 # ---- refusals: nothing is launched, so these also run without a device -------------------------------
 
 def refusals(ctx):
