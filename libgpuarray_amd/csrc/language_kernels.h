@@ -170,6 +170,18 @@ LM_FN ga_uint lm_minus_inf(ga_float) { return 0xff800000u; }
 LM_FN ga_uint lm_minus_inf(ga_half) { return 0xfc00fc00u; }
 LM_FN ga_uint lm_minus_inf(ga_bfloat16) { return 0xff80ff80u; }
 
+/* Zeroes `bytes` bytes from b on, whose elements have 2 or 4, by `lanes` lanes (32 or more). */
+LM_FN void lm_zero(GLOBAL_MEM char *b, ga_long bytes, ga_uint lane, ga_uint lanes) {
+  ga_long head = (ga_long)(-(ga_size)b & 15);
+  if (head > bytes) head = bytes;
+  const ga_long chunks = (bytes - head) / 16, tail = head + chunks * 16;
+  GLOBAL_MEM lm_u4 *q = (GLOBAL_MEM lm_u4 *)(b + head);
+  const lm_u4 zero = {0, 0, 0, 0};
+  for (ga_long c = lane; c < chunks; c += lanes) __builtin_nontemporal_store(zero, q + c);
+  const ga_long at = lane * 2 < head ? lane * 2 : tail + (lane * 2 - head);
+  if (at < bytes) *(GLOBAL_MEM ga_ushort *)(b + at) = 0;
+}
+
 #if LM_KIND == LM_K_EMBED
 struct lm_embed {
   GLOBAL_MEM LM_O *out;
@@ -181,8 +193,7 @@ struct lm_embed {
   float scale;
   ga_uint lanes_log2, segments;
 };
-/* elements of a lane: 16 bytes of the narrower side */
-#define LM_C (sizeof(LM_X) < sizeof(LM_O) ? 16 / (int)sizeof(LM_X) : 16 / (int)sizeof(LM_O))
+#define LM_C (16 / (int)sizeof(LM_O))   /* elements of a lane: 16 bytes of the result */
 #define LM_ROWS 4
 
 /* 2^lanes_log2 lanes share a row's 256 * LM_C columns or fewer; a lane moves the
@@ -265,17 +276,8 @@ LM_FN void lm_clear(const lm_sorting &p, ga_uint first) {
   const ga_long waves = (ga_long)(GDIM_0 - first) * 16;
   for (ga_long u = p.fill_unit0 + (ga_long)(GID_0 - first) * 16 + (LID_0 >> 6); u < p.fill_unit1; u += waves) {
     const ga_long row = u / segments, seg = u % segments;
-    GLOBAL_MEM char *b = p.fill + row * p.fill_row + seg * LM_SEGMENT;
-    ga_long bytes = p.fill_bytes - seg * LM_SEGMENT;
-    if (bytes > LM_SEGMENT) bytes = LM_SEGMENT;
-    ga_long head = (ga_long)(-(ga_size)b & 15);
-    if (head > bytes) head = bytes;
-    const ga_long chunks = (bytes - head) / 16, tail = head + chunks * 16;
-    GLOBAL_MEM lm_u4 *q = (GLOBAL_MEM lm_u4 *)(b + head);
-    const lm_u4 zero = {0, 0, 0, 0};
-    for (ga_long c = lane; c < chunks; c += 64) __builtin_nontemporal_store(zero, q + c);
-    const ga_long at = lane * 2 < head ? lane * 2 : tail + (lane * 2 - head);   /* elements are 2 or 4 bytes */
-    if (at < bytes) *(GLOBAL_MEM ga_ushort *)(b + at) = 0;
+    const ga_long bytes = p.fill_bytes - seg * LM_SEGMENT;
+    lm_zero(p.fill + row * p.fill_row + seg * LM_SEGMENT, bytes < LM_SEGMENT ? bytes : LM_SEGMENT, lane, 64);
   }
 }
 
@@ -484,6 +486,7 @@ struct lm_embed_grad {
   float scale;
   ga_int accumulate;
   ga_uint n, chunk, chunks, tiles, rows, lanes_log2;
+  ga_uint dense, part_tiles;                   /* the table's rows lie end to end */
 };
 
 /* The columns of a lane: LM_W from `from` on, of which the first `skip` belong
@@ -541,38 +544,68 @@ LM_FN void lm_fetch_rows(const lm_embed_grad &p, const ga_uint (&at)[LM_AHEAD], 
 }
 
 /* Few tokens need no sorting: a group takes p.rows rows of the table and up to
- * four times 64 * LM_W columns of them (as many rows as give each of its wavefronts
- * four pieces), looks all ids through once, which leaves a mask of the tokens of
- * each row, and adds those in order; one launch in place of three. */
+ * four times 64 * LM_W columns of them, zeroes them, end to end if it can, and
+ * looks all ids through once, which leaves a mask of the tokens of each row; it
+ * adds those in order and writes the rows that have some.  One launch in place of four. */
 #define LM_FEW 256        /* tokens at most */
-#define LM_FEW_ROWS 16    /* rows at most */
+#define LM_FEW_ROWS 512   /* rows at most */
 KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
   LOCAL_MEM ga_ulong masks[LM_FEW_ROWS][LM_FEW / 64];
+  LOCAL_MEM ga_ushort with[LM_FEW];
+  LOCAL_MEM ga_uint count;
+  LOCAL_MEM ga_uint some, next;   /* do these rows, does the one after them have tokens */
   const ga_uint lane = LID_0 & 63, wave = LID_0 >> 6;
-  const ga_uint parts = (p.tiles + 3) / 4, part = GID_0 % parts;
-  const ga_uint tiles = p.tiles - part * 4 < 4 ? p.tiles - part * 4 : 4;
+  const ga_uint parts = (p.tiles + p.part_tiles - 1) / p.part_tiles, part = GID_0 % parts, tile0 = part * p.part_tiles;
+  const ga_uint tiles = p.tiles - tile0 < p.part_tiles ? p.tiles - tile0 : p.part_tiles;
   const ga_long r0 = (ga_long)(GID_0 / parts) * p.rows;
+  const ga_uint rows = p.v - r0 < p.rows ? (ga_uint)(p.v - r0) : p.rows;
   const ga_long id = LID_0 < p.n ? lm_id(*lm_at(p.ids, (ga_long)LID_0 * p.id_step), p.ignore, LM_NONE, p.v) : -1;
   if (id == -2) *p.err = -1;
-  const ga_uint row = id >= r0 && id < r0 + p.rows ? (ga_uint)(id - r0) : LM_FEW_ROWS;
-  for (ga_uint k = 0; k < p.rows; k++) {
-    const ga_ulong m = __builtin_amdgcn_ballot_w64(row == k);
-    if (lane == k) masks[k][wave] = m;
+  if (LID_0 == 0) some = next = count = 0;
+  for (ga_uint i = LID_0; i < rows * (LM_FEW / 64); i += 256) (&masks[0][0])[i] = 0;
+  GLOBAL_MEM char *b = (GLOBAL_MEM char *)p.grad + r0 * p.grad_row;
+  const ga_long row = p.d * (ga_long)sizeof(LM_O);
+  const bool flat = p.dense && parts == 1, shared = flat && row >= 16 && (row & 15) != 0;
+  if (!p.accumulate && rows > 0 && !shared) {
+    if (flat) {
+      lm_zero(b, rows * row, LID_0, 256);
+    } else {
+      const ga_long col = (ga_long)tile0 * 64 * LM_W, cols = p.d - col < tiles * 64 * LM_W ? p.d - col : tiles * 64 * LM_W;
+      for (ga_uint k = 0; k < rows; k++)
+        lm_zero(b + k * p.grad_row + col * (ga_long)sizeof(LM_O), cols * (ga_long)sizeof(LM_O), LID_0, 256);
+    }
   }
   local_barrier();
-  for (ga_uint unit = wave; unit < p.rows * tiles; unit += 4) {
-    const ga_uint k = unit / tiles, tile = part * 4 + unit % tiles;
-    if (r0 + k >= p.v) break;
+  if (id >= r0 && id < r0 + rows) {
+    atomicOr((unsigned long long *)&masks[id - r0][wave], 1ull << lane);
+    some = 1;
+  }
+  if (id == r0 + rows) next = 1;
+  local_barrier();
+  if (!p.accumulate && shared) {
+    /* A 16-byte chunk that two groups share is one store of the first of them,
+     * but where the second one's first row has tokens, and so is not all zeros
+     * (22723 rows of 4413 bfloat16 42 us, with stores of what is left at both ends 48). */
+    ga_long from = 0, to = rows * row;
+    if (r0 > 0 && (masks[0][0] | masks[0][1] | masks[0][2] | masks[0][3]) == 0) from = (ga_long)(-(ga_size)b & 15);
+    if (r0 + rows < p.v && !next) to += (ga_long)(-(ga_size)(b + to) & 15);
+    lm_zero(b + from, to - from, LID_0, 256);
+  }
+  if (!some) return;
+  for (ga_uint k = LID_0; k < rows; k += 256)    /* (in any order: each row is a sum of its own) */
+    if (masks[k][0] | masks[k][1] | masks[k][2] | masks[k][3]) with[atomicAdd(&count, 1u)] = (ga_ushort)k;
+  /* (the zeros are in the L2 before a sum follows them) */
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  local_barrier();
+  for (ga_uint unit = wave; unit < count * tiles; unit += 4) {
+    const ga_uint k = (ga_uint)__builtin_amdgcn_readfirstlane((int)with[unit / tiles]), tile = tile0 + unit % tiles;
     ga_ulong left[LM_FEW / 64];
-    ga_ulong any = 0;
 #pragma unroll
     for (int w = 0; w < LM_FEW / 64; w++) {
       left[w] = masks[k][w];
       left[w] = (ga_ulong)(ga_uint)__builtin_amdgcn_readfirstlane((int)(left[w] >> 32)) << 32 |
                 (ga_uint)__builtin_amdgcn_readfirstlane((int)left[w]);
-      any |= left[w];
     }
-    if (any == 0 && p.accumulate) continue;
     const lm_columns mine = lm_columns_of(((ga_long)tile * 64 + lane) * LM_W, p.d);
     float sum[LM_W];
 #pragma unroll

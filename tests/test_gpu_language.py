@@ -218,6 +218,29 @@ def test_embedding_grad(ctx, n, v, d, dout, grad, accumulate):
     check_embedding_grad(g, x, ids, v, 1.5, -100, grad, base)
 
 
+@pytest.mark.parametrize("n,v,d", [(1, 5000, 1), (256, 3000, 1), (200, 4100, 7), (3, 5000, 8), (256, 4099, 125), (70, 4500, 983), (9, 4200, 4413),
+                                   (250, 2, 3001), (256, 30, 2048)])
+@pytest.mark.parametrize("dout,grad", [("float16", "float16"), ("bfloat16", "float32"), ("float32", "bfloat16")])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_embedding_grad_of_few_tokens(ctx, n, v, d, dout, grad, accumulate, shift):
+    """Groups of many rows that share 16-byte chunks at their ends, with tokens on either side of such an end or
+    none; the memory before and behind the rows stays."""
+    rng = np.random.default_rng(n + v + d)
+    x = encode(rng.standard_normal((n, d)), dout)
+    ids = rng.integers(0, v, n)
+    ids[: n // 3] = np.minimum(v - 1, 8192 // (d * np_type(grad).itemsize) * rng.integers(0, 3, n // 3))
+    ids[n // 2] = -100
+    base = encode(rng.standard_normal((v, d)), grad)
+    root = gpuarray.array(np.concatenate([encode([9.0] * shift, grad), base.ravel(), encode([9.0] * 5, grad)]), context=ctx)
+    size = np_type(grad).itemsize
+    g = gpuarray.from_strided(root, shift * size, (v, d), (d * size, size))
+    ga.embedding_grad(gpuarray.array(x, context=ctx), gpuarray.array(ids, context=ctx), g, scale=1.5, ignore=-100, accumulate=accumulate)
+    check_embedding_grad(g, x, ids, v, 1.5, -100, grad, base if accumulate else None)
+    around = decode(root)
+    assert np.all(around[:shift] == 9) and np.all(around[shift + v * d:] == 9)
+
+
 @pytest.mark.parametrize("n,v,d,share", [(20000, 50257, 72, 0.4), (40000, 700, 64, 0.0), (70001, 65537, 40, 0.9),
                                          (16384, 16384, 64, 0.0), (16385, 300000, 8, 0.1), (150000, 2, 33, 0.0),
                                          (33000, 1, 16, 0.0)])
@@ -1020,18 +1043,16 @@ def test_refusals(ctx):
 
 
 def test_refusals_of_more_lanes_than_a_launch_has(ctx):
-    """2^26 rows of one column each have a wavefront, 2^28 rows of a gradient of few tokens 16 a group."""
+    """2^26 rows of one column each have a wavefront."""
     t = 1 << 26
     logits = gpuarray.from_strided(gpuarray.zeros((1,), "float16", context=ctx), 0, (t, 1), (0, 2))
     stats = gpuarray.from_strided(gpuarray.zeros((2,), context=ctx), 0, (t, 2), (0, 4))
     ids = gpuarray.from_strided(gpuarray.zeros((1,), "int32", context=ctx), 0, (t,), (0,))
     dlogp = gpuarray.from_strided(gpuarray.zeros((1,), context=ctx), 0, (t,), (0,))
     logp, dlogits = gpuarray.empty((t,), context=ctx), gpuarray.empty((t, 1), "float16", context=ctx)
-    grad = gpuarray.empty((1 << 28, 1), "float16", context=ctx)
     before = ctx.last_launch_hash()
     for call in (lambda: ga.token_logprobs(logits, ids, out=ga.TokenLogprobs(logp, None, None, None, None)),
-                 lambda: ga.token_logprobs_grad(logits, ids, stats, dlogp, out=dlogits),
-                 lambda: ga.embedding_grad(logits[:3], ids[:3], grad)):
+                 lambda: ga.token_logprobs_grad(logits, ids, stats, dlogp, out=dlogits)):
         with pytest.raises(_lib.GpuArrayException) as e:
             call()
         assert e.value.code == _lib.GA_XLARGE_ERROR
