@@ -438,9 +438,11 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
     // Many rows that do not begin on 16-byte boundaries are taken whole, so that they are
     // zeroed end to end (22000 rows of 4413 bfloat16: 44 us, in parts 56; but 1000
     // rows of 6000 floats 17.5 us, in parts 10.5).
-    a.part_tiles = dense && d * osize % 16 != 0 && tiles <= 16 && v >= 4096 ? 16 : 4;
-    a.rows = (uint32_t)std::min<size_t>(std::max<size_t>(8192 / (std::min(d, a.part_tiles * cols) * osize), 1), 512);
-    const size_t parts = (tiles + a.part_tiles - 1) / a.part_tiles, row_groups = v ? (v + a.rows - 1) / a.rows : 1;
+    a.part_tiles = !accumulate && dense && d * osize % 16 != 0 && tiles <= 16 && v >= 4096 ? 16 : 4;
+    const size_t parts = (tiles + a.part_tiles - 1) / a.part_tiles;
+    a.rows = (uint32_t)std::min({std::max<size_t>(8192 / (std::min(d, a.part_tiles * cols) * osize), 1), v * parts / 512 + 1, (size_t)512});
+    const size_t row_groups = accumulate ? n : v ? (v + a.rows - 1) / a.rows : 1;
+    if (row_groups == 0) return GA_NO_ERROR;
     if (parts > max_groups(256) / row_groups) return c.fail(GA_XLARGE_ERROR, "too many elements");
     if (err == GA_NO_ERROR) err = lm_launch(kfew, row_groups * parts, 256, &a);
     return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;

@@ -549,6 +549,65 @@ LM_FN void lm_fetch_rows(const lm_embed_grad &p, const ga_uint (&at)[LM_AHEAD], 
  * adds those in order and writes the rows that have some.  One launch in place of four. */
 #define LM_FEW 256        /* tokens at most */
 #define LM_FEW_ROWS 512   /* rows at most */
+/* A wavefront adds the tokens of a row, those whose bits are set, over one tile of columns. */
+LM_FN void lm_add_few(const lm_embed_grad &p, ga_uint key, ga_uint tile, ga_ulong (&left)[LM_FEW / 64]) {
+  const ga_uint lane = LID_0 & 63;
+      const lm_columns mine = lm_columns_of(((ga_long)tile * 64 + lane) * LM_W, p.d);
+      float sum[LM_W];
+#pragma unroll
+      for (int e = 0; e < LM_W; e++) sum[e] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < LM_FEW / 64; w++) {
+        while (left[w] != 0) {
+          ga_uint at[LM_AHEAD];
+          ga_uint n = 0;
+#pragma unroll
+          for (int u = 0; u < LM_AHEAD; u++) {
+            at[u] = left[w] != 0 ? w * 64 + (ga_uint)__builtin_ctzll(left[w]) : at[u > 0 ? u - 1 : 0];
+            n += left[w] != 0;
+            left[w] &= left[w] - 1;
+          }
+          float y[LM_AHEAD][LM_W];
+          lm_fetch_rows(p, at, mine, y);
+#pragma unroll
+          for (int u = 0; u < LM_AHEAD; u++) {
+            if (u < n) {
+#pragma unroll
+              for (int e = 0; e < LM_W; e++) sum[e] += y[u][e];
+            }
+          }
+        }
+      }
+  lm_write_run(p, key, mine, sum);
+}
+/* What is added to: a group for each token and p.part_tiles tiles, one tile a
+ * wavefront at a time; the first token of a row adds them all. */
+LM_FN void lm_add_to_few(const lm_embed_grad &p, ga_long id) {
+  LOCAL_MEM ga_long ids[LM_FEW];
+  LOCAL_MEM ga_ulong mask[LM_FEW / 64];
+  const ga_uint parts = (p.tiles + p.part_tiles - 1) / p.part_tiles, token = GID_0 / parts, part = GID_0 % parts;
+  ids[LID_0] = id;
+  local_barrier();
+  const ga_long mine = ids[token];
+  const ga_ulong m = __builtin_amdgcn_ballot_w64(id == mine);
+  if ((LID_0 & 63) == 0) mask[LID_0 >> 6] = m;
+  local_barrier();
+  if (mine < 0) return;
+  ga_ulong all[LM_FEW / 64];
+#pragma unroll
+  for (int w = LM_FEW / 64 - 1; w >= 0; w--) {
+    all[w] = mask[w];
+    all[w] = (ga_ulong)(ga_uint)__builtin_amdgcn_readfirstlane((int)(all[w] >> 32)) << 32 |
+             (ga_uint)__builtin_amdgcn_readfirstlane((int)all[w]);
+    if (w == token >> 6 ? (all[w] & ((1ull << (token & 63)) - 1)) != 0 : w < token >> 6 && all[w] != 0) return;
+  }
+  for (ga_uint i = LID_0 >> 6; i < p.part_tiles && part * p.part_tiles + i < p.tiles; i += 4) {
+    ga_ulong left[LM_FEW / 64];
+#pragma unroll
+    for (int w = 0; w < LM_FEW / 64; w++) left[w] = all[w];
+    lm_add_few(p, (ga_uint)mine, part * p.part_tiles + i, left);
+  }
+}
 KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
   LOCAL_MEM ga_ulong masks[LM_FEW_ROWS][LM_FEW / 64];
   LOCAL_MEM ga_ushort with[LM_FEW];
@@ -558,15 +617,19 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
   const ga_uint parts = (p.tiles + p.part_tiles - 1) / p.part_tiles, part = GID_0 % parts, tile0 = part * p.part_tiles;
   const ga_uint tiles = p.tiles - tile0 < p.part_tiles ? p.tiles - tile0 : p.part_tiles;
   const ga_long r0 = (ga_long)(GID_0 / parts) * p.rows;
-  const ga_uint rows = p.v - r0 < p.rows ? (ga_uint)(p.v - r0) : p.rows;
+  const ga_uint rows = r0 >= p.v ? 0 : p.v - r0 < p.rows ? (ga_uint)(p.v - r0) : p.rows;
   const ga_long id = LID_0 < p.n ? lm_id(*lm_at(p.ids, (ga_long)LID_0 * p.id_step), p.ignore, LM_NONE, p.v) : -1;
   if (id == -2) *p.err = -1;
+  if (p.accumulate) {
+    lm_add_to_few(p, id);
+    return;
+  }
   if (LID_0 == 0) some = next = count = 0;
   for (ga_uint i = LID_0; i < rows * (LM_FEW / 64); i += 256) (&masks[0][0])[i] = 0;
   GLOBAL_MEM char *b = (GLOBAL_MEM char *)p.grad + r0 * p.grad_row;
   const ga_long row = p.d * (ga_long)sizeof(LM_O);
   const bool flat = p.dense && parts == 1, shared = flat && row >= 16 && (row & 15) != 0;
-  if (!p.accumulate && rows > 0 && !shared) {
+  if (rows > 0 && !shared) {
     if (flat) {
       lm_zero(b, rows * row, LID_0, 256);
     } else {
@@ -582,7 +645,7 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
   }
   if (id == r0 + rows) next = 1;
   local_barrier();
-  if (!p.accumulate && shared) {
+  if (shared) {
     /* A 16-byte chunk that two groups share is one store of the first of them,
      * but where the second one's first row has tokens, and so is not all zeros
      * (22723 rows of 4413 bfloat16 42 us, with stores of what is left at both ends 48). */
@@ -606,33 +669,7 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_few(const lm_embed_grad p) {
       left[w] = (ga_ulong)(ga_uint)__builtin_amdgcn_readfirstlane((int)(left[w] >> 32)) << 32 |
                 (ga_uint)__builtin_amdgcn_readfirstlane((int)left[w]);
     }
-    const lm_columns mine = lm_columns_of(((ga_long)tile * 64 + lane) * LM_W, p.d);
-    float sum[LM_W];
-#pragma unroll
-    for (int e = 0; e < LM_W; e++) sum[e] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < LM_FEW / 64; w++) {
-      while (left[w] != 0) {
-        ga_uint at[LM_AHEAD];
-        ga_uint n = 0;
-#pragma unroll
-        for (int u = 0; u < LM_AHEAD; u++) {
-          at[u] = left[w] != 0 ? w * 64 + (ga_uint)__builtin_ctzll(left[w]) : at[u > 0 ? u - 1 : 0];
-          n += left[w] != 0;
-          left[w] &= left[w] - 1;
-        }
-        float y[LM_AHEAD][LM_W];
-        lm_fetch_rows(p, at, mine, y);
-#pragma unroll
-        for (int u = 0; u < LM_AHEAD; u++) {
-          if (u < n) {
-#pragma unroll
-            for (int e = 0; e < LM_W; e++) sum[e] += y[u][e];
-          }
-        }
-      }
-    }
-    lm_write_run(p, (ga_uint)(r0 + k), mine, sum);
+    lm_add_few(p, (ga_uint)(r0 + k), tile, left);
   }
 }
 
