@@ -259,11 +259,11 @@ struct lm_sorting {
   GLOBAL_MEM const LM_ID *ids;      /* of the first pass */
   GLOBAL_MEM const ga_uint *key_in, *order_in;
   GLOBAL_MEM ga_uint *key, *order;  /* results of the pass */
-  GLOBAL_MEM ga_uint *counts;       /* [digit][group], then [digit] totals */
+  GLOBAL_MEM ga_uint *counts;       /* [digit][group], then [digit] totals; [group][digit] if `direct` */
   GLOBAL_MEM ga_int *err;
   ga_long id_step, ignore, v;
   ga_uint n, groups, shift, bits, passes;
-  ga_uint pad;
+  ga_uint direct;                   /* no lm_sort_scan: every group adds the counts itself */
   GLOBAL_MEM char *fill;            /* rows to clear: */
   ga_long fill_rows, fill_row, fill_bytes, fill_unit0, fill_unit1;
 };
@@ -412,7 +412,7 @@ KERNEL void __launch_bounds__(1024) lm_sort_count(const lm_sorting p) {
     }
   }
   local_barrier();
-  if (LID_0 < (1u << p.bits)) p.counts[(ga_size)LID_0 * p.groups + GID_0] = bins[LID_0];
+  if (LID_0 < (1u << p.bits)) p.counts[p.direct ? (GID_0 << p.bits) + LID_0 : (ga_size)LID_0 * p.groups + GID_0] = bins[LID_0];
 }
 /* what the earlier groups have of a digit, a wavefront per digit; */
 KERNEL void __launch_bounds__(1024) lm_sort_scan(const lm_sorting p) {
@@ -456,8 +456,19 @@ KERNEL void __launch_bounds__(1024) lm_sort_move(const lm_sorting p) {
   lm_rank(k, rank, counts, p.shift, p.bits);
   (void)lm_wave_prefix(counts, p.bits);
   const bool mine = LID_0 < (1u << p.bits);
-  const ga_uint start = lm_scan(mine ? p.counts[((ga_size)p.groups << p.bits) + LID_0] : 0);
-  if (mine) base[LID_0] = start + p.counts[(ga_size)LID_0 * p.groups + GID_0];
+  ga_uint total = 0, before = 0;   /* of digit LID_0 in all groups, and in the earlier ones */
+  if (!p.direct) {
+    if (mine) total = p.counts[((ga_size)p.groups << p.bits) + LID_0], before = p.counts[(ga_size)LID_0 * p.groups + GID_0];
+  } else if (mine) {
+#pragma unroll 16
+    for (ga_uint g = 0; g < p.groups; g++) {
+      const ga_uint c = p.counts[(g << p.bits) + LID_0];
+      total += c;
+      before += g < GID_0 ? c : 0;
+    }
+  }
+  const ga_uint start = lm_scan(total);
+  if (mine) base[LID_0] = start + before;
   local_barrier();
 #pragma unroll
   for (int r = 0; r < LM_R; r++) {
