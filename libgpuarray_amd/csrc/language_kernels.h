@@ -723,6 +723,7 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_sum(const lm_embed_grad p) {
   const ga_uint before = p0 > 0 ? p.key[p0 - 1] : 0xffffffffu;
   const ga_uint after = p0 + n < p.n ? p.key[p0 + n] : 0xffffffffu;
   ga_uint run = p.key[p0];
+  if (run == none) return;     /* no tokens, to the end */
   bool here = run != before;   /* the run began in this chunk */
   for (ga_uint sub = 0; sub < n; sub += lanes) {
     const ga_uint i = p0 + sub + lane;
