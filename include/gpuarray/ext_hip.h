@@ -68,6 +68,10 @@ typedef int (*ga_hip_reload_tuning_fn)(gpucontext *ctx);
  * moves dense aligned rows as 16-byte chunks. */
 typedef char *(*ga_hip_take1_source_fn)(int chunks, int a_typecode, int v_typecode,
                                         int i_typecode, unsigned int tnd);
+/* "hip_language_source": kernel text of an operator of language.h, as a malloc'd
+ * string; `variant` is its number, 0 to 6 in the order of language_kernels.h, with the typecodes of
+ * operand, result and ids from bits 8, 20 and 32 and the operator's own part from bit 44. */
+typedef char *(*ga_hip_language_source_fn)(unsigned long long variant);
 /* "hip_module_cache_stats": out[0..2] = entries in the hot, warm and cold
  * lists of the context's loaded-module cache (the reference's 2Q policy,
  * src/cache/twoq.c), out[3] = code objects currently loaded. */

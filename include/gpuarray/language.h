@@ -14,11 +14,13 @@
  *            result is rounded once, to nearest even.
  *   layout   rows (the last axis) have unit stride; any other stride is
  *            taken as it is, negative and zero ones too (results must not
- *            overlap themselves).  Rows need not be aligned to more than
+ *            overlap themselves, and the memory from a result's first element
+ *            to its last holds no other argument).  Rows need not be aligned to more than
  *            their element.
  *   ids      a negative id counts from the end of the vocabulary, as in
  *            GpuArray_take1, except the id `ignore`, which stands for no
- *            token (GA_NO_IGNORE: no id does).  An id out of range never
+ *            token (GA_NO_IGNORE: no id does).  An unsigned one of 2^63 or
+ *            more is out of range.  An id out of range never
  *            reads or writes memory: it sets the context's error word, which
  *            `check_error` reads back (blocking), resets and reports as
  *            GA_VALUE_ERROR "Index out of bounds", and which otherwise stays
@@ -31,7 +33,8 @@
  *   graphs   a call on a stream that records a graph launches kernels only,
  *            once an earlier call of the same types and sizes has built the kernels
  *            and grown the context's scratch; otherwise it is refused with
- *            GA_UNSUPPORTED_ERROR.  Partial results lie in that scratch, so
+ *            GA_UNSUPPORTED_ERROR, and so is a call with `check_error`, which
+ *            would wait.  Partial results lie in that scratch, so
  *            graphs recorded from a context are replayed on its stream, one
  *            after the other (as for GpuReduction_call).
  */
@@ -134,7 +137,7 @@ GPUARRAY_PUBLIC int GpuArray_clip_global_norm(GpuArray **rs,
  * table of them in device memory.  The arrays count as they are when it is
  * made; rs == NULL: for norms alone; rs may be `as`, or name `as` elements, to clip in place.
  * Making one copies the table to the device, and is refused while the stream
- * records a graph; calls may be recorded. */
+ * records a graph; calls may be recorded, and replayed until it is freed. */
 typedef struct _GpuGlobalNorm GpuGlobalNorm;
 GPUARRAY_PUBLIC int GpuGlobalNorm_new(GpuGlobalNorm **g, gpucontext *ctx,
                                       const GpuArray **as, GpuArray **rs,

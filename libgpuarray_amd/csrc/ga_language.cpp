@@ -184,7 +184,7 @@ int lm_counters(gpucontext *ctx, void **out) {
   gpudata *b = ga_hip_redux_counters(ctx);
   if (b == nullptr)
     return ga_hip_capturing(ctx) ? ga_err_set(ctx->err, GA_UNSUPPORTED_ERROR,
-                                              "The counters are not made yet and the stream records a graph: call once before recording")
+                                              "No counters yet and the stream records a graph: call once before recording")
                                  : ctx->err->code;
   *out = b->devptr;
   return GA_NO_ERROR;
@@ -346,7 +346,13 @@ void ga_language_cache_free(gpucontext *ctx) {
 
 // The kernel text of a variant (packed as lm_variant::key packs it), as a
 // malloc'd string; behind the "hip_language_source" hook.
-char *ga_language_gen_source(unsigned long long variant) { return strdup(lm_source(lm_variant(variant)).c_str()); }
+char *ga_language_gen_source(unsigned long long variant) {
+  try {
+    return strdup(lm_source(lm_variant(variant)).c_str());
+  } catch (...) {
+    return nullptr;
+  }
+}
 
 // ---- embedding -----------------------------------------------------------------
 
@@ -419,6 +425,8 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   const size_t cols = 64 * 16 / std::max(osize, gpuarray_get_elsize(dout->typecode));   // of a wavefront
   const size_t tiles = (d + cols - 1) / cols;
   // rows that half a wavefront covers: several chunks of tokens side by side in one
+  // (65536 tokens of 64 bfloat16 added to floats 41 us, with a wavefront a chunk
+  // 50; of 120 45 and 50; a million of 16 101 and 122)
   unsigned lanes_log2 = 3;
   while (((size_t)cols / 64 << lanes_log2) < d && lanes_log2 < 6) lanes_log2++;
   const bool narrow = lanes_log2 < 6, dense = v <= 1 || grad->strides[0] == (ssize_t)(d * osize);
@@ -430,6 +438,8 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   int err = lm_errbuf(ctx, grad, &errbuf);
   if (err != GA_NO_ERROR) return err;
   a.err = errbuf->devptr;
+  // Up to 256 tokens, as many as a group has lanes, are not sorted (256 of 1024 bfloat16 into
+  // 50257 rows of floats that are cleared 33 us, sorted 46; into 1000 rows of 256 5 and 13; added 5.5 and 16).
   if (n <= 256) {
     GpuKernel *kfew = nullptr;
     err = lm_kernel(ctx, vg, "lm_embed_grad_few", sizeof(embed_grad_args), &kfew);
@@ -449,7 +459,8 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   }
   // Tokens of a chunk: enough chunks to fill the chip with wavefronts, and
   // not so few tokens that partial sums (two rows a chunk at most) count, nor
-  // the parts of a token that comes very often.
+  // the parts of a token that comes very often (65536 tokens of 2048 added, by the least number of wavefronts:
+  // 2048 185 us, 4096 138, 8192 128, 16384 132).
   const size_t per_wave = narrow ? (size_t)64 >> lanes_log2 : 1;   // chunks
   size_t chunk = 8;
   while (chunk < 256 && n / (chunk * 2) / per_wave * tiles >= (narrow ? 2048u : 8192u)) chunk *= 2;
@@ -600,10 +611,17 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
   if (t == 0 || (logp == nullptr && entropy == nullptr && stats == nullptr && top == 0)) return GA_NO_ERROR;
   if (v == 0) return c.fail(GA_VALUE_ERROR, "empty vocabulary");
   if (v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many columns");
-  // A row that a wavefront covers in two rounds of loads belongs to one
-  // wavefront, longer ones to a group, which grows while there are too few
+  // A row that a wavefront covers in eight rounds of loads belongs to one
+  // wavefront, a longer one to a group, which grows while there are too few
   // rows to fill the chip; below that, rows are cut in pieces of at least two
-  // chunks per lane, of which the last one to end joins them all.
+  // chunks per lane, of which the last one to end joins them all.  Rows of bfloat16 with
+  // entropy, us by the lanes 64, 256, 512, 1024 (and pieces):
+  //   32768 rows of 2000     33    57   136   323
+  //   32768 rows of 4000     51    69   131   315
+  //   4096 rows of 50257     77    74    75    97
+  //   512 rows of 50257      35    15    13    16
+  //   128 rows of 50257      31    11     8.0   7.8   (8.3)
+  //   8 rows of 50257        24     8.0   6.2   6.5   (5.6)
   const size_t row_chunks = v * gpuarray_get_elsize(logits->typecode) / 16 + 1;
   const size_t cus = ga_hip_numprocs(ctx) ? ga_hip_numprocs(ctx) : 256;
   unsigned lanes = 64;
@@ -930,7 +948,7 @@ int GpuArray_embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids
                        int check_error) {
   try {
     return embedding(out, table, ids, scale, ignore, check_error);
-  } catch (const std::bad_alloc &) {
+  } catch (...) {   // (std::bad_alloc, std::length_error)
     return no_memory(GpuArray_context(out));
   }
 }
@@ -939,7 +957,7 @@ int GpuArray_embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray
                             int accumulate, int check_error) {
   try {
     return embedding_grad(grad, dout, ids, scale, ignore, accumulate, check_error);
-  } catch (const std::bad_alloc &) {
+  } catch (...) {   // (std::bad_alloc, std::length_error)
     return no_memory(GpuArray_context(grad));
   }
 }
@@ -949,7 +967,7 @@ int GpuArray_token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, 
                             int check_error) {
   try {
     return token_logprobs(logp, entropy, stats, top_logp, top_ids, logits, ids, scale, ignore, check_error);
-  } catch (const std::bad_alloc &) {
+  } catch (...) {   // (std::bad_alloc, std::length_error)
     return no_memory(GpuArray_context(logits));
   }
 }
@@ -959,7 +977,7 @@ int GpuArray_token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, cons
                                  double scale, ssize_t ignore, int check_error) {
   try {
     return token_logprobs_grad(dlogits, logits, ids, stats, dlogp, entropy, dentropy, scale, ignore, check_error);
-  } catch (const std::bad_alloc &) {
+  } catch (...) {   // (std::bad_alloc, std::length_error)
     return no_memory(GpuArray_context(logits));
   }
 }
@@ -968,7 +986,7 @@ int GpuGlobalNorm_new(GpuGlobalNorm **g, gpucontext *ctx, const GpuArray **as, G
   *g = nullptr;
   try {
     return global_norm_new(g, ctx, as, rs, n);
-  } catch (const std::bad_alloc &) {
+  } catch (...) {   // (std::bad_alloc, std::length_error)
     return no_memory(ctx);
   }
 }
@@ -983,7 +1001,7 @@ void GpuGlobalNorm_free(GpuGlobalNorm *g) {
 int GpuGlobalNorm_norm(const GpuGlobalNorm *g, GpuArray *norm) {
   try {
     return global_norm_call(g, false, 0.0, norm, "GpuGlobalNorm_norm");
-  } catch (const std::bad_alloc &) {
+  } catch (...) {   // (std::bad_alloc, std::length_error)
     return no_memory(g->ctx);
   }
 }
@@ -991,7 +1009,7 @@ int GpuGlobalNorm_norm(const GpuGlobalNorm *g, GpuArray *norm) {
 int GpuGlobalNorm_clip(const GpuGlobalNorm *g, double max_norm, GpuArray *norm) {
   try {
     return global_norm_call(g, true, max_norm, norm, "GpuGlobalNorm_clip");
-  } catch (const std::bad_alloc &) {
+  } catch (...) {   // (std::bad_alloc, std::length_error)
     return no_memory(g->ctx);
   }
 }
@@ -999,7 +1017,7 @@ int GpuGlobalNorm_clip(const GpuGlobalNorm *g, double max_norm, GpuArray *norm) 
 int GpuArray_global_norm(GpuArray *norm, const GpuArray **as, size_t n) {
   try {
     return norm_and_clip(nullptr, as, n, 0.0, norm, "global_norm");
-  } catch (const std::bad_alloc &) {
+  } catch (...) {   // (std::bad_alloc, std::length_error)
     return no_memory(GpuArray_context(norm));
   }
 }
@@ -1007,7 +1025,7 @@ int GpuArray_global_norm(GpuArray *norm, const GpuArray **as, size_t n) {
 int GpuArray_clip_global_norm(GpuArray **rs, const GpuArray **as, size_t n, double max_norm, GpuArray *norm) {
   try {
     return norm_and_clip(rs != nullptr ? rs : (GpuArray **)as, as, n, max_norm, norm, "clip_global_norm");
-  } catch (const std::bad_alloc &) {
+  } catch (...) {   // (std::bad_alloc, std::length_error)
     return n != 0 ? no_memory(GpuArray_context(as[0])) : GA_MEMORY_ERROR;
   }
 }
