@@ -570,32 +570,32 @@ LM_FN void lm_fetch_rows(const lm_embed_grad &p, const ga_uint (&at)[LM_AHEAD], 
 /* A wavefront adds the tokens of a row, those whose bits are set, over one tile of columns. */
 LM_FN void lm_add_few(const lm_embed_grad &p, ga_uint key, ga_uint tile, ga_ulong (&left)[LM_FEW / 64]) {
   const ga_uint lane = LID_0 & 63;
-      const lm_columns mine = lm_columns_of(((ga_long)tile * 64 + lane) * LM_W, p.d);
-      float sum[LM_W];
+  const lm_columns mine = lm_columns_of(((ga_long)tile * 64 + lane) * LM_W, p.d);
+  float sum[LM_W];
 #pragma unroll
-      for (int e = 0; e < LM_W; e++) sum[e] = 0.0f;
+  for (int e = 0; e < LM_W; e++) sum[e] = 0.0f;
 #pragma unroll
-      for (int w = 0; w < LM_FEW / 64; w++) {
-        while (left[w] != 0) {
-          ga_uint at[LM_AHEAD];
-          ga_uint n = 0;
+  for (int w = 0; w < LM_FEW / 64; w++) {
+    while (left[w] != 0) {
+      ga_uint at[LM_AHEAD];
+      ga_uint n = 0;
 #pragma unroll
-          for (int u = 0; u < LM_AHEAD; u++) {
-            at[u] = left[w] != 0 ? w * 64 + (ga_uint)__builtin_ctzll(left[w]) : at[u > 0 ? u - 1 : 0];
-            n += left[w] != 0;
-            left[w] &= left[w] - 1;
-          }
-          float y[LM_AHEAD][LM_W];
-          lm_fetch_rows(p, at, mine, y);
+      for (int u = 0; u < LM_AHEAD; u++) {
+        at[u] = left[w] != 0 ? w * 64 + (ga_uint)__builtin_ctzll(left[w]) : at[u > 0 ? u - 1 : 0];
+        n += left[w] != 0;
+        left[w] &= left[w] - 1;
+      }
+      float y[LM_AHEAD][LM_W];
+      lm_fetch_rows(p, at, mine, y);
 #pragma unroll
-          for (int u = 0; u < LM_AHEAD; u++) {
-            if (u < n) {
+      for (int u = 0; u < LM_AHEAD; u++) {
+        if (u < n) {
 #pragma unroll
-              for (int e = 0; e < LM_W; e++) sum[e] += y[u][e];
-            }
-          }
+          for (int e = 0; e < LM_W; e++) sum[e] += y[u][e];
         }
       }
+    }
+  }
   lm_write_run(p, key, mine, sum);
 }
 /* What is added to: a group for each token and p.part_tiles tiles, one tile a
