@@ -613,8 +613,8 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
   if (v > 0x3fffffff) return c.fail(GA_XLARGE_ERROR, "too many columns");
   // A row that a wavefront covers in eight rounds of loads belongs to one
   // wavefront, a longer one to a group, which grows while there are too few
-  // rows to fill the chip; below that, rows are cut in pieces of at least two
-  // chunks per lane, of which the last one to end joins them all.  Rows of bfloat16 with
+  // rows to fill the chip; below that, rows are cut in pieces of at least one
+  // batch for each lane, of which the last one to end joins them all.  Rows of bfloat16 with
   // entropy, us by the lanes 64, 256, 512, 1024 (and pieces):
   //   32768 rows of 2000     33    57   136   323
   //   32768 rows of 4000     51    69   131   315
@@ -632,7 +632,10 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
   size_t pieces = 1, piece_chunks = row_chunks;
   if (row_chunks > 512 && t * 2 <= cus && t <= ga_hip_redux_counters_max) {
     lanes = 256;
-    pieces = std::min((2 * cus + t - 1) / t, (row_chunks + 511) / 512);
+    // (one batch of loads: 16 elements a lane; half of that or twice as much: 8 rows of 50257 floats,
+    // 20 alternatives, 11.8, 10.4 and 11.4 us, of bfloat16 11.6, 10.2 and 11.3)
+    const size_t batch = 256 * gpuarray_get_elsize(logits->typecode);
+    pieces = std::min((2 * cus + t - 1) / t, (row_chunks + batch - 1) / batch);
     piece_chunks = (row_chunks + pieces - 1) / pieces;
     pieces = (row_chunks + piece_chunks - 1) / piece_chunks;
   }
