@@ -1007,19 +1007,27 @@ LM_FN ga_ulong lm_lane(ga_ulong k, int lane) {
          (ga_uint)__builtin_amdgcn_readlane((int)(ga_uint)k, lane);
 }
 
-/* The same network on 32-bit words: the k-th largest of 64 of them, for every lane. */
+/* The same network on 32-bit words: a word that n of the 64 are not below, for every
+ * lane; the n-th largest, or, for n up to 8, the n-th largest of the 16 maxima of four
+ * lanes, which costs half as much and lets few more pass (for 5 of 64 5.7 in place of 5.2). */
 template <int MASK> LM_FN void lm_step32(ga_uint &k) {
   const ga_uint other = lm_xor<MASK>(k);
   const bool lower = (LID_0 & (1u << (31 - __builtin_clz(MASK)))) == 0;
   k = lower ? max(k, other) : min(k, other);
 }
 LM_FN ga_uint lm_kth(ga_uint k, ga_int n) {
+  if (n <= 8) {
+    k = max(k, lm_xor<16>(k));
+    k = max(k, lm_xor<32>(k));
+  }
   lm_step32<1>(k);
   lm_step32<3>(k); lm_step32<1>(k);
   lm_step32<7>(k); lm_step32<2>(k); lm_step32<1>(k);
   lm_step32<15>(k); lm_step32<4>(k); lm_step32<2>(k); lm_step32<1>(k);
-  lm_step32<31>(k); lm_step32<8>(k); lm_step32<4>(k); lm_step32<2>(k); lm_step32<1>(k);
-  lm_step32<63>(k); lm_step32<16>(k); lm_step32<8>(k); lm_step32<4>(k); lm_step32<2>(k); lm_step32<1>(k);
+  if (n > 8) {
+    lm_step32<31>(k); lm_step32<8>(k); lm_step32<4>(k); lm_step32<2>(k); lm_step32<1>(k);
+    lm_step32<63>(k); lm_step32<16>(k); lm_step32<8>(k); lm_step32<4>(k); lm_step32<2>(k); lm_step32<1>(k);
+  }
   return (ga_uint)__builtin_amdgcn_readlane((int)k, n - 1);
 }
 
