@@ -1082,8 +1082,8 @@ LM_FN void lm_raise(lm_best &b, ga_uint ordered) {
  * whoever misses a rise keeps more than it needs.  Where `top` is not small each of them
  * also leaves its m-th best element, m = top / W rounded up: no fewer than `top`
  * are not below the lowest of those, which is more than one of them finds alone
- * (4096 rows of 50257 bfloat16 with entropy: 50 alternatives 158 -> 133 us, 20 129 -> 124, and
- * for 5 it is not worth its barrier). */
+ * (4096 rows of 50257 bfloat16 with entropy: 50 alternatives 133 us, without parts 158; for 5 it is not
+ * worth its barrier). */
 #define LM_WAVES (LM_LANES / 64)
 #if LM_LANES > 64 && LM_TOP
 static LOCAL_MEM ga_uint lm_shared_bar, lm_parts[LM_WAVES];
@@ -1333,8 +1333,8 @@ LM_FN void lm_join_pieces(const lm_logprobs &p, ga_long r) {
 /* One pass over the row with the running maximum and sums; what an element costs is a
  * multiply-add, an exponential and an addition, one more multiply-add with the entropy, and half a
  * maximum.  4096 rows of 50257 bfloat16 with entropy take 67 us (412 MB, 6.1 TB/s) where the vector
- * instructions alone take about 52; 65536 rows of 1000 floats with 5 alternatives 60 to 65 us
- * (262 MB, 4.2 TB/s): a wavefront sees its row in one batch, and the alternatives' networks and rounds
+ * instructions alone take about 52; 65536 rows of 1000 floats with 5 alternatives 58 to 63 us
+ * (262 MB, 4.3 TB/s): a wavefront sees its row in one batch, and the alternatives' networks and rounds
  * are half of its instructions.
  *
  * LM_LANES lanes share a row, or one of its pieces (LM_SPLIT): a loop over
