@@ -242,11 +242,11 @@ bool overlaps_itself(const GpuArray *a) {
 }
 
 // Checks of one operator's arguments; the first failure stays.
-struct checker {
+struct argument_rules {
   gpucontext *ctx;
   const char *who;
   int err = GA_NO_ERROR;
-  checker(gpucontext *c, const char *w) : ctx(c), who(w) {}
+  argument_rules(gpucontext *c, const char *w) : ctx(c), who(w) {}
   int fail(int code, const char *what) {
     if (err == GA_NO_ERROR) err = ga_err_fmt(ctx->err, code, "%s: %s", who, what);
     return err;
@@ -359,7 +359,7 @@ char *ga_language_gen_source(unsigned long long variant) {
 static int embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, double scale, ssize_t ignore,
                      int check_error) {
   gpucontext *ctx = GpuArray_context(out);
-  checker c(ctx, "embedding");
+  argument_rules c(ctx, "embedding");
   c.array(out, "out", 2);
   c.array(table, "table", 2);
   c.array(ids, "ids", 1);
@@ -384,7 +384,8 @@ static int embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, 
   unsigned lanes_log2 = 0;
   while (lanes_log2 < 8 && ((size_t)1 << lanes_log2) < row_lanes) lanes_log2++;
   const size_t row_groups = (n + ((size_t)1024 >> lanes_log2) - 1) / ((size_t)1024 >> lanes_log2);
-  if (row_groups > max_groups(256) || segments > max_groups(256) / row_groups) return c.fail(GA_XLARGE_ERROR, "too many elements");
+  if (row_groups > max_groups(256) || segments > max_groups(256) / row_groups)
+    return c.fail(GA_XLARGE_ERROR, "too many elements");
   GpuKernel *k;
   gpudata *errbuf = nullptr;
   int err = lm_kernel(ctx, lm_variant(LM_EMBED, table->typecode, out->typecode, ids->typecode, 0), "lm_embed_rows",
@@ -400,7 +401,7 @@ static int embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, 
 static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *ids, double scale, ssize_t ignore,
                           int accumulate, int check_error) {
   gpucontext *ctx = GpuArray_context(grad);
-  checker c(ctx, "embedding_grad");
+  argument_rules c(ctx, "embedding_grad");
   c.array(grad, "grad", 2);
   c.array(dout, "dout", 2);
   c.array(ids, "ids", 1);
@@ -450,7 +451,8 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
     // rows of 6000 floats 17.5 us, in parts 10.5).
     a.part_tiles = !accumulate && dense && d * osize % 16 != 0 && tiles <= 16 && v >= 4096 ? 16 : 4;
     const size_t parts = (tiles + a.part_tiles - 1) / a.part_tiles;
-    a.rows = (uint32_t)std::min({std::max<size_t>(8192 / (std::min(d, a.part_tiles * cols) * osize), 1), v * parts / 512 + 1, (size_t)512});
+    const size_t fit = std::max<size_t>(8192 / (std::min(d, a.part_tiles * cols) * osize), 1);
+    a.rows = (uint32_t)std::min({fit, v * parts / 512 + 1, (size_t)512});
     const size_t row_groups = accumulate ? n : v ? (v + a.rows - 1) / a.rows : 1;
     if (row_groups == 0) return GA_NO_ERROR;
     if (parts > max_groups(256) / row_groups) return c.fail(GA_XLARGE_ERROR, "too many elements");
@@ -572,7 +574,7 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
 static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, GpuArray *top_logp, GpuArray *top_ids,
                           const GpuArray *logits, const GpuArray *ids, double scale, ssize_t ignore, int check_error) {
   gpucontext *ctx = GpuArray_context(logits);
-  checker c(ctx, "token_logprobs");
+  argument_rules c(ctx, "token_logprobs");
   c.array(logits, "logits", 2);
   if (c.err != GA_NO_ERROR) return c.err;
   const size_t t = logits->dimensions[0], v = logits->dimensions[1];
@@ -671,7 +673,7 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
                                const GpuArray *dlogp, const GpuArray *entropy, const GpuArray *dentropy, double scale,
                                ssize_t ignore, int check_error) {
   gpucontext *ctx = GpuArray_context(dlogits);
-  checker c(ctx, "token_logprobs_grad");
+  argument_rules c(ctx, "token_logprobs_grad");
   c.array(dlogits, "dlogits", 2);
   c.array(logits, "logits", 2);
   c.array(stats, "stats", 2);
@@ -712,8 +714,8 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
   if (segments > 4 * max_groups(256) / t) return c.fail(GA_XLARGE_ERROR, "too many elements");
   GpuKernel *k;
   gpudata *errbuf = nullptr;
-  int err = lm_kernel(ctx, lm_variant(LM_LOGPROBS_GRAD, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT, entropy != nullptr),
-                      "lm_logprobs_grad_rows", sizeof(logprobs_grad_args), &k);
+  const lm_variant var(LM_LOGPROBS_GRAD, logits->typecode, GA_FLOAT, ids ? ids->typecode : GA_INT, entropy != nullptr);
+  int err = lm_kernel(ctx, var, "lm_logprobs_grad_rows", sizeof(logprobs_grad_args), &k);
   if (err == GA_NO_ERROR) err = lm_errbuf(ctx, logits, &errbuf);
   if (err != GA_NO_ERROR) return err;
   auto ptr = [](const GpuArray *x) -> void * { return x ? at(x) : nullptr; };
@@ -742,7 +744,7 @@ struct norm_plan {
 static const size_t NORM_PIECE = 1024;       // chunks of 16 bytes
 static const size_t NORM_MAX_GROUPS = 256;   // per table
 
-static int norm_check(checker &c, const GpuArray *norm) {
+static int norm_check(argument_rules &c, const GpuArray *norm) {
   if (norm == nullptr) return c.err;
   if (norm->nd > 1 || (norm->nd == 1 && norm->dimensions[0] != 1))
     return c.fail(GA_INVALID_ERROR, "must be 0-d or have one element", "norm");
@@ -755,7 +757,7 @@ static int norm_check(checker &c, const GpuArray *norm) {
 }
 
 // The arrays `as` and, if rs is not NULL, what clipping writes, checked against each other.
-static int norm_arrays(checker &c, GpuArray **rs, const GpuArray **as, size_t n, norm_plan *plan) {
+static int norm_arrays(argument_rules &c, GpuArray **rs, const GpuArray **as, size_t n, norm_plan *plan) {
   std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
   plan->tensors.reserve(n);
   for (size_t i = 0; i < n; i++) {
@@ -804,7 +806,7 @@ static int norm_arrays(checker &c, GpuArray **rs, const GpuArray **as, size_t n,
 }
 
 // `norm` must lie outside all the arrays.
-static int norm_apart(checker &c, const norm_plan &plan, const GpuArray *norm) {
+static int norm_apart(argument_rules &c, const norm_plan &plan, const GpuArray *norm) {
   if (norm == nullptr) return GA_NO_ERROR;
   const uintptr_t lo = (uintptr_t)at(norm), hi = lo + GpuArray_ITEMSIZE(norm);
   static const size_t sizes[4] = {4, 2, 2, 8};
@@ -823,7 +825,7 @@ struct norm_table {
   const void *device;
   uint32_t n, pieces;
 };
-static int norm_run(checker &c, const std::vector<norm_table> &tables, bool clip, double max_norm, const GpuArray *norm) {
+static int norm_run(argument_rules &c, const std::vector<norm_table> &tables, bool clip, double max_norm, const GpuArray *norm) {
   gpucontext *ctx = c.ctx;
   const bool by_table = tables.size() == 1 && tables[0].tensors == nullptr;
   const size_t size = by_table ? sizeof(table_args) : sizeof(tensors_args);
@@ -872,7 +874,7 @@ static int norm_run(checker &c, const std::vector<norm_table> &tables, bool clip
 // One call on a list of arrays, which travel with the arguments of the launches.
 static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double max_norm, GpuArray *norm, const char *who) {
   if (n == 0 && norm == nullptr) return GA_NO_ERROR;
-  checker c(GpuArray_context(norm != nullptr ? norm : as[0]), who);
+  argument_rules c(GpuArray_context(norm != nullptr ? norm : as[0]), who);
   norm_plan plan;
   if (std::isnan(max_norm) || max_norm < 0) return c.fail(GA_VALUE_ERROR, "max_norm must be 0 or above");
   if (norm_check(c, norm) != GA_NO_ERROR || norm_arrays(c, rs, as, n, &plan) != GA_NO_ERROR ||
@@ -901,7 +903,7 @@ struct _GpuGlobalNorm {
 };
 
 static int global_norm_new(GpuGlobalNorm **out, gpucontext *ctx, const GpuArray **as, GpuArray **rs, size_t n) {
-  checker c(ctx, "GpuGlobalNorm_new");
+  argument_rules c(ctx, "GpuGlobalNorm_new");
   if (ga_hip_capturing(ctx))
     return c.fail(GA_UNSUPPORTED_ERROR, "the stream records a graph: make the operator before recording");
   std::unique_ptr<GpuGlobalNorm> g(new GpuGlobalNorm());
@@ -933,7 +935,7 @@ static int global_norm_new(GpuGlobalNorm **out, gpucontext *ctx, const GpuArray 
 }
 
 static int global_norm_call(const GpuGlobalNorm *g, bool clip, double max_norm, GpuArray *norm, const char *who) {
-  checker c(g->ctx, who);
+  argument_rules c(g->ctx, who);
   if (std::isnan(max_norm) || max_norm < 0) return c.fail(GA_VALUE_ERROR, "max_norm must be 0 or above");
   if (clip && !g->clips) return c.fail(GA_INVALID_ERROR, "the operator was made without results");
   if (norm_check(c, norm) != GA_NO_ERROR || norm_apart(c, g->plan, norm) != GA_NO_ERROR) return c.err;
