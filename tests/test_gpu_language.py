@@ -862,6 +862,83 @@ def test_language_operators_replay_from_a_graph(ctx):
         hip.hipGraphDestroy(graph)
 
 
+def test_two_graphs_share_the_workspaces(ctx):
+    """Single steps and a small batch, recorded apart and replayed in turn: rows in pieces and their counters, few
+    tokens added and not, the scratch of the sort."""
+    hip = C.CDLL("libamdhip64.so")
+    stream = C.c_void_p(_lib.extension("hip_get_stream", C.c_void_p, [C.c_void_p])(ctx.ctx))
+    rng = np.random.default_rng(29)
+    v, d = 50257, 24
+    mk = lambda shape, dt="float32": gpuarray.zeros(shape, dt, context=ctx)  # noqa: E731
+    table = gpuarray.array(rng.standard_normal((v, d)).astype(np.float32), context=ctx)
+
+    class Step(object):
+        def __init__(self, n, t):
+            self.logits = gpuarray.array(rng.standard_normal((t, v)).astype(np.float16), context=ctx)
+            self.ids, self.targets = mk((n,), "int32"), mk((t,), "int64")
+            self.dlogp = gpuarray.array(np.full(t, -1.0 / t, np.float32), context=ctx)
+            self.out = dict(h=mk((n, d)), logp=mk((t,)), ent=mk((t,)), stats=mk((t, 2)), topl=mk((t, 20)),
+                            topi=mk((t, 20), "int32"), dl=mk((t, v), "float16"), g=mk((v, d)), norm=mk(()))
+            self.sum = mk((v, d))
+            self.op = ga.GlobalNorm([self.out["g"], self.out["dl"]])
+
+        def issue(self):
+            o = self.out
+            ga.embedding(table, self.ids, out=o["h"], check=False)
+            ga.token_logprobs(self.logits, self.targets, out=ga.TokenLogprobs(o["logp"], o["ent"], o["stats"], o["topl"], o["topi"]),
+                              check=False)
+            ga.token_logprobs_grad(self.logits, self.targets, o["stats"], self.dlogp, out=o["dl"], check=False)
+            ga.embedding_grad(o["h"], self.ids, o["g"], check=False)
+            ga.embedding_grad(o["h"], self.ids, self.sum, accumulate=True, check=False)
+            self.op.clip(0.5, norm=o["norm"])
+
+        def values(self):
+            return {k: np.asarray(a) for k, a in self.out.items()}
+
+    steps = [Step(8, 3), Step(700, 40)]
+    graphs = []
+    for s in steps:
+        s.issue()
+    ctx.sync()
+    try:
+        for s in steps:
+            graph, gexec = C.c_void_p(), C.c_void_p()
+            assert hip.hipStreamBeginCapture(stream, 0) == 0
+            try:
+                s.issue()
+            finally:
+                rc = hip.hipStreamEndCapture(stream, C.byref(graph))
+            assert rc == 0
+            assert hip.hipGraphInstantiate(C.byref(gexec), graph, None, None, C.c_size_t(0)) == 0
+            graphs.append((graph, gexec))
+        for turn in range(4):
+            for s in steps:
+                s.ids.write(rng.integers(0, v, s.ids.shape[0]).astype(np.int32))
+                s.targets.write(rng.integers(0, v, s.targets.shape[0]))
+                s.sum.memset(0)
+            for s in steps:
+                s.issue()
+            ctx.sync()
+            want, sums = [s.values() for s in steps], [np.asarray(s.sum) for s in steps]
+            for s in steps:
+                for a in s.out.values():
+                    a.write(np.full(a.shape, 3, a.dtype))
+                s.sum.memset(0)
+            for i in (0, 1, 0, 1)[turn % 2:]:
+                assert hip.hipGraphLaunch(graphs[i][1], stream) == 0
+            ctx.sync()
+            for i, s in enumerate(steps):
+                got = s.values()
+                for k in got:
+                    assert np.array_equal(got[k], want[i][k]), (turn, i, k)
+                times = (0, 1, 0, 1)[turn % 2:].count(i)          # every replay adds the same rows once more
+                assert np.all(np.abs(np.asarray(s.sum) - times * sums[i]) <= 4 * U * np.abs(times * sums[i]))
+    finally:
+        for graph, gexec in graphs:
+            hip.hipGraphExecDestroy(gexec)
+            hip.hipGraphDestroy(graph)
+
+
 def test_a_bigram_model_is_trained(ctx):
     """Rows of a (v, v) table are the logits of the next token: two steps of these operators and an update through
     GpuElemwise against the same steps in 64 bits."""
