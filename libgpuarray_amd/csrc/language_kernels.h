@@ -830,6 +830,13 @@ KERNEL void __launch_bounds__(256) lm_embed_grad_join(const lm_embed_grad p) {
 }
 #endif
 
+/* R = by * m, the largest logit in powers of two, is rounded to a float, and what the rounding leaves,
+ * r = by * m - R, is part of every exponent by * x - R: of the largest element's too, which is r in place of 0.
+ * Below 2^30 that is 32 at most, half a step of R, and the exponential and the sums hold it. From there on r would
+ * leave the range of the exponential (past 2^31: 128 and more); but by * x of neighbouring numbers is 64 or more apart
+ * then, 2^-64 of an element is none, and so only the elements that are equal to m count, with exponent 0. */
+#define LM_FAR 1073741824.0f
+
 #if LM_KIND == LM_K_LOGPROBS
 struct lm_logprobs {
   GLOBAL_MEM const LM_X *logits;
@@ -852,17 +859,16 @@ struct lm_logprobs {
  *   s = sum of 2^(by * x - R(m)),   w = sum of (by * x - R(m)) 2^(by * x - R(m)),
  * where m is the largest x; R(m) being a number that is known exactly, its
  * rounding is no error of s or w.  One multiply-add and one exponential per
- * element.  -inf has no part in either sum.  Where |R| is past 1e30 the
- * difference between neighbouring values is past 1e22, so that s counts the
- * elements that are equal to m and w is 0: rows of a type's lowest value. */
+ * element.  -inf has no part in either sum.  Where |R| is past LM_FAR s
+ * counts the elements that are equal to m, and w is 0: rows of a mask's value, and
+ * what a lane has of one before it meets anything else. */
 struct lm_state {
   float m, s, w, pad;
 };
 #define LM_LOWEST (-3.402823466e+38f)
-#define LM_FAR 1e30f
 
-/* R(from) - R(to), from <= to; far below, and where either is far out, -300, which
- * is as good as -inf for the exponential and safe to multiply with 0 */
+/* R(from) - R(to), from <= to; far below, as every smaller number is where either is past LM_FAR, at least -300,
+ * which is as good as -inf for the exponential and safe to multiply with 0 */
 LM_FN float lm_shift(float from, float to, float by) {
   const float d = __builtin_fmaxf(from * by - to * by, -300.0f);
   return from == to ? 0.0f : d;

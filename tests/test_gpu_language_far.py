@@ -1,0 +1,130 @@
+"""Log probabilities of rows with logits far out: finite masks, rows of nothing but a mask, maxima of any size,
+against the definition in 64 bits.
+
+The kernels sum 2^(by * x - R) with by = scale * log2(e) and R = by * m rounded, m the largest x.  What the rounding
+leaves, r = by * m - R, is no error, but it is part of every exponent: as long as R is below 2^30 it is at most 32, half
+a step there.  Past that only the elements that are equal to m count: neighbouring numbers differ by 64 or more in by * x,
+and 2^-64 of an element is nothing next to it.
+
+With F = 32 ln 2 < 23, what r adds to the bounds of test_gpu_language.py: an exponent by * x - R is rounded at a size
+of up to |z| log2(e) + 32, which is F u of its power of two (24 u of the sum); the logarithm of the sum is up to F larger
+and off by 4 u of that, the product r ln 2 by 2 u of it: 24 u + 6 F u < 164 u of the log sum.  The sum of the products
+that the entropy is taken from is larger by r of the sum, off by twice the sum's relative error and 8 u."""
+import numpy as np
+import pytest
+
+import libgpuarray_amd as ga
+from libgpuarray_amd import gpuarray
+from test_gpu_language import U, decode, encode, logprob_bounds, run_logprobs, softmax64
+
+pytestmark = pytest.mark.gpu
+
+LOG2E = 1.4426950408889634
+F = 23
+MASKS = {"float32": [-1e4, -1e9, -1e10, -3e10, -1e20, -1e30, float(np.finfo(np.float32).min)],
+         "bfloat16": [-1e9, -1e10, -3e10, -1e20, -1e30, float(ga.from_bfloat16(np.array([0xff7f], np.uint16).view(ga.bfloat16))[0])],
+         "float16": [-1e4, -65504.0]}
+CASES = [(kind, low) for kind in MASKS for low in MASKS[kind]]
+
+
+def masked_rows(v, low, rng):
+    """Rows with `low` in whole lanes, wavefronts and pieces; a running maximum has to leave it in most of them."""
+    k = max(v // 16, 1)
+    x = np.round(rng.standard_normal((10, v)) * 2, 2)
+    x[0] = low
+    x[1, :-k] = low
+    x[2, : v // 2] = low
+    x[3, rng.random(v) < 0.9] = low
+    x[4, -1] = low
+    x[5] = 0.0
+    x[5, v // 2] = -low                                  # one large maximum
+    x[6, [0, v // 2, v - 1]] = -low                      # three of them
+    x[7] = low
+    x[7, : v // 2] = -np.inf
+    x[8] = low
+    x[8, : v // 2] = low * 0.5                           # half of what was a mask is the maximum
+    x[9] = -1000.0
+    x[9, : v // 2] = low
+    x[9, -k:] = 3.0
+    return x
+
+
+def remainders(x, scale):
+    """32 for rows that have R anywhere between 2^8 and 2^30 (below that the bounds of nearer logits hold), else 0; -> F or 0."""
+    r = np.abs(np.where(np.isfinite(x), x, 0)) * scale * LOG2E
+    return np.where(((r >= 2.0 ** 8) & (r <= 2.0 ** 30 * (1 + 2.0 ** -20))).any(1), F, 0)
+
+
+def in_float(a):
+    """64-bit values with those that no float holds infinite."""
+    return np.where(np.abs(a) >= 2.0 ** 128 * (1 - 2.0 ** -25), np.copysign(np.inf, a), a)
+
+
+def expected(x, scale):
+    """(m, log sum, log p, entropy) and bounds of the last three."""
+    m, ls, z, p = softmax64(x, scale)
+    ls_err, lp_err, h_err = logprob_bounds(x, scale)
+    f = remainders(x, scale)
+    s_rel = (x.shape[1] / 64 + 32 + 128 + 4 + 24) * U + 3 * U * (p * np.where(p > 0, np.abs(z), 0)).sum(1)
+    ls_err = ls_err + np.where(f > 0, 164 * U, 0)
+    lp_err = lp_err + np.where(f > 0, 164 * U, 0)[:, None]
+    h_err = h_err + f * (2 * s_rel + 8 * U) + np.where(f > 0, 164 * U, 0)
+    return m, ls, z - ls[:, None], ls - (p * np.where(p > 0, z, 0)).sum(1), ls_err, lp_err, h_err
+
+
+def close(got, want, bound):
+    want = in_float(want)
+    fin = np.isfinite(want)
+    assert np.array_equal(got[~fin], want[~fin]), np.argwhere((got != want) & ~fin)[:4]
+    off = np.abs(got[fin] - want[fin])
+    assert np.all(off <= bound[fin]), (float((off / bound[fin]).max()), got[fin][:8], want[fin][:8])
+
+
+def check_far(ctx, x, scale, top, rng):
+    x64 = decode(x)
+    t, v = x64.shape
+    ids = rng.integers(0, v, t)
+    m, ls, lp, entropy, ls_err, lp_err, h_err = expected(x64, scale)
+    logp, h, stats, top_logp, top_ids = run_logprobs(ctx, gpuarray.array(x, context=ctx), gpuarray.array(ids, context=ctx), v,
+                                                     scale, top)
+    assert np.array_equal(stats[:, 0], m.astype(np.float32))
+    close(stats[:, 1], ls, ls_err)
+    close(logp, lp[np.arange(t), ids], lp_err[np.arange(t), ids])
+    close(h, entropy, h_err)
+    order = np.argsort(-x64, axis=1, kind="stable")[:, :top]
+    assert np.array_equal(top_ids, order)
+    close(top_logp, np.take_along_axis(lp, order, 1), np.take_along_axis(lp_err, order, 1))
+
+
+@pytest.mark.parametrize("kind,low", CASES)
+@pytest.mark.parametrize("v", [20, 1000, 60000])
+def test_finite_masks(ctx, kind, low, v):
+    rng = np.random.default_rng(v)
+    x = encode(masked_rows(v, low, rng), kind)
+    for scale, top in ((0.5, 5), (1.0, 20), (float(np.float32(1.4)), 1)):
+        check_far(ctx, x, scale, top, rng)
+
+
+@pytest.mark.parametrize("low", [-1e9, -1e10, -1e20])
+@pytest.mark.parametrize("t,v", [(300, 5000), (140, 60000)])
+def test_finite_masks_of_rows_that_a_group_shares(ctx, low, t, v):
+    rng = np.random.default_rng(t)
+    x = masked_rows(v, low, rng)[np.arange(t) % 10].astype(np.float32)
+    check_far(ctx, x, 1.0, 5, rng)
+
+
+def maxima(exponent):
+    """Maxima m with by * m on both sides of 2^exponent, positive and negative, and neighbours of them."""
+    m = np.array([2.0 ** exponent / LOG2E * f for f in (0.75, 0.97, 0.9999999, 1.0, 1.0000001, 1.03, 1.3)], np.float32)
+    m = np.concatenate([m, -m])
+    x = np.full((m.size, 700), -np.inf, np.float32)
+    x[:, ::3] = m[:, None]
+    x[:, 1::3] = np.nextafter(m, np.float32(-np.inf))[:, None]
+    x[:, 2::6] = (m - np.abs(m) * np.float32(0.01))[:, None]
+    return x
+
+
+@pytest.mark.parametrize("exponent", [20, 24, 27, 28, 29, 30, 31, 32, 33, 40, 64])
+def test_maxima_around_the_limit(ctx, exponent):
+    """The two ways of counting meet at 2^30."""
+    check_far(ctx, maxima(exponent), 1.0, 5, np.random.default_rng(exponent))
