@@ -867,11 +867,11 @@ struct lm_state {
 };
 #define LM_LOWEST (-3.402823466e+38f)
 
-/* R(from) - R(to), from <= to; far below, as every smaller number is where either is past LM_FAR, at least -300,
- * which is as good as -inf for the exponential and safe to multiply with 0 */
+/* R(from) - R(to), from <= to; -300, which is as good as -inf for the exponential and safe to multiply
+ * with 0, where that is lower, and for any two that differ where R(to) is past LM_FAR (both may be rounded to the same number). */
 LM_FN float lm_shift(float from, float to, float by) {
-  const float d = __builtin_fmaxf(from * by - to * by, -300.0f);
-  return from == to ? 0.0f : d;
+  const float r = to * by, d = __builtin_fmaxf(from * by - r, -300.0f);
+  return from == to ? 0.0f : __builtin_fabsf(r) <= LM_FAR ? d : -300.0f;
 }
 LM_FN void lm_rescale(lm_state &a, float m, float by) {
   const float d = lm_shift(a.m, m, by), f = __builtin_amdgcn_exp2f(d);

@@ -128,3 +128,19 @@ def maxima(exponent):
 def test_maxima_around_the_limit(ctx, exponent):
     """The two ways of counting meet at 2^30."""
     check_far(ctx, maxima(exponent), 1.0, 5, np.random.default_rng(exponent))
+
+
+def one_among_neighbours(v, size):
+    """Rows of the next lower number, and one maximum that meets them when lanes, wavefronts or pieces are joined."""
+    rng = np.random.default_rng(v)
+    m = np.concatenate([rng.uniform(size, 2 * size, 12), -rng.uniform(size, 2 * size, 12)]).astype(np.float32)
+    x = np.repeat(np.nextafter(m, np.float32(-np.inf))[:, None], v, 1)
+    x[np.arange(m.size), rng.integers(0, v, m.size)] = m
+    return x
+
+
+@pytest.mark.parametrize("size", [2.0 ** 22, 2.0 ** 28, 2.0 ** 30, 2.0 ** 31, 1e20, 1e30, 1.6e38])
+@pytest.mark.parametrize("v", [20, 700, 60000])
+def test_one_maximum_among_its_neighbours(ctx, size, v):
+    """What is rounded to the same multiple of log2(e) is not equal for that."""
+    check_far(ctx, one_among_neighbours(v, size), 1.0, 5, np.random.default_rng(1))
