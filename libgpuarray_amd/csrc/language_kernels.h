@@ -1526,7 +1526,7 @@ KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad 
 #endif
   const float big = p.by * m;
   const bool nothing = ls == -INFINITY;
-  const bool far = !(__builtin_fabsf(big) <= 1e30f);   /* as for the statistics: p is exp(-ls) where x is m, else 0 */
+  const bool far = !(__builtin_fabsf(big) <= LM_FAR);   /* R is no part of the exponent then, as in the statistics */
   const float rest = (far ? 0.0f : __builtin_fmaf(p.by, m, -big)) + ls * 1.4426950408889634f;
   const float a = -p.scale * (g + gh * h) + (ls - ls), b = -p.scale * gh * 0.6931471805599453f;   /* (NaN where ls is) */
   const float own = p.scale * g;
@@ -1543,7 +1543,7 @@ KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad 
 #pragma unroll
       for (int e = 0; e < LM_E; e++) {
         float l = __builtin_fmaf(y[u][e], p.by, -big) - rest;
-        if (far) l = y[u][e] == m ? -rest : -300.0f;
+        if (far) l = (y[u][e] - m) * p.by - rest;
         const float q = __builtin_amdgcn_exp2f(l);
 #if LM_ENT
         d[e] = q * __builtin_fmaf(b, __builtin_fmaxf(l, -300.0f), a);

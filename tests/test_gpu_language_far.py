@@ -15,7 +15,7 @@ import pytest
 
 import libgpuarray_amd as ga
 from libgpuarray_amd import gpuarray
-from test_gpu_language import U, decode, encode, logprob_bounds, run_logprobs, softmax64
+from test_gpu_language import HALF_STEP, TINY, U, decode, encode, grad64, logprob_bounds, run_logprobs, softmax64
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,59 @@ def one_among_neighbours(v, size):
 def test_one_maximum_among_its_neighbours(ctx, size, v):
     """What is rounded to the same multiple of log2(e) is not equal for that."""
     check_far(ctx, one_among_neighbours(v, size), 1.0, 5, np.random.default_rng(1))
+
+
+# ---- the gradient -----------------------------------------------------------------------------------
+
+def check_far_grad(ctx, x, kind, scale, rng):
+    """With statistics that are rounded from 64 bits, and with those that the operator leaves."""
+    x64 = decode(x)
+    t, v = x64.shape
+    ids = rng.integers(0, v, t)
+    g, gh = (rng.standard_normal(t).astype(np.float32) for _ in range(2))
+    want, bound, h, m, ls = grad64(x64, ids, g.astype(np.float64), gh.astype(np.float64), scale)
+    _, _, lp, _, ls_err, _, h_err = expected(x64, scale)
+    _, _, _, p = softmax64(x64, scale)
+    lp, size = np.where(p > 0, lp, 0), np.abs(g) + np.abs(gh)
+    # r is part of the exponent, of what is taken from it, and of the difference: three roundings at a size that is up to
+    # 32 larger, F u each of p and of log p
+    rest = np.where(remainders(x64, scale) > 0, 3 * F * U, 0)[:, None]
+    bound = bound + scale * p * rest * (np.abs(g)[:, None] + np.abs(gh)[:, None] * (np.abs(lp) + np.abs(h)[:, None] + 1))
+    dev = lambda a: gpuarray.array(a, context=ctx)  # noqa: E731
+    own = ga.token_logprobs(dev(x), dev(ids), scale=scale, entropy=True)
+    exact = dev(np.stack([m, ls], 1).astype(np.float32)), dev(h.astype(np.float32))
+    # what the operator's own statistics may be off by
+    joined = scale * p * (ls_err[:, None] * (size[:, None] * 2 + np.abs(gh)[:, None] * (np.abs(lp) + np.abs(h)[:, None])) +
+                          (h_err * np.abs(gh))[:, None])
+    for stats, entropy, more in ((*exact, 0), (own.stats, own.entropy, joined)):
+        limit = (bound + more) * (1 + 2.0 ** -7) + np.abs(want) * HALF_STEP[kind] + TINY[kind]
+        got = decode(ga.token_logprobs_grad(dev(x), dev(ids), stats, dev(g), entropy=entropy, dentropy=dev(gh), scale=scale))
+        off = np.abs(got - want)
+        assert np.all(off <= limit), (np.argwhere(~(off <= limit))[:4], float(np.nanmax(off / limit)))
+        want_g, bound_g = grad64(x64, ids, g.astype(np.float64), np.zeros(t), scale)[:2]
+        limit = (bound_g + scale * p * rest * np.abs(g)[:, None] + (more != 0) * scale * p * ls_err[:, None] * np.abs(g)[:, None])
+        limit = limit * (1 + 2.0 ** -7) + np.abs(want_g) * HALF_STEP[kind] + TINY[kind]
+        got = decode(ga.token_logprobs_grad(dev(x), dev(ids), stats, dev(g), scale=scale))
+        off = np.abs(got - want_g)
+        assert np.all(off <= limit), (np.argwhere(~(off <= limit))[:4], float(np.nanmax(off / limit)))
+
+
+@pytest.mark.parametrize("kind,low", CASES)
+@pytest.mark.parametrize("v", [20, 1000, 60000])
+def test_gradient_of_finite_masks(ctx, kind, low, v):
+    rng = np.random.default_rng(v + 1)
+    x = encode(masked_rows(v, low, rng), kind)
+    for scale in (0.5, 1.0, float(np.float32(1.4))):
+        check_far_grad(ctx, x, kind, scale, rng)
+
+
+@pytest.mark.parametrize("exponent", [20, 24, 27, 28, 29, 30, 31, 32, 33, 40, 64])
+def test_gradient_of_maxima_around_the_limit(ctx, exponent):
+    rng = np.random.default_rng(exponent + 1)
+    check_far_grad(ctx, maxima(exponent), "float32", 1.0, rng)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 22, 2.0 ** 28, 2.0 ** 30, 2.0 ** 31, 1e20, 1e30, 1.6e38])
+@pytest.mark.parametrize("v", [20, 700])
+def test_gradient_of_one_maximum_among_its_neighbours(ctx, size, v):
+    check_far_grad(ctx, one_among_neighbours(v, size), "float32", 1.0, np.random.default_rng(2))
