@@ -1194,6 +1194,11 @@ LM_FN lm_token lm_token_of(const lm_logprobs &p, ga_long r, LM_ID id) {
   }
   return k;
 }
+/* scale * (x - m), also where the difference is in no float (the product need not be so) */
+LM_FN float lm_scaled_difference(float x, float m, float scale) {
+  const float d = x - m;
+  return __builtin_fabsf(d) < INFINITY || x == -INFINITY ? d * scale : x * scale - m * scale;
+}
 /* What is written for row r; a whole wavefront. */
 LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a, ga_ulong list, lm_token token) {
   const ga_uint lane = LID_0 & 63;
@@ -1212,7 +1217,7 @@ LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a
         *p.err = -1;
         lp = NAN;
       } else if (token.id >= 0) {
-        lp = nothing ? -INFINITY : (token.x - m) * p.scale - ls;
+        lp = nothing ? -INFINITY : lm_scaled_difference(token.x, m, p.scale) - ls;
         if (ls != ls) lp = NAN;
       }
       *lm_at(p.logp, r * p.logp_step) = lp;
@@ -1239,7 +1244,7 @@ LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a
     if (lane < p.top) put(lane, NAN, lane);
     return;
   }
-  if (lane < n) put(lane, (lm_key_value(list) - m) * p.scale - ls, lm_key_index(list));
+  if (lane < n) put(lane, lm_scaled_difference(lm_key_value(list), m, p.scale) - ls, lm_key_index(list));
   /* fewer than `top` elements above -inf: the lowest indices of -inf follow.
    * They are among the first 2 * 64 elements, or the row is shorter. */
   for (ga_long base = 0; n < p.top && base < p.v; base += 64) {

@@ -200,3 +200,26 @@ def test_gradient_of_maxima_around_the_limit(ctx, exponent):
 @pytest.mark.parametrize("v", [20, 700])
 def test_gradient_of_one_maximum_among_its_neighbours(ctx, size, v):
     check_far_grad(ctx, one_among_neighbours(v, size), "float32", 1.0, np.random.default_rng(2))
+
+
+# ---- logits that are farther apart than the largest float ---------------------------------------------
+
+@pytest.mark.parametrize("scale", [0.25, 2.0 ** -20, 1.0])
+@pytest.mark.parametrize("v", [20, 60000])
+def test_logits_farther_apart_than_a_float(ctx, scale, v):
+    """x - m is -inf in 32 bits where scale * (x - m) need not be."""
+    top = float(np.finfo(np.float32).max)
+    x = np.full((4, v), -np.inf, np.float32)
+    x[0] = -top
+    x[0, 7] = top
+    x[1] = -2e38
+    x[1, v - 1] = 2.5e38
+    x[2, [3, 9]] = -3e38, 3e38
+    x[3, ::2] = -1e38
+    x[3, 1] = 3e38
+    check_far(ctx, x, scale, 3, np.random.default_rng(v))
+    ids = gpuarray.array(np.array([0, 0, 3, 0]), context=ctx)
+    got = np.asarray(ga.token_logprobs(gpuarray.array(x, context=ctx), ids, scale=scale).logp)
+    want = in_float(np.array([-2 * top, -4.5e38, -6e38, -4e38]) * scale)
+    fin = np.isfinite(want)
+    assert np.array_equal(got[~fin], want[~fin]) and np.all(np.abs(got[fin] - want[fin]) <= 6 * U * np.abs(want[fin]))
