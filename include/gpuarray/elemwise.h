@@ -35,7 +35,7 @@ GPUARRAY_PUBLIC GpuElemwise *GpuElemwise_new(gpucontext *ctx,
                                              gpuelemwise_arg *args,
                                              unsigned int nd, int flags);
 #define GE_NOADDR64    0x0001  /* do not pre-build 64-bit index kernels */
-#define GE_CONVERT_F16 0x0002  /* half arrays are seen as float in expr */
+#define GE_CONVERT_F16 0x0002  /* half arrays are seen as float in expr (bfloat16 always is) */
 
 GPUARRAY_PUBLIC void GpuElemwise_free(GpuElemwise *ge);
 

@@ -29,6 +29,15 @@ static int ga_extcopy(GpuArray *dst, const GpuArray *src) {
     return ga_err_set(ctx->err, GA_INVALID_ERROR, "src and dst context differ");
   if (ctx->extcopy_cache == nullptr) ctx->extcopy_cache = new extcopy_map();
   extcopy_map &m = *(extcopy_map *)ctx->extcopy_cache;
+  // bfloat16 is a float in an expression; from one to the other the bits are copied
+  GpuArray bits[2];
+  if (src->typecode == GA_BFLOAT16 && dst->typecode == GA_BFLOAT16) {
+    bits[0] = *src;
+    bits[1] = *dst;
+    bits[0].typecode = bits[1].typecode = GA_USHORT;
+    src = &bits[0];
+    dst = &bits[1];
+  }
   auto key = std::make_pair(src->typecode, dst->typecode);
   GpuElemwise *ge = nullptr;
   auto it = m.find(key);

@@ -152,10 +152,19 @@ bool local_is_float(const GpuElemwise *ge, const ge_arg &a) {
   return (ge->flags & GE_CONVERT_F16) && a.typecode == GA_HALF;
 }
 
+// What an argument is in the expression.  bfloat16 has no arithmetic of its own and is a float there,
+// whatever the flags: elements convert exactly when they are read, and are rounded once when they are written.
+const char *local_ctype(const GpuElemwise *ge, const ge_arg &a) {
+  return local_is_float(ge, a) || a.typecode == GA_BFLOAT16 ? "ga_float" : ctype(a.typecode);
+}
+
+// The kernel's parameter for a scalar: its name, but where the expression has a local of that name.
+std::string scalar_param(const ge_arg &a) { return a.typecode == GA_BFLOAT16 ? "ga_s_" + a.name : a.name; }
+
 // "T name;" plus the load, given an lvalue expression for the element.
 void emit_load(const GpuElemwise *ge, std::string &s, const ge_arg &a, const std::string &src) {
   const bool cvt = local_is_float(ge, a);
-  appendf(s, "%s %s;", cvt ? "ga_float" : ctype(a.typecode), a.name.c_str());
+  appendf(s, "%s %s;", local_ctype(ge, a), a.name.c_str());
   if (a.reads()) {
     if (cvt) appendf(s, " %s = ga_half2float(%s);", a.name.c_str(), src.c_str());
     else appendf(s, " %s = %s;", a.name.c_str(), src.c_str());
@@ -167,6 +176,14 @@ void emit_store(const GpuElemwise *ge, std::string &s, const ge_arg &a, const st
   if (!a.writes()) return;
   if (local_is_float(ge, a)) appendf(s, "%s = ga_float2half(%s);\n", dst.c_str(), a.name.c_str());
   else appendf(s, "%s = %s;\n", dst.c_str(), a.name.c_str());
+}
+
+// The expression, after the locals of scalars that are not what the kernel has as its parameter.
+void emit_expr(const GpuElemwise *ge, std::string &s) {
+  for (const ge_arg &a : ge->args)
+    if (!a.is_array() && a.typecode == GA_BFLOAT16)
+      appendf(s, "%s %s = %s;\n", local_ctype(ge, a), a.name.c_str(), scalar_param(a).c_str());
+  s += ge->expr;
 }
 
 void emit_header(const GpuElemwise *ge, std::string &s) {
@@ -267,7 +284,7 @@ std::string gen_flat(const GpuElemwise *ge, std::vector<int> &ktypes, unsigned u
       ktypes.push_back(GA_BUFFER);
       ktypes.push_back(GA_SIZE);
     } else {
-      appendf(s, ", %s %s", ctype(a.typecode), a.name.c_str());
+      appendf(s, ", %s %s", ctype(a.typecode), scalar_param(a).c_str());
       ktypes.push_back(a.typecode);
     }
   }
@@ -369,7 +386,7 @@ std::string gen_flat(const GpuElemwise *ge, std::vector<int> &ktypes, unsigned u
     appendf(s, "const ga_size i = ga_head + ga_c * %uu + ga_v; (void)i;\n{\n", V);
     for (const ge_arg &a : ge->args)
       if (a.is_array()) emit_load(ge, s, a, a.name + "_u[ga_u].e[ga_v]");
-    s += ge->expr;
+    emit_expr(ge, s);
     s += ";\n";
     for (const ge_arg &a : ge->args)
       if (a.is_array()) emit_store(ge, s, a, a.name + "_u[ga_u].e[ga_v]");
@@ -402,7 +419,7 @@ std::string gen_flat(const GpuElemwise *ge, std::vector<int> &ktypes, unsigned u
     if (pmask) s += p_coords("i");
     for (const ge_arg &a : ge->args)
       if (a.is_array()) emit_load(ge, s, a, is_p(a) ? p_elem(a, "ga_p0", "ga_p1", "ga_p2") : a.name + "_p[i]");
-    s += ge->expr;
+    emit_expr(ge, s);
     s += ";\n";
     for (const ge_arg &a : ge->args)
       if (a.is_array()) emit_store(ge, s, a, a.name + "_p[i]");
@@ -412,7 +429,7 @@ std::string gen_flat(const GpuElemwise *ge, std::vector<int> &ktypes, unsigned u
   if (pmask) s += p_coords("i");
   for (const ge_arg &a : ge->args)
     if (a.is_array()) emit_load(ge, s, a, is_p(a) ? p_elem(a, "ga_p0", "ga_p1", "ga_p2") : a.name + "_p[i]");
-  s += ge->expr;
+  emit_expr(ge, s);
   s += ";\n";
   for (const ge_arg &a : ge->args)
     if (a.is_array()) emit_store(ge, s, a, a.name + "_p[i]");
@@ -491,7 +508,7 @@ std::string gen_narrow_block(const GpuElemwise *ge, bool idx64, unsigned F, unsi
         ktypes.push_back(GA_SSIZE);
       }
     } else {
-      appendf(s, ", %s %s", ctype(a.typecode), a.name.c_str());
+      appendf(s, ", %s %s", ctype(a.typecode), scalar_param(a).c_str());
       ktypes.push_back(a.typecode);
     }
   }
@@ -637,7 +654,7 @@ std::string gen_narrow_block(const GpuElemwise *ge, bool idx64, unsigned F, unsi
         else src = elem_at(a, yy, l);
         emit_load(ge, s, a, src);
       }
-      s += ge->expr;
+      emit_expr(ge, s);
       s += ";\n";
       for (size_t j = 0; j < ge->args.size(); j++) {
         const ge_arg &a = ge->args[j];
@@ -776,7 +793,7 @@ std::string gen_narrow_staged(const GpuElemwise *ge, bool idx64, unsigned F, uns
         ktypes.push_back(GA_SSIZE);
       }
     } else {
-      appendf(s, ", %s %s", ctype(a.typecode), a.name.c_str());
+      appendf(s, ", %s %s", ctype(a.typecode), scalar_param(a).c_str());
       ktypes.push_back(a.typecode);
     }
   }
@@ -862,7 +879,7 @@ std::string gen_narrow_staged(const GpuElemwise *ge, bool idx64, unsigned F, uns
     };
     for (size_t j = 0; j < ge->args.size(); j++)
       if (ge->args[j].is_array()) emit_load(ge, s, ge->args[j], place(j));
-    s += ge->expr;
+    emit_expr(ge, s);
     s += ";\n";
     for (size_t j = 0; j < ge->args.size(); j++)
       if (ge->args[j].is_array() && ge->args[j].writes()) emit_store(ge, s, ge->args[j], place(j));
@@ -969,7 +986,7 @@ std::string gen_record_tiles(const GpuElemwise *ge, unsigned nd, bool idx64, uns
         ktypes.push_back(GA_SSIZE);
       }
     } else {
-      appendf(s, ", %s %s", ctype(a.typecode), a.name.c_str());
+      appendf(s, ", %s %s", ctype(a.typecode), scalar_param(a).c_str());
       ktypes.push_back(a.typecode);
     }
   }
@@ -1060,7 +1077,7 @@ std::string gen_record_tiles(const GpuElemwise *ge, unsigned nd, bool idx64, uns
     };
     for (size_t j = 0; j < ge->args.size(); j++)
       if (ge->args[j].is_array()) emit_load(ge, s, ge->args[j], place(j));
-    s += ge->expr;
+    emit_expr(ge, s);
     s += ";\n";
     for (size_t j = 0; j < ge->args.size(); j++)
       if (ge->args[j].is_array() && ge->args[j].writes()) emit_store(ge, s, ge->args[j], place(j));
@@ -1117,7 +1134,7 @@ std::string gen_strided(const GpuElemwise *ge, unsigned nd, bool idx64, unsigned
         ktypes.push_back(GA_SSIZE);
       }
     } else {
-      appendf(s, ", %s %s", ctype(a.typecode), a.name.c_str());
+      appendf(s, ", %s %s", ctype(a.typecode), scalar_param(a).c_str());
       ktypes.push_back(a.typecode);
     }
   }
@@ -1175,7 +1192,7 @@ std::string gen_strided(const GpuElemwise *ge, unsigned nd, bool idx64, unsigned
               a.name.c_str(), a.name.c_str(), I, I, a.name.c_str(), xd);
       emit_load(ge, s, a, at);
     }
-    s += ge->expr;
+    emit_expr(ge, s);
     s += ";\n";
     for (const ge_arg &a : ge->args) {
       if (!a.is_array()) continue;
@@ -1279,7 +1296,7 @@ std::string gen_strided(const GpuElemwise *ge, unsigned nd, bool idx64, unsigned
     if (is_t(j)) emit_load(ge, s, a, a.name + "_t[ga_lx * 65u + ga_ly]");
     else emit_load(ge, s, a, a.name + "_g[ga_k]");
   }
-  s += ge->expr;
+  emit_expr(ge, s);
   s += ";\n";
   for (size_t j = 0; j < ge->args.size(); j++) {
     const ge_arg &a = ge->args[j];
@@ -1349,7 +1366,7 @@ std::string gen_strided_vec(const GpuElemwise *ge, unsigned nd, bool idx64, unsi
         ktypes.push_back(GA_SSIZE);
       }
     } else {
-      appendf(s, ", %s %s", ctype(a.typecode), a.name.c_str());
+      appendf(s, ", %s %s", ctype(a.typecode), scalar_param(a).c_str());
       ktypes.push_back(a.typecode);
     }
   }
@@ -1507,7 +1524,7 @@ std::string gen_strided_vec(const GpuElemwise *ge, unsigned nd, bool idx64, unsi
     }
     for (const ge_arg &a : ge->args)
       if (a.is_array()) emit_load(ge, s, a, a.name + "_u[ga_e].e[ga_v]");
-    s += ge->expr;
+    emit_expr(ge, s);
     s += ";\n";
     for (const ge_arg &a : ge->args)
       if (a.is_array()) emit_store(ge, s, a, a.name + "_u[ga_e].e[ga_v]");
@@ -1800,7 +1817,7 @@ std::string gen_strided_vec(const GpuElemwise *ge, unsigned nd, bool idx64, unsi
     if (is_t(j)) emit_load(ge, s, a, a.name + "_t[ga_ly * " + TP + " + " + TCOL + "GA_QP(ga_v)]");
     else emit_load(ge, s, a, a.name + "_u[ga_k].e[ga_v]");
   }
-  s += ge->expr;
+  emit_expr(ge, s);
   s += ";\n";
   for (size_t j = 0; j < ge->args.size(); j++) {
     const ge_arg &a = ge->args[j];
