@@ -24,7 +24,7 @@ import numpy as np
 
 from . import gpuarray
 from . import reduction as _red
-from .dtypes import dtype_to_ctype, get_common_dtype, get_np_obj
+from .dtypes import bfloat16, dtype_to_ctype, get_common_dtype, get_np_obj
 from .elemwise import GpuElemwise, arg, as_argument, compare, elemwise1, elemwise2, ielemwise2
 
 _F16, _F32, _F64 = np.dtype("float16"), np.dtype("float32"), np.dtype("float64")
@@ -145,7 +145,7 @@ class ndgpuarray(gpuarray.GpuArray):
         kind, size = self.dtype.kind, self.dtype.itemsize
         if kind in "ub":
             return self.copy()
-        if kind == "f":
+        if kind == "f" or self.dtype == bfloat16:
             oper = "res = fabs(a)"
         elif size == 8:
             oper = "res = a < 0 ? -a : a"       # no 64-bit abs() in the device dialect

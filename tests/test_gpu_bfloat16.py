@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import libgpuarray_amd as ga
-from libgpuarray_amd import GpuElemwise, arg, gpuarray
+from libgpuarray_amd import GpuElemwise, arg, gpuarray, ndgpuarray
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,13 @@ def test_copies_keep_every_bit(ctx):
     b[:, ::-1] = a
     assert np.array_equal(bits(b), want[:, ::-1])
     assert np.array_equal(np.asarray(a.T.astype("float32")), ga.from_bfloat16(host.T), equal_nan=True)
+
+
+# ---- ndgpuarray -------------------------------------------------------------------------------------
+
+def test_abs(ctx):
+    x = np.concatenate([X, [-0.0, np.inf, -np.inf, np.nan]]).astype(np.float32)
+    got = abs(on_gpu(ctx, x, ndgpuarray))
+    assert type(got) is ndgpuarray
+    same(got, np.abs(x))
+    same(-on_gpu(ctx, x, ndgpuarray), -x)
