@@ -42,8 +42,8 @@ _COMPARE = {"lt": "<", "le": "<=", "eq": "==", "ne": "!=", "ge": ">=", "gt": ">"
 
 
 def _compute_ctype(dt):
-    """C type a result of dtype `dt` is computed in (halves are computed as floats)."""
-    return dtype_to_ctype(_F32 if dt == _F16 else dt)
+    """C type a result of dtype `dt` is computed in (what has 16 bits is computed as floats)."""
+    return dtype_to_ctype(_F32 if dt in (_F16, bfloat16) else dt)
 
 
 def _statement(dst, sym, float_form, ctype, x="a", y="b"):
@@ -68,11 +68,14 @@ def _inplace_ctype(name, self, other):
       /=   double if either side is float64, else float if either is float32
       //=  by the left array's type alone
       %=   by the common type, double only when the left array is float64 (so
-           that a float32 array and a Python float meet in float32, as in NumPy)."""
+           that a float32 array and a Python float meet in float32, as in NumPy;
+           so does whatever meets bfloat16, which has no common type in NumPy)."""
     if name not in ("truediv", "floordiv", "mod"):
         return None
     mine, theirs = self.dtype, np.asarray(get_np_obj(other)).dtype
-    if name == "mod":
+    if name == "mod" and bfloat16 in (mine, theirs):
+        kinds = (mine if mine == _F64 else _F32,)
+    elif name == "mod":
         kinds = (np.dtype(get_common_dtype(self, other, mine == _F64)),)
     elif name == "floordiv":
         kinds = (mine,)
@@ -80,7 +83,7 @@ def _inplace_ctype(name, self, other):
         kinds = (mine, theirs)
     if _F64 in kinds:
         return "double"
-    if _F32 in kinds or _F16 in kinds:
+    if _F32 in kinds or _F16 in kinds or bfloat16 in kinds:
         return "float"
     return None
 

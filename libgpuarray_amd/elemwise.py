@@ -192,7 +192,7 @@ def elemwise2(a, op, b, ary, odtype=None, oper=None,
         res = ary._empty_like_me(dtype=odtype)
     if oper is None:
         ot = odtype
-        if convert_f16 and ot == np.dtype("float16"):
+        if convert_f16 and ot == np.dtype("float16") or ot == bfloat16:
             ot = np.dtype("float32")
         oper = op_tmpl % {"op": op, "out_t": dtype_to_ctype(ot)}
     k = _kernel(ary.context, oper, args, convert_f16)

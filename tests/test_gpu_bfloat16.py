@@ -1,5 +1,7 @@
 """bfloat16 arrays under expressions and Python's operators: what is computed is the same on floats, rounded once to
 nearest even.  The reference has no such type; the rules are those of its half arrays."""
+import operator
+
 import numpy as np
 import pytest
 
@@ -107,3 +109,47 @@ def test_abs(ctx):
     assert type(got) is ndgpuarray
     same(got, np.abs(x))
     same(-on_gpu(ctx, x, ndgpuarray), -x)
+
+
+FORMS = {"floordiv": lambda a, b: np.floor((a / b).astype(np.float32)), "mod": np.fmod}
+
+
+@pytest.mark.parametrize("name", ["floordiv", "mod"])
+def test_floor_division_and_remainder(ctx, name):
+    """floor(a / b) and fmod(a, b) on floats, as for halves: of two arrays, in place and together."""
+    a, b = bf(X), bf(Y)
+    with np.errstate(all="ignore"):
+        want = FORMS[name](a, b)
+    x, y = on_gpu(ctx, a, ndgpuarray), on_gpu(ctx, b, ndgpuarray)
+    same(getattr(operator, name)(x, y), want)
+    same(divmod(x, y)[name == "mod"], want)
+    again = getattr(operator, "i" + name)(x, y)
+    assert again is x
+    same(x, want)
+
+
+@pytest.mark.parametrize("name", ["floordiv", "mod"])
+@pytest.mark.parametrize("other", [2.5, -3, np.float32(0.75)])
+def test_floor_division_and_remainder_by_a_number_in_place(ctx, name, other):
+    a = bf(X[:6])
+    x = on_gpu(ctx, a, ndgpuarray)
+    getattr(operator, "i" + name)(x, other)
+    same(x, FORMS[name](a, np.float32(other)))
+
+
+def test_floor_division_of_floats_by_bfloat16_in_place(ctx):
+    x = gpuarray.array(X[:6], context=ctx, cls=ndgpuarray)
+    y = on_gpu(ctx, bf(Y[:6]), ndgpuarray)
+    x //= y
+    assert np.array_equal(np.asarray(x), np.floor(X[:6] / bf(Y[:6])))
+    x = gpuarray.array(X[:6], context=ctx, cls=ndgpuarray)
+    x %= y
+    assert np.array_equal(np.asarray(x), np.fmod(X[:6], bf(Y[:6])))
+
+
+def test_helpers_compute_on_floats(ctx):
+    """elemwise2 with the result's type given: operands of more bits keep them."""
+    from libgpuarray_amd.elemwise import elemwise2
+    a = (X * np.float32(1 + 2.0 ** -9))
+    x, y = gpuarray.array(a, context=ctx), on_gpu(ctx, Y)
+    same(elemwise2(x, "-", y, x, odtype=ga.bfloat16), a - bf(Y))
