@@ -56,7 +56,7 @@ def _statement(dst, sym, float_form, ctype, x="a", y="b"):
 
 
 def _result_dtype(name, x, y):
-    if name == "truediv":
+    if name == "truediv" and not (getattr(x, "dtype", None) == bfloat16 == getattr(y, "dtype", None)):
         return np.asarray(get_np_obj(x) / get_np_obj(y)).dtype
     return get_common_dtype(x, y, True)
 

@@ -145,6 +145,8 @@ def get_common_dtype(obj1, obj2, allow_double):
 
 def upcast(*args):
     """reference pygpu/dtypes.py:195-199"""
+    if args and all(np.dtype(t) == bfloat16 for t in args):
+        return bfloat16
     a = np.array([0], dtype=args[0])
     for t in args[1:]:
         a = a + np.array([0], dtype=t)

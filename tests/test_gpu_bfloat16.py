@@ -153,3 +153,24 @@ def test_helpers_compute_on_floats(ctx):
     a = (X * np.float32(1 + 2.0 ** -9))
     x, y = gpuarray.array(a, context=ctx), on_gpu(ctx, Y)
     same(elemwise2(x, "-", y, x, odtype=ga.bfloat16), a - bf(Y))
+
+
+def test_division(ctx):
+    """bfloat16 is the type of what two of them give, as for + - *."""
+    a, b = bf(X), bf(Y)
+    x, y = on_gpu(ctx, a, ndgpuarray), on_gpu(ctx, b, ndgpuarray)
+    same(x / y, a / b)
+    x /= y
+    same(x, a / b)
+    x *= 0.5                                              # in place a number needs no common type
+    same(x, bf(a / b) * np.float32(0.5))
+    for what in (lambda: x / 2.0, lambda: 2.0 / x, lambda: x / gpuarray.zeros((10,), context=ctx, cls=ndgpuarray)):
+        with pytest.raises(TypeError):
+            what()
+
+
+def test_concatenation(ctx):
+    from libgpuarray_amd import operations
+    a, b = on_gpu(ctx, X), on_gpu(ctx, Y)
+    same(operations.concatenate([a, b, a[:3]]), np.concatenate([X, Y, X[:3]]))
+    same(operations.vstack([a, b]), np.stack([X, Y]))
