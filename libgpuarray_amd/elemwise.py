@@ -122,7 +122,7 @@ def _kernel(context, oper, args, convert_f16):
     context: the helpers below are called per operation (every `a + b` of an
     ndgpuarray), and building the C object costs several times a launch."""
     cache = context.__dict__.setdefault("_elemwise_cache", {})
-    key = (oper, convert_f16, tuple((x.name, x.dtype.str, x.flags) for x in args))
+    key = (oper, convert_f16, tuple((x.name, x.dtype, x.flags) for x in args))
     k = cache.get(key)
     if k is None:
         if len(cache) >= 512:

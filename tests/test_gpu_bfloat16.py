@@ -174,3 +174,21 @@ def test_concatenation(ctx):
     a, b = on_gpu(ctx, X), on_gpu(ctx, Y)
     same(operations.concatenate([a, b, a[:3]]), np.concatenate([X, Y, X[:3]]))
     same(operations.vstack([a, b]), np.stack([X, Y]))
+
+
+def test_records_of_two_bytes_have_kernels_of_their_own(ctx):
+    """NumPy names every record of two bytes alike; what is kept for one type must not serve another."""
+    from libgpuarray_amd.elemwise import elemwise1
+    pair = np.dtype([("low", "u1"), ("high", "u1")])
+    gpuarray.register_dtype(pair, "pair_of_bytes")
+    host = np.array([(1, 2), (250, 255), (7, 0)], pair)
+    mark = "res = a; "                                  # of this test alone: no kernel is kept for it yet
+    same(elemwise1(on_gpu(ctx, X), None, oper=mark), X)
+    a = gpuarray.array(host, context=ctx)
+    with pytest.raises(ga.GpuArrayException):           # the kernel texts know no type of that name
+        elemwise1(a, None, oper=mark)
+    text = ("typedef struct { ga_ubyte low, high; } pair_of_bytes;\n")
+    out = gpuarray.empty((3,), pair, context=ctx)
+    GpuElemwise(ctx, "r.low = a.high; r.high = a.low", [arg("r", pair, write=True), arg("a", pair, read=True)],
+                preamble=text)(out, a)
+    assert np.array_equal(np.asarray(out)["low"], host["high"]) and np.array_equal(np.asarray(out)["high"], host["low"])
