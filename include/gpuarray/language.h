@@ -116,7 +116,7 @@ GPUARRAY_PUBLIC int GpuArray_token_logprobs_grad(
     const GpuArray *dentropy, double scale, ssize_t ignore, int check_error);
 
 /* norm = sqrt(sum of the squares of all elements of the n arrays), summed in
- * 64 bits.  norm is 0-d (or has one element), GA_FLOAT or GA_DOUBLE.  The
+ * 64 bits, also of doubles whose squares are in none.  norm is 0-d (or has one element), GA_FLOAT or GA_DOUBLE.  The
  * arrays are contiguous, in either order, of any shapes and of mixed types;
  * one that is listed twice counts twice. */
 GPUARRAY_PUBLIC int GpuArray_global_norm(GpuArray *norm, const GpuArray **as,

@@ -270,6 +270,9 @@ def main():
     for kind in (4, 5):
         check("norm operator %d on a table in device memory" % kind, gen_l(kind | GA_FLOAT << 8 | GA_FLOAT << 20 | GA_INT << 32 | 1 << 44))
         lm += 1
+    for extra in (2, 3):
+        check("norm with doubles, variant %d" % extra, gen_l(4 | GA_FLOAT << 8 | GA_FLOAT << 20 | GA_INT << 32 | extra << 44))
+        lm += 1
     for ids, items in [(GA_INT, 1), (GA_LONG, 4), (GA_LONG, 16)]:
         check("tokens in the order of their ids, %d a lane" % items, gen_l(6 | GA_FLOAT << 8 | GA_FLOAT << 20 | ids << 32 | items << 44))
         lm += 1

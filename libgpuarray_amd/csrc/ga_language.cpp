@@ -101,7 +101,8 @@ struct norm_args {      // followed by the arrays themselves, or the address of 
   void *partials, *result, *norm, *counter;
   double max_norm;
   uint32_t partial0, npartials, n, pieces, piece;
-  int32_t norm_double, pad[2];
+  int32_t norm_double;
+  uint32_t ends, pad;
 };
 struct tensors_args {
   norm_args a;
@@ -123,7 +124,8 @@ std::string lm_source(const lm_variant &v) {
   name("LM_ID", v.id);
   if (v.kind == LM_EMBED_GRAD) s += std::string("#define LM_NARROW ") + (v.extra ? "1\n" : "0\n");
   if (v.kind == LM_SORT) s += "#define LM_R " + std::to_string(v.extra ? v.extra : 4) + "\n";
-  if (v.kind == LM_NORM || v.kind == LM_CLIP) s += "#define LM_TENSORS " + std::to_string(v.extra ? 0 : LM_TENSORS) + "\n";
+  if (v.kind == LM_NORM || v.kind == LM_CLIP) s += "#define LM_TENSORS " + std::to_string(v.extra & 1 ? 0 : LM_TENSORS) + "\n";
+  if (v.kind == LM_NORM) s += std::string("#define LM_ENDS ") + (v.extra & 2 ? "1\n" : "0\n");
   if (v.kind == LM_LOGPROBS_GRAD) s += std::string("#define LM_ENT ") + (v.extra ? "1\n" : "0\n");
   if (v.kind == LM_LOGPROBS) {
     s += "#define LM_LANES " + std::to_string((v.extra & 31 ? v.extra & 31 : 1) * 64) + "\n";
@@ -734,6 +736,7 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
 // What a call works on: arrays with at least one element, in pieces.
 struct norm_plan {
   std::vector<tensor_arg> tensors;
+  bool doubles = false;   // whose squares may leave the range of a double
 };
 
 // Pieces of 16 KiB: four chunks for each lane of a group, loaded at once.
@@ -792,6 +795,7 @@ static int norm_arrays(argument_rules &c, GpuArray **rs, const GpuArray **as, si
     tensor_arg t = {at(a), at(r), (int64_t)count, (uint32_t)p,   // (`first` holds the count of pieces until a table is made)
                     a->typecode == GA_FLOAT ? 0u : a->typecode == GA_HALF ? 1u : a->typecode == GA_BFLOAT16 ? 2u : 3u};
     plan->tensors.push_back(t);
+    plan->doubles |= a->typecode == GA_DOUBLE;
   }
   // no two results overlap, and none overlaps an operand that is not itself
   std::sort(written.begin(), written.end());
@@ -825,18 +829,21 @@ struct norm_table {
   const void *device;
   uint32_t n, pieces;
 };
-static int norm_run(argument_rules &c, const std::vector<norm_table> &tables, bool clip, double max_norm, const GpuArray *norm) {
+static int norm_run(argument_rules &c, const std::vector<norm_table> &tables, bool doubles, bool clip, double max_norm,
+                    const GpuArray *norm) {
   gpucontext *ctx = c.ctx;
   const bool by_table = tables.size() == 1 && tables[0].tensors == nullptr;
   const size_t size = by_table ? sizeof(table_args) : sizeof(tensors_args);
-  const lm_variant vn(LM_NORM, GA_FLOAT, GA_FLOAT, GA_INT, by_table), vc(LM_CLIP, GA_FLOAT, GA_FLOAT, GA_INT, by_table);
+  const lm_variant vn(LM_NORM, GA_FLOAT, GA_FLOAT, GA_INT, by_table | (doubles ? 2u : 0u)), vc(LM_CLIP, GA_FLOAT, GA_FLOAT, GA_INT, by_table);
   char *scratch = nullptr;
   void *counters = nullptr;
   GpuKernel *kpieces = nullptr, *kclip = nullptr;
   int err = lm_kernel(ctx, vn, "lm_norm_pieces", size, &kpieces);
   if (err == GA_NO_ERROR && clip) err = lm_kernel(ctx, vc, "lm_clip_pieces", size, &kclip);
   if (err == GA_NO_ERROR) err = lm_counters(ctx, &counters);
-  if (err == GA_NO_ERROR) err = lm_scratch(ctx, 256 + tables.size() * NORM_MAX_GROUPS * sizeof(double), &scratch);
+  // partial sums: of the squares, and where there are doubles of the large and of the small ones behind them
+  const size_t partials = tables.size() * NORM_MAX_GROUPS;
+  if (err == GA_NO_ERROR) err = lm_scratch(ctx, 256 + (doubles ? 3 : 1) * partials * sizeof(double), &scratch);
   if (err != GA_NO_ERROR) return err;
 
   tensors_args args;
@@ -849,6 +856,7 @@ static int norm_run(argument_rules &c, const std::vector<norm_table> &tables, bo
   a.norm_double = norm != nullptr && norm->typecode == GA_DOUBLE;
   a.max_norm = max_norm;
   a.piece = (uint32_t)NORM_PIECE;
+  a.ends = doubles ? (uint32_t)partials : 0;
   auto take = [&](const norm_table &t) {
     a.n = t.n;
     a.pieces = t.pieces;
@@ -890,7 +898,7 @@ static int norm_and_clip(GpuArray **rs, const GpuArray **as, size_t n, double ma
     tables.back().pieces += p;
   }
   if (tables.empty()) tables.push_back({nullptr, nullptr, 0, 0});
-  return norm_run(c, tables, rs != nullptr, max_norm, norm);
+  return norm_run(c, tables, plan.doubles, rs != nullptr, max_norm, norm);
 }
 
 struct _GpuGlobalNorm {
@@ -942,7 +950,7 @@ static int global_norm_call(const GpuGlobalNorm *g, bool clip, double max_norm, 
   if (g->table == nullptr && norm == nullptr) return GA_NO_ERROR;
   const std::vector<norm_table> tables = {
       {nullptr, g->table ? g->table->devptr : nullptr, (uint32_t)g->plan.tensors.size(), g->pieces}};
-  return norm_run(c, tables, clip, max_norm, norm);
+  return norm_run(c, tables, g->plan.doubles, clip, max_norm, norm);
 }
 
 // ---- the C entry points: nothing thrown leaves them ----------------------------------

@@ -1585,14 +1585,15 @@ struct lm_tensor {
   ga_uint first, type;           /* type: 0 float, 1 half, 2 bfloat16, 3 double */
 };
 struct lm_tensors {
-  GLOBAL_MEM double *partials;   /* sums of squares, one per group */
+  GLOBAL_MEM double *partials;   /* sums of squares, one per group; `ends` later, of the large and the small ones */
   GLOBAL_MEM double *result;     /* the factor */
   GLOBAL_MEM void *norm;
   GLOBAL_MEM ga_uint *counter;   /* a zero that the last table's groups count on; NULL for the others */
   double max_norm;
   ga_uint partial0, npartials;
   ga_uint n, pieces, piece;
-  ga_int norm_double, pad[2];
+  ga_int norm_double;
+  ga_uint ends, pad;             /* (of LM_ENDS) */
 #if LM_TENSORS
   lm_tensor tensors[LM_TENSORS];
 #else
@@ -1616,8 +1617,13 @@ LM_FN ga_uint lm_find(const lm_tensors &p, ga_uint piece) {
     case 0: F(ga_float); break;   \
     case 1: F(ga_half); break;    \
     case 2: F(ga_bfloat16); break; \
-    default: F(ga_double); break; \
+    LM_DOUBLES(F)                 \
   }
+#if LM_KIND == LM_K_CLIP || LM_ENDS
+#define LM_DOUBLES(F) default: F(ga_double); break;
+#else
+#define LM_DOUBLES(F)
+#endif
 LM_FN double lm_lane_xor(double v, int mask) {
   const ga_ulong b = __builtin_bit_cast(ga_ulong, v);
   const int from = (int)(((LID_0 & 63) ^ mask) << 2);
@@ -1625,16 +1631,9 @@ LM_FN double lm_lane_xor(double v, int mask) {
   const ga_uint hi = (ga_uint)__builtin_amdgcn_ds_bpermute(from, (int)(ga_uint)(b >> 32));
   return __builtin_bit_cast(double, (ga_ulong)hi << 32 | lo);
 }
-/* the sum over a group */
-LM_FN double lm_group_sum(double v) {
-  LOCAL_MEM double part[LM_GROUP / 64];
+LM_FN double lm_wave_sum(double v) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v += lm_lane_xor(v, d);
-  if ((LID_0 & 63) == 0) part[LID_0 >> 6] = v;
-  local_barrier();
-  v = part[0];
-#pragma unroll
-  for (int w = 1; w < LM_GROUP / 64; w++) v += part[w];
   return v;
 }
 LM_FN void lm_unpack(const lm_u4 &q, double *y, ga_double) {
@@ -1650,11 +1649,84 @@ template <> struct lm_wide<ga_double> { typedef double type; };
 #if LM_KIND == LM_K_NORM
 #define LM_U 8   /* chunks in flight per lane */
 
-/* The squares of n elements of type T, summed in 64 bits by the group:
- * a multiply-add of doubles costs what one of floats does, and neither the
- * largest nor the smallest float's square leaves their range. */
-template <class T> LM_FN double lm_squares(GLOBAL_MEM const T *x, ga_long n) {
+/* Sums of squares in 64 bits: a multiply-add of doubles costs what one of floats does, and neither the
+ * largest nor the smallest float's square leaves their range.  A double's may.  Where there are doubles
+ * (LM_ENDS) those past 2^486 and those below 2^-511 are summed on their own, multiplied by 2^-600 or 2^600, so that no sum of
+ * up to 2^50 squares overflows and none that counts is lost (three sums, as J. L. Blue has them, 1978).  Hardly any
+ * array has such numbers: a look at the upper words of a batch finds them, and what has none
+ * leaves and fetches one sum, whose sign says so (75 million doubles 105.6 us, unscaled 103.9; 3000 4.8 and 4.2). */
+struct lm_sums {
+  double s;
+#if LM_ENDS
+  double large, small;
+#endif
+};
+template <int N> LM_FN void lm_add_squares(lm_sums &, double (&s)[4], const float (&y)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; e++) s[e & 3] = __builtin_fma((double)y[e], (double)y[e], s[e & 3]);
+}
+#if LM_ENDS
+#define LM_LARGE 0x1p486
+#define LM_SMALL 0x1p-511
+#define LM_DOWN 0x1p-600
+#define LM_UP 0x1p600
+template <int N> LM_FN void lm_add_squares(lm_sums &t, double (&s)[4], const double (&y)[N]) {
+  bool far = false;
+#pragma unroll
+  for (int e = 0; e < N; e++)   /* the upper words of 2^-511 and 2^486 */
+    far |= ((ga_uint)(__builtin_bit_cast(ga_ulong, y[e]) >> 32) & 0x7fffffffu) - 0x20000000u >= 0x5e500000u - 0x20000000u;
+  if (__builtin_amdgcn_ballot_w64(far) == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e++) s[e & 3] = __builtin_fma(y[e], y[e], s[e & 3]);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < N; e++) {
+    const double a = __builtin_fabs(y[e]), l = a > LM_LARGE ? y[e] * LM_DOWN : 0.0, m = a < LM_SMALL ? y[e] * LM_UP : 0.0;
+    const double c = a > LM_LARGE || a < LM_SMALL ? 0.0 : y[e];
+    t.large = __builtin_fma(l, l, t.large);
+    t.small = __builtin_fma(m, m, t.small);
+    s[e & 3] = __builtin_fma(c, c, s[e & 3]);
+  }
+}
+LM_FN bool lm_ends(const lm_sums &t) { return t.large != 0.0 || t.small != 0.0; }
+LM_FN double lm_marked(double s, bool ends) { return __builtin_copysign(s, ends ? -1.0 : 1.0); }
+LM_FN bool lm_is_marked(double s) { return (__builtin_bit_cast(ga_ulong, s) >> 63) != 0; }
+#endif
+/* the sums over a group */
+LM_FN lm_sums lm_group_sum(lm_sums t) {
+  LOCAL_MEM double part[LM_GROUP / 64];
+  t.s = lm_wave_sum(t.s);
+#if LM_ENDS
+  LOCAL_MEM double large[LM_GROUP / 64], small[LM_GROUP / 64];
+  const bool ends = __builtin_amdgcn_ballot_w64(lm_ends(t)) != 0;
+  t.s = lm_marked(t.s, ends);
+  if (ends) {
+    t.large = lm_wave_sum(t.large);
+    t.small = lm_wave_sum(t.small);
+    if ((LID_0 & 63) == 0) large[LID_0 >> 6] = t.large, small[LID_0 >> 6] = t.small;
+  }
+#endif
+  if ((LID_0 & 63) == 0) part[LID_0 >> 6] = t.s;
+  local_barrier();
+#if LM_ENDS
+  t.s = t.large = t.small = 0.0;
+#pragma unroll
+  for (int w = 0; w < LM_GROUP / 64; w++) {
+    t.s += __builtin_fabs(part[w]);
+    if (lm_is_marked(part[w])) t.large += large[w], t.small += small[w];
+  }
+#else
+  t.s = part[0];
+#pragma unroll
+  for (int w = 1; w < LM_GROUP / 64; w++) t.s += part[w];
+#endif
+  return t;
+}
+/* The squares of n elements of type T. */
+template <class T> LM_FN void lm_squares(lm_sums &t, GLOBAL_MEM const T *x, ga_long n) {
   constexpr int E = 16 / (int)sizeof(T);
+  typedef typename lm_wide<T>::type wide;
   double s[4] = {0.0, 0.0, 0.0, 0.0};
   ga_long head = (ga_long)((-(ga_size)x & 15) / sizeof(T));
   if (head > n) head = n;
@@ -1663,22 +1735,18 @@ template <class T> LM_FN double lm_squares(GLOBAL_MEM const T *x, ga_long n) {
   GLOBAL_MEM const lm_u4 *q = (GLOBAL_MEM const lm_u4 *)(x + head);
   const ga_long k = LID_0 < head ? (ga_long)LID_0 : tail + (LID_0 - head);
   if (k < n) {
-    const double y = (double)lm_get(x[k]);
-    s[0] = y * y;
+    const wide y[1] = {lm_get(x[k])};
+    lm_add_squares(t, s, y);
   }
-  const auto add = [&](const lm_u4 &raw) {
-    typename lm_wide<T>::type y[E];
-    lm_unpack(raw, y, T());
-#pragma unroll
-    for (int e = 0; e < E; e++) s[e & 3] = __builtin_fma((double)y[e], (double)y[e], s[e & 3]);
-  };
   lm_u4 raw[LM_U];
   ga_uint c0 = 0;
   for (; c0 + LM_GROUP * LM_U <= whole; c0 += LM_GROUP * LM_U) {
+    wide y[LM_U * E];
 #pragma unroll
     for (int u = 0; u < LM_U; u++) raw[u] = q[c0 + u * LM_GROUP + LID_0];
 #pragma unroll
-    for (int u = 0; u < LM_U; u++) add(raw[u]);
+    for (int u = 0; u < LM_U; u++) lm_unpack(raw[u], y + u * E, T());
+    lm_add_squares(t, s, y);
   }
   if (c0 < whole) {     /* (unconditional loads: all of them in flight) */
 #pragma unroll
@@ -1687,20 +1755,36 @@ template <class T> LM_FN double lm_squares(GLOBAL_MEM const T *x, ga_long n) {
       raw[u] = q[c < whole ? c : whole - 1];
     }
 #pragma unroll
-    for (int u = 0; u < LM_U; u++)
-      if (c0 + u * LM_GROUP + LID_0 < whole) add(raw[u]);
+    for (int u = 0; u < LM_U; u++) {
+      wide y[E];
+      lm_unpack(raw[u], y, T());
+      if (c0 + u * LM_GROUP + LID_0 < whole) lm_add_squares(t, s, y);
+    }
   }
-  return (s[0] + s[1]) + (s[2] + s[3]);
+  t.s += (s[0] + s[1]) + (s[2] + s[3]);
 }
 /* The norm and the factor from all partial sums, by one group. */
 LM_FN void lm_norm_of_partials(const lm_tensors &p) {
-  double s = 0.0;
-  for (ga_uint k = LID_0; k < p.npartials; k += LM_GROUP)
-    s += __builtin_bit_cast(double, lm_fetch((GLOBAL_MEM const ga_ulong *)p.partials + k));
+  lm_sums t = {};
+  const auto part = [&](ga_uint k) { return __builtin_bit_cast(double, lm_fetch((GLOBAL_MEM const ga_ulong *)p.partials + k)); };
+  for (ga_uint k = LID_0; k < p.npartials; k += LM_GROUP) {
+#if LM_ENDS
+    const double s = part(k);
+    t.s += __builtin_fabs(s);
+    if (lm_is_marked(s)) t.large += part(p.ends + k), t.small += part(2 * p.ends + k);
+#else
+    t.s += part(k);
+#endif
+  }
   local_barrier();   /* (the LDS of an earlier sum is free again) */
-  s = lm_group_sum(s);
+  t = lm_group_sum(t);
+  double norm = __builtin_sqrt(t.s);
+#if LM_ENDS
+  if (t.large != 0.0) norm = __builtin_sqrt(t.s * LM_DOWN * LM_DOWN + t.large) * LM_UP;
+  else if (t.s == 0.0) norm = __builtin_sqrt(t.small) * LM_DOWN;
+  else if (t.small != 0.0) norm = __builtin_sqrt(t.s + t.small * LM_DOWN * LM_DOWN);
+#endif
   if (LID_0 == 0) {
-    const double norm = __builtin_sqrt(s);
     p.result[0] = norm > p.max_norm && norm < (double)INFINITY ? p.max_norm / norm : 1.0;
     if (p.norm != nullptr) {
       if (p.norm_double) *(GLOBAL_MEM double *)p.norm = norm;
@@ -1712,7 +1796,7 @@ LM_FN void lm_norm_of_partials(const lm_tensors &p) {
  * of bfloat16 in 148 arrays take 107 us (5.6 TB/s; the vector units are busy a quarter of that); 256 to 2048
  * groups, ranges or interleaved blocks of 1 to 16 pieces, streaming loads or none: no faster. */
 KERNEL void __launch_bounds__(LM_GROUP) lm_norm_pieces(const lm_tensors p) {
-  double s = 0.0;
+  lm_sums sums = {};
   const ga_uint share = (p.pieces + GDIM_0 - 1) / GDIM_0;
   ga_uint piece = GID_0 * share;
   const ga_uint end = p.pieces - piece < share ? p.pieces : piece + share;
@@ -1726,16 +1810,25 @@ KERNEL void __launch_bounds__(LM_GROUP) lm_norm_pieces(const lm_tensors p) {
     const ga_long per = (ga_long)p.piece * (16 / (ga_long)sizeof(T));             \
     const ga_long from = (ga_long)(piece - t.first) * per, left = t.count - from; \
     const ga_long n = (ga_long)(stop - piece) * per;                              \
-    s += lm_squares((GLOBAL_MEM const T *)t.in + from, left < n ? left : n);      \
+    lm_squares(sums, (GLOBAL_MEM const T *)t.in + from, left < n ? left : n);     \
   }
       LM_BY_TYPE(t.type, LM_SQUARES)
       piece = stop;
     }
   }
-  s = lm_group_sum(s);
+  sums = lm_group_sum(sums);
   LOCAL_MEM ga_uint last;
   if (LID_0 == 0) {
-    lm_publish((GLOBAL_MEM ga_ulong *)p.partials + p.partial0 + GID_0, __builtin_bit_cast(ga_ulong, s));
+    GLOBAL_MEM ga_ulong *mine = (GLOBAL_MEM ga_ulong *)p.partials + p.partial0 + GID_0;
+#if LM_ENDS
+    const bool ends = lm_ends(sums);
+    if (ends) {
+      lm_publish(mine + p.ends, __builtin_bit_cast(ga_ulong, sums.large));
+      lm_publish(mine + 2 * p.ends, __builtin_bit_cast(ga_ulong, sums.small));
+    }
+    sums.s = lm_marked(sums.s, ends);
+#endif
+    lm_publish(mine, __builtin_bit_cast(ga_ulong, sums.s));
     last = p.counter != nullptr && lm_count_in(p.counter, GDIM_0);
   }
   local_barrier();

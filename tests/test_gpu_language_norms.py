@@ -1,0 +1,70 @@
+"""The global norm and clipping at the ends of the range of their types, and norms alone."""
+import numpy as np
+import pytest
+
+import libgpuarray_amd as ga
+from libgpuarray_amd import gpuarray
+from test_gpu_language import U, decode
+
+pytestmark = pytest.mark.gpu
+
+
+def norm_of(hosts):
+    """The norm in 64 bits, of values that are brought near 1 by a power of two first."""
+    x = np.concatenate([np.ravel(decode(h)) for h in hosts])
+    big = np.abs(x).max() if x.size else 0.0
+    if big == 0 or not np.isfinite(big):
+        return float(big)
+    e = np.frexp(big)[1]
+    with np.errstate(over="ignore"):
+        return float(np.ldexp(np.sqrt((np.ldexp(x, -e) ** 2).sum()), e))
+
+
+DOUBLES = [[1e200], [-1e200, 1.0], [1e308, 1e308, 1e-308], [1e-200], [1e-170, 3e-162, -1e-200], [5e-324], [5e-324, 1e-310],
+           [1e-155, 1.0], [2.0 ** 486, 2.0 ** 487, 2.0 ** -511, 2.0 ** -512], [1.0, 2.0, 1e-300], [0.0], [1e154, 1e155]]
+
+
+@pytest.mark.parametrize("values", DOUBLES, ids=str)
+@pytest.mark.parametrize("count", [1, 9, 20001])
+def test_norm_of_doubles_of_any_size(ctx, values, count):
+    """Squares past 2^1024 and below 2^-1074 are in no double, the norm may be."""
+    rng = np.random.default_rng(count)
+    host = np.zeros(count * 3 + len(values))
+    at = rng.permutation(host.size)[: len(values) * min(count, 100)]
+    host[at] = np.resize(values, at.size) * rng.uniform(0.5, 1, at.size)
+    host[at[0]] = values[0]
+    others = np.full(700, 1.5, np.float32)
+    for hosts in ([host], [host, others], [others, host[: host.size // 2], host[host.size // 2:]]):
+        devs = [gpuarray.array(h, context=ctx) for h in hosts]
+        want = norm_of(hosts)
+        out = gpuarray.zeros((1,), "float64", context=ctx)
+        for norm in (ga.global_norm(devs, out), ga.GlobalNorm(devs).norm(gpuarray.zeros((1,), "float64", context=ctx))):
+            got = float(np.asarray(norm)[0])
+            if np.isinf(want):
+                assert np.isinf(got)
+                continue
+            # up to 2^16 squares, each and each addition off by 2^-53, a root, and a product with a power of two
+            assert abs(got - want) <= want * 2.0 ** -36 + 5e-324, (got, want)
+        with np.errstate(over="ignore"):
+            assert np.asarray(ga.global_norm(devs)) == np.float32(float(np.asarray(out)[0]))
+        if want == 0 or np.isinf(want):
+            continue
+        bound = want / 3.7 if want / 3.7 > 1e-290 else want * 2
+        by = bound / want if bound < want else 1.0
+        ga.clip_by_global_norm(devs, bound)
+        for h, d in zip(hosts, devs):
+            half = 2 * U if h.dtype == np.float32 else 2.0 ** -34
+            assert np.all(np.abs(decode(d) - decode(h) * by) <= np.abs(decode(h)) * by * half + 5e-324)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_doubles_without_a_norm_are_left_alone(ctx, bad):
+    host = np.full(3000, 1e-200)
+    host[77], host[1234] = 1e300, bad
+    a, b = gpuarray.array(host, context=ctx), gpuarray.array(np.ones(5, np.float32), context=ctx)
+    norm = np.asarray(ga.clip_by_global_norm([a, b], 1.0, norm=gpuarray.zeros((1,), "float64", context=ctx)))
+    assert not np.isfinite(norm[0])
+    assert np.array_equal(np.asarray(a), host, equal_nan=True) and np.all(np.asarray(b) == 1)
+    over = gpuarray.array(np.full(4, 1.5e308), context=ctx)     # the norm itself is in no double
+    assert np.isinf(np.asarray(ga.clip_by_global_norm([over], 1.0)))
+    assert np.all(np.asarray(over) == 1.5e308)
