@@ -126,7 +126,8 @@ GPUARRAY_PUBLIC int GpuArray_global_norm(GpuArray *norm, const GpuArray **as,
  * above max_norm, else rs[i] = as[i], without waiting for the norm on the
  * host.  rs[i] may be as[i] itself (rs == NULL: all of them are) or an array
  * of its shape, type and strides; no other overlap, between any two, is allowed.
- * The factor is rounded to 32 bits (64 for GA_DOUBLE), the product once.
+ * The factor is rounded to 32 bits (64 for GA_DOUBLE), the product once; where the
+ * factor is too small to be a normal number of that type, as[i] is divided by norm first, in 64 bits.
  * norm receives the norm before clipping, and may be NULL. */
 GPUARRAY_PUBLIC int GpuArray_clip_global_norm(GpuArray **rs,
                                               const GpuArray **as, size_t n,

@@ -4,7 +4,7 @@ import pytest
 
 import libgpuarray_amd as ga
 from libgpuarray_amd import gpuarray
-from test_gpu_language import U, decode
+from test_gpu_language import HALF_STEP, TINY, U, decode, encode
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,29 @@ def test_doubles_without_a_norm_are_left_alone(ctx, bad):
     over = gpuarray.array(np.full(4, 1.5e308), context=ctx)     # the norm itself is in no double
     assert np.isinf(np.asarray(ga.clip_by_global_norm([over], 1.0)))
     assert np.all(np.asarray(over) == 1.5e308)
+
+
+@pytest.mark.parametrize("kind,value,bound", [("float32", 3e38, 1.0), ("float32", 3e38, 1e-5), ("float32", 1e38, 1e-9), ("float32", 1e30, 1e-30),
+                                              ("bfloat16", 1e38, 1e-3), ("bfloat16", 3e38, 1e-20), ("float16", 6e4, 1e-38),
+                                              ("float64", 1e300, 1e-5), ("float64", 1e300, 1e-20), ("float64", 1e307, 1e-200)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_clipping_by_a_factor_below_the_smallest_normal_number(ctx, kind, value, bound, shift):
+    """max_norm / norm below 2^-126 (2^-1022 for doubles) has few bits left, or none; the product has all of them."""
+    rng = np.random.default_rng(3)
+    x = rng.uniform(-1, 1, 5000) * value / 64
+    x[[0, 4999]] = value, -value / 3
+    host = x if kind == "float64" else encode(x, kind)
+    want = norm_of([host[shift:]])
+    root = gpuarray.array(host, context=ctx)
+    into = gpuarray.empty((5000,), host.dtype, context=ctx)
+    devs, outs = [root[shift:]], [into[shift:]]
+    ga.clip_by_global_norm(devs, bound, out=outs)
+    exact = decode(host[shift:]) / want * bound
+    half, tiny = HALF_STEP.get(kind, 2.0 ** -36), TINY.get(kind, 5e-324)
+    assert np.all(np.abs(decode(outs[0]) - exact) <= np.abs(exact) * (half + 2.0 ** -34) + tiny)
+    op = ga.GlobalNorm(devs)                                   # in place, by the operator
+    op.clip(bound)
+    assert np.array_equal(decode(devs[0]), decode(outs[0]))
+    mixed = [gpuarray.array(np.full(3, 1e200), context=ctx), gpuarray.array(np.full(300, 1e30, np.float32), context=ctx)]
+    ga.clip_by_global_norm(mixed, 1.0)                         # a double's norm, a float's factor: 1e30 / 1.7e200 is 0 in a float
+    assert np.max(np.abs(np.asarray(mixed[0]) * np.sqrt(3) - 1)) < 2.0 ** -48 and not np.any(np.asarray(mixed[1]))
