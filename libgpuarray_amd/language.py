@@ -142,12 +142,14 @@ class GlobalNorm(object):
     """The 2-norm over all elements of a list of contiguous arrays, and
     clipping by it, for callers that clip the same gradients every step: `out`
     is the list of arrays that clipping writes (None: the arrays themselves,
-    no two of which may overlap then).  Holds the arrays, as they are now, and
+    no two of which may overlap then; False: none, for norms alone, where an array
+    may be listed twice).  Holds the arrays, as they are now, and
     a table of them on the device."""
 
     def __init__(self, arrays, out=None, context=None):
-        self.arrays, self.out, self.context, (a, r) = _lists(arrays, out, context)
-        if r is None and all(x.flags.writeable for x in self.arrays):
+        alone = out is False
+        self.arrays, self.out, self.context, (a, r) = _lists(arrays, None if alone else out, context)
+        if r is None and not alone and all(x.flags.writeable for x in self.arrays):
             r = a                  # (read-only arrays have a norm, but are not clipped in place)
         self.g = C.c_void_p()
         _check(lib.GpuGlobalNorm_new(C.byref(self.g), self.context.ctx, a, r, len(self.arrays)), self.context.ctx)

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 def norm_of(hosts):
     """The norm in 64 bits, of values that are brought near 1 by a power of two first."""
-    x = np.concatenate([np.ravel(decode(h)) for h in hosts])
+    x = np.concatenate([np.zeros(0)] + [np.ravel(decode(h)) for h in hosts])
     big = np.abs(x).max() if x.size else 0.0
     if big == 0 or not np.isfinite(big):
         return float(big)
@@ -94,3 +94,22 @@ def test_clipping_by_a_factor_below_the_smallest_normal_number(ctx, kind, value,
     mixed = [gpuarray.array(np.full(3, 1e200), context=ctx), gpuarray.array(np.full(300, 1e30, np.float32), context=ctx)]
     ga.clip_by_global_norm(mixed, 1.0)                         # a double's norm, a float's factor: 1e30 / 1.7e200 is 0 in a float
     assert np.max(np.abs(np.asarray(mixed[0]) * np.sqrt(3) - 1)) < 2.0 ** -48 and not np.any(np.asarray(mixed[1]))
+
+
+def test_norm_operator_without_results(ctx):
+    """out=False: norms alone, for lists that could not be clipped: one array twice, overlapping views, shared weights."""
+    x = gpuarray.array(np.arange(1, 2001, dtype=np.float32), context=ctx)
+    y = gpuarray.array(np.full((3, 5), 2.0, np.float64), context=ctx)
+    for arrays in ([x, x], [x[:100], x[50:150], y], [y], []):
+        op = ga.GlobalNorm(arrays, out=False, context=ctx)
+        want = norm_of([np.asarray(a) for a in arrays])
+        got = float(np.asarray(op.norm(gpuarray.zeros((), "float64", context=ctx))))
+        assert abs(got - want) <= want * 2.0 ** -40
+        assert op.out is None
+        with pytest.raises(ga.GpuArrayException):
+            op.clip(1.0)
+    assert np.array_equal(np.asarray(x), np.arange(1, 2001))
+    with pytest.raises(TypeError):                            # (it is the operator that is for norms alone)
+        ga.clip_by_global_norm([y], 1.0, out=False)
+    with pytest.raises(ga.GpuArrayException):                 # to be clipped in place, no two may overlap
+        ga.GlobalNorm([x, x])
