@@ -867,14 +867,19 @@ struct lm_state {
 };
 #define LM_LOWEST (-3.402823466e+38f)
 
-/* R(from) - R(to), from <= to; -300, which is as good as -inf for the exponential and safe to multiply
- * with 0, where that is lower, and for any two that differ where R(to) is past LM_FAR (both may be rounded to the same number). */
-LM_FN float lm_shift(float from, float to, float by) {
-  const float r = to * by, d = __builtin_fmaxf(from * by - r, -300.0f);
-  return from == to ? 0.0f : __builtin_fabsf(r) <= LM_FAR ? d : -300.0f;
+/* R(from) - R(to), from <= to, R(to) no farther out than LM_FAR; at least -300, which is as good as -inf for the
+ * exponential and safe to multiply with 0 */
+LM_FN float lm_near_shift(float from, float to, float by) {
+  const float d = __builtin_fmaxf(from * by - to * by, -300.0f);
+  return from == to ? 0.0f : d;
 }
-LM_FN void lm_rescale(lm_state &a, float m, float by) {
-  const float d = lm_shift(a.m, m, by), f = __builtin_amdgcn_exp2f(d);
+/* the same for any; farther out numbers that differ may have one R, and none but equal ones count */
+LM_FN float lm_shift(float from, float to, float by) {
+  const float r = to * by, d = __builtin_fabsf(r) <= LM_FAR ? __builtin_fmaxf(from * by - r, -300.0f) : -300.0f;
+  return from == to ? 0.0f : d;
+}
+LM_FN void lm_rescale(lm_state &a, float m, float d) {   /* d: the shift from a.m to m */
+  const float f = __builtin_amdgcn_exp2f(d);
 #if LM_ENT
   a.w = f * __builtin_fmaf(a.s, d, a.w);
 #endif
@@ -883,8 +888,8 @@ LM_FN void lm_rescale(lm_state &a, float m, float by) {
 }
 LM_FN void lm_join(lm_state &a, lm_state b, float by) {
   const float m = __builtin_fmaxf(a.m, b.m);
-  lm_rescale(a, m, by);
-  lm_rescale(b, m, by);
+  lm_rescale(a, m, lm_shift(a.m, m, by));
+  lm_rescale(b, m, lm_shift(b.m, m, by));
   a.s += b.s;
   a.w += b.w;
 }
@@ -899,7 +904,7 @@ template <int MASK> LM_FN void lm_sum_xor(lm_state &a) {
 LM_FN void lm_join_wave(lm_state &a, float by) {
   float m = a.m;
   lm_max_xor<1>(m); lm_max_xor<2>(m); lm_max_xor<7>(m); lm_max_xor<15>(m); lm_max_xor<16>(m); lm_max_xor<32>(m);
-  lm_rescale(a, m, by);
+  lm_rescale(a, m, lm_shift(a.m, m, by));
   lm_sum_xor<1>(a); lm_sum_xor<2>(a); lm_sum_xor<7>(a); lm_sum_xor<15>(a); lm_sum_xor<16>(a); lm_sum_xor<32>(a);
 }
 LM_FN float lm_max3(float a, float b, float c) {
@@ -917,11 +922,11 @@ template <int N> LM_FN float lm_max_of(const float (&y)[N], float a) {
 
 /* N elements of every lane join its statistics. */
 template <int N> LM_FN void lm_add(lm_state &a, const float (&y)[N], float most, float by) {
-  lm_rescale(a, __builtin_fmaxf(a.m, most), by);
-  const float r = a.m * by;
+  const float m = __builtin_fmaxf(a.m, most), r = m * by;
   const bool far = !(__builtin_fabsf(r) <= LM_FAR);
   float s[2] = {0.0f, 0.0f}, w[2] = {0.0f, 0.0f};
   if (__builtin_amdgcn_ballot_w64(far) == 0) {
+    lm_rescale(a, m, lm_near_shift(a.m, m, by));
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const float t = __builtin_fmaf(y[i], by, -r), e = __builtin_amdgcn_exp2f(t);
@@ -942,11 +947,12 @@ template <int N> LM_FN void lm_add(lm_state &a, const float (&y)[N], float most,
     }
 #endif
   } else {
+    lm_rescale(a, m, lm_shift(a.m, m, by));
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const float t = far ? 0.0f : __builtin_fmaf(y[i], by, -r);
       float e = __builtin_amdgcn_exp2f(t);
-      if (far) e = y[i] == a.m ? 1.0f : (y[i] != y[i] ? y[i] : 0.0f);
+      if (far) e = y[i] == m ? 1.0f : (y[i] != y[i] ? y[i] : 0.0f);
       s[i & 1] += e;
       w[i & 1] = __builtin_fmaf(e, __builtin_fmaxf(t, -300.0f), w[i & 1]);
     }
@@ -1194,10 +1200,9 @@ LM_FN lm_token lm_token_of(const lm_logprobs &p, ga_long r, LM_ID id) {
   }
   return k;
 }
-/* scale * (x - m), also where the difference is in no float (the product need not be so) */
-LM_FN float lm_scaled_difference(float x, float m, float scale) {
-  const float d = x - m;
-  return __builtin_fabsf(d) < INFINITY || x == -INFINITY ? d * scale : x * scale - m * scale;
+/* log p of an element: scale * (x - m) - ls, by halves, as the difference itself may be in no float */
+LM_FN float lm_logp(float x, float half_m, float scale, float ls) {
+  return __builtin_fmaf(__builtin_fmaf(x, 0.5f, -half_m) * scale, 2.0f, -ls);
 }
 /* What is written for row r; a whole wavefront. */
 LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a, ga_ulong list, lm_token token) {
@@ -1205,7 +1210,7 @@ LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a
   const float rm = a.m * p.by;
   const bool nothing = a.s == 0.0f;
   const float s = a.m == INFINITY ? NAN : a.s;
-  const float m = nothing ? -INFINITY : a.m;
+  const float m = nothing ? -INFINITY : a.m, half_m = 0.5f * m;
   const float lg = __builtin_logf(s);
   /* R(m) is off by * m by a rounding; past LM_FAR the sum is relative to m itself */
   const float off = __builtin_fabsf(rm) <= LM_FAR ? __builtin_fmaf(a.m, p.by, -rm) * 0.6931471805599453f : 0.0f;
@@ -1217,7 +1222,7 @@ LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a
         *p.err = -1;
         lp = NAN;
       } else if (token.id >= 0) {
-        lp = nothing ? -INFINITY : lm_scaled_difference(token.x, m, p.scale) - ls;
+        lp = nothing ? -INFINITY : lm_logp(token.x, half_m, p.scale, ls);
         if (ls != ls) lp = NAN;
       }
       *lm_at(p.logp, r * p.logp_step) = lp;
@@ -1244,7 +1249,7 @@ LM_FN void lm_logprobs_finish(const lm_logprobs &p, ga_long r, const lm_state &a
     if (lane < p.top) put(lane, NAN, lane);
     return;
   }
-  if (lane < n) put(lane, lm_scaled_difference(lm_key_value(list), m, p.scale) - ls, lm_key_index(list));
+  if (lane < n) put(lane, lm_logp(lm_key_value(list), half_m, p.scale, ls), lm_key_index(list));
   /* fewer than `top` elements above -inf: the lowest indices of -inf follow.
    * They are among the first 2 * 64 elements, or the row is shorter. */
   for (ga_long base = 0; n < p.top && base < p.v; base += 64) {
