@@ -475,13 +475,18 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   while (v >> bits != 0) bits++;
   const unsigned passes = (bits + 9) / 10;
   bits = (bits + passes - 1) / passes;
-  // Up to 4096 tokens one group sorts by itself, up to 16384 where clearing the
-  // rows takes longer than that (2.2 us for 1024 tokens); more are sorted by many,
-  // with few tokens a lane while there are few groups (kernel time of the sort of
-  // 8192 ids below 50257: one group 17 us, many 15; 16384: 37 and 16; 65536: one token a
-  // lane 17, four 26; 8192 tokens into 50257 rows of 1024 floats that are cleared: one group 50 us, many 59).
+  // Up to 8192 tokens, 8 a lane, one group sorts by itself, up to 16384 where clearing the
+  // rows takes longer than that; more are sorted by many, with few tokens a lane while there are
+  // few groups.  Kernel time of the sort of ids below 50257, us:
+  //   tokens                   4097    8192    8193   16384
+  //   one group                18.3    19.2    35.1    39.6
+  //   many                     21.1    23.0    23.2    20.0
+  //   tokens                  65536  250000  500000 1000000 1200000
+  //   one a lane                 24      32      40      65      79
+  //   two                        26      37      37      50      65
+  //   four                       30      41      48      48      62
   const size_t clear_bytes = accumulate ? 0 : v * d * osize;
-  const bool small = n <= 4096 || (n <= 16384 && clear_bytes / n >= 14000);
+  const bool small = n <= 8192 || (n <= 16384 && clear_bytes / n >= 14000);
   const size_t per_lane = small ? (n + 1023) / 1024 : n <= ((size_t)1 << 18) ? 1 : n <= ((size_t)1 << 20) ? 2 : 4;
   unsigned items = 1;
   while (items < per_lane) items *= 2;
@@ -620,12 +625,12 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
   // rows to fill the chip; below that, rows are cut in pieces of at least one
   // batch for each lane, of which the last one to end joins them all.  Rows of bfloat16 with
   // entropy, us by the lanes 64, 256, 512, 1024 (and pieces):
-  //   32768 rows of 2000     33    57   136   323
-  //   32768 rows of 4000     51    69   131   315
-  //   4096 rows of 50257     77    74    75    97
-  //   512 rows of 50257      35    15    13    16
-  //   128 rows of 50257      31    11     8.0   7.8   (8.3)
-  //   8 rows of 50257        24     8.0   6.2   6.5   (5.6)
+  //   32768 rows of 2000     32    59   139   331
+  //   32768 rows of 4000     51    68   134   324
+  //   4096 rows of 50257     68    68    73   101
+  //   512 rows of 50257      32    15    13    15
+  //   128 rows of 50257      30    11     7.9   7.8   (8.4)
+  //   8 rows of 50257        29     9.2   6.9   6.8   (5.6)
   const size_t row_chunks = v * gpuarray_get_elsize(logits->typecode) / 16 + 1;
   const size_t cus = ga_hip_numprocs(ctx) ? ga_hip_numprocs(ctx) : 256;
   unsigned lanes = 64;
