@@ -113,3 +113,21 @@ def test_norm_operator_without_results(ctx):
         ga.clip_by_global_norm([y], 1.0, out=False)
     with pytest.raises(ga.GpuArrayException):                 # to be clipped in place, no two may overlap
         ga.GlobalNorm([x, x])
+
+
+def test_long_lists_with_doubles_of_any_size(ctx):
+    """More arrays than travel with one launch, so that the partial sums come from several."""
+    rng = np.random.default_rng(5)
+    kinds = ["float64", "float32", "bfloat16"]
+    for large, small in ((1e250, 1e-250), (1.0, 1e-250), (0.0, 1e-250)):
+        hosts = [rng.uniform(0.5, 1, 5 + i % 9) * (large if i % 120 == 3 else small) if i % 3 == 0 else
+                 encode(rng.standard_normal(7) * (large == 1.0), kinds[i % 3]) for i in range(300)]
+        want = norm_of(hosts)
+        devs = [gpuarray.array(h, context=ctx) for h in hosts]
+        for norm in (ga.global_norm(devs, gpuarray.zeros((), "float64", context=ctx)),
+                     ga.GlobalNorm(devs).norm(gpuarray.zeros((), "float64", context=ctx))):
+            assert abs(float(np.asarray(norm)) - want) <= want * 2.0 ** -36
+        ga.clip_by_global_norm(devs, want / 8)
+        for h, d in zip(hosts, devs):
+            exact = decode(h) / 8
+            assert np.all(np.abs(decode(d) - exact) <= np.abs(exact) * 2.0 ** (-34 if h.dtype == np.float64 else -7))
