@@ -1094,7 +1094,7 @@ LM_FN void lm_raise(lm_best &b, ga_uint ordered) {
  * whoever misses a rise keeps more than it needs.  Where `top` is not small each of them
  * also leaves its m-th best element, m = top / W rounded up: no fewer than `top`
  * are not below the lowest of those, which is more than one of them finds alone
- * (4096 rows of 50257 bfloat16 with entropy: 50 alternatives 133 us, without parts 158; for 5 it is not
+ * (4096 rows of 50257 bfloat16 with entropy: 50 alternatives 126 us, without parts 153, 20 116 and 124; for 5 it is not
  * worth its barrier). */
 #define LM_WAVES (LM_LANES / 64)
 #if LM_LANES > 64 && LM_TOP
@@ -1348,7 +1348,7 @@ LM_FN void lm_join_pieces(const lm_logprobs &p, ga_long r) {
 
 /* One pass over the row with the running maximum and sums; what an element costs is a
  * multiply-add, an exponential and an addition, one more multiply-add with the entropy, and half a
- * maximum.  4096 rows of 50257 bfloat16 with entropy take 67 us (412 MB, 6.1 TB/s) where the vector
+ * maximum.  4096 rows of 50257 bfloat16 with entropy take 67 to 69 us (412 MB, 6.0 TB/s) where the vector
  * instructions alone take about 52; 65536 rows of 1000 floats with 5 alternatives 58 to 63 us
  * (262 MB, 4.3 TB/s): a wavefront sees its row in one batch, and the alternatives' networks and rounds
  * are half of its instructions.
