@@ -76,7 +76,8 @@ GPUARRAY_PUBLIC int GpuArray_embedding_grad(GpuArray *grad,
 #define GA_TOKEN_LOGPROBS_MAX_TOP 64
 
 /* Log probabilities under p(j) = exp(scale * x[j]) / sum_k exp(scale * x[k])
- * for each row x of logits (t, v); scale > 0 is an inverse temperature.
+ * for each row x of logits (t, v); scale > 0 is an inverse temperature, in 32
+ * bits and with scale * log2(e) in 32 bits too (up to 2.3e38).
  *   logp      (t)     log p of ids[i]; 0 where ids[i] is `ignore`, NaN where
  *                     it is out of range
  *   entropy   (t)     -sum p log p

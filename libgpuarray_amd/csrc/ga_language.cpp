@@ -243,6 +243,9 @@ bool overlaps_itself(const GpuArray *a) {
   return false;
 }
 
+// scale * log2(e), for exponentials of 2
+inline float in_powers_of_two(double scale) { return (float)((double)(float)scale * 1.4426950408889634); }
+
 // Checks of one operator's arguments; the first failure stays.
 struct argument_rules {
   gpucontext *ctx;
@@ -307,9 +310,13 @@ struct argument_rules {
       fail(GA_UNSUPPORTED_ERROR, "check_error waits, and the stream records a graph");
   }
   // a scale that a float holds
-  void scale(double s, bool positive) {
-    if (err == GA_NO_ERROR && (!std::isfinite((float)s) || (positive && !((float)s > 0.0f))))
-      fail(GA_VALUE_ERROR, positive ? "scale must be finite and above 0" : "scale must be finite");
+  void scale(double s) {
+    if (err == GA_NO_ERROR && !std::isfinite((float)s)) fail(GA_VALUE_ERROR, "scale must be finite");
+  }
+  // one of exponents, above 0, which a float holds in powers of two as well
+  void exponent_scale(double s) {
+    if (err == GA_NO_ERROR && !((float)s > 0.0f && std::isfinite(in_powers_of_two(s))))
+      fail(GA_VALUE_ERROR, "scale must be above 0, and finite when it is multiplied by log2(e)");
   }
 };
 
@@ -376,7 +383,7 @@ static int embedding(GpuArray *out, const GpuArray *table, const GpuArray *ids, 
   c.result(out, "out");
   c.apart(out, table, "out");
   c.apart(out, ids, "out");
-  c.scale(scale, false);
+  c.scale(scale);
   c.waits(check_error);
   if (c.err != GA_NO_ERROR) return c.err;
   if (n == 0 || d == 0) return GA_NO_ERROR;
@@ -418,7 +425,7 @@ static int embedding_grad(GpuArray *grad, const GpuArray *dout, const GpuArray *
   c.result(grad, "grad");
   c.apart(grad, dout, "grad");
   c.apart(grad, ids, "grad");
-  c.scale(scale, false);
+  c.scale(scale);
   c.waits(check_error);
   if (c.err != GA_NO_ERROR) return c.err;
   if (d == 0 || (v == 0 && n == 0)) return GA_NO_ERROR;
@@ -611,7 +618,7 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
     c.apart(results[i], ids, names[i]);
     for (int j = 0; j < i; j++) c.apart(results[i], results[j], names[i]);
   }
-  c.scale(scale, true);
+  c.exponent_scale(scale);
   c.waits(check_error);
   if (c.err != GA_NO_ERROR) return c.err;
   const size_t top = top_ids ? top_ids->dimensions[1] : 0;
@@ -669,7 +676,7 @@ static int token_logprobs(GpuArray *logp, GpuArray *entropy, GpuArray *stats, Gp
                      errbuf->devptr, scratch, logits->strides[0], step(ids, 0), step(logp, 0), step(entropy, 0),
                      step(stats, 0), step(stats, 1), step(top_logp, 0), step(top_logp, 1), step(top_ids, 0),
                      step(top_ids, 1), (int64_t)t, (int64_t)v, ignore, (float)scale,
-                     (float)((double)(float)scale * 1.4426950408889634), (int32_t)top,
+                     in_powers_of_two(scale), (int32_t)top,
                      top_ids != nullptr && top_ids->typecode == GA_LONG, (uint32_t)pieces, (uint32_t)piece_chunks,
                      (uint32_t)partial_bytes, 0, counters};
   err = lm_launch(k, groups, std::max(lanes, 256u), &a);
@@ -710,7 +717,7 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
   }
   c.apart(dlogits, stats, "dlogits");
   if (c.err == GA_NO_ERROR && !same_place(dlogits, logits)) c.apart(dlogits, logits, "dlogits");
-  c.scale(scale, true);
+  c.exponent_scale(scale);
   c.waits(check_error);
   if (c.err != GA_NO_ERROR) return c.err;
   if (t == 0 || v == 0) return GA_NO_ERROR;
@@ -730,7 +737,7 @@ static int token_logprobs_grad(GpuArray *dlogits, const GpuArray *logits, const 
   logprobs_grad_args a = {at(dlogits), at(logits), ptr(ids), at(stats), ptr(dlogp), ptr(entropy), ptr(dentropy),
                           errbuf->devptr, dlogits->strides[0], logits->strides[0], step(ids, 0), stats->strides[0],
                           stats->strides[1], step(dlogp, 0), step(entropy, 0), step(dentropy, 0), (int64_t)t,
-                          (int64_t)v, ignore, (float)scale, (float)((double)(float)scale * 1.4426950408889634),
+                          (int64_t)v, ignore, (float)scale, in_powers_of_two(scale),
                           (uint32_t)segments};
   err = lm_launch(k, (t * segments + 3) / 4, 256, &a);
   return err == GA_NO_ERROR && check_error ? lm_check_error(ctx, errbuf) : err;

@@ -14,7 +14,7 @@ import numpy as np
 import pytest
 
 import libgpuarray_amd as ga
-from libgpuarray_amd import gpuarray
+from libgpuarray_amd import _lib, gpuarray
 from test_gpu_language import HALF_STEP, TINY, U, decode, encode, grad64, logprob_bounds, run_logprobs, softmax64
 
 pytestmark = pytest.mark.gpu
@@ -223,3 +223,18 @@ def test_logits_farther_apart_than_a_float(ctx, scale, v):
     want = in_float(np.array([-2 * top, -4.5e38, -6e38, -4e38]) * scale)
     fin = np.isfinite(want)
     assert np.array_equal(got[~fin], want[~fin]) and np.all(np.abs(got[fin] - want[fin]) <= 6 * U * np.abs(want[fin]))
+
+
+# ---- the largest and smallest scales ------------------------------------------------------------------
+
+def test_scales_that_are_too_large_in_powers_of_two_are_refused(ctx):
+    z = lambda shape, dt="float32": gpuarray.zeros(shape, dt, context=ctx)  # noqa: E731
+    x, ids, t1, t2 = z((4, 16)), z((4,), "int64"), z((4,)), z((4, 2))
+    before = ctx.last_launch_hash()
+    for scale in (2.4e38, 3.4e38):
+        for call in (lambda: ga.token_logprobs(x, ids, scale=scale, out=ga.TokenLogprobs(t1, None, None, None, None)),
+                     lambda: ga.token_logprobs_grad(x, ids, t2, t1, scale=scale, out=x)):
+            with pytest.raises(ga.GpuArrayException) as e:
+                call()
+            assert e.value.code == _lib.GA_VALUE_ERROR
+    assert ctx.last_launch_hash() == before
