@@ -1538,8 +1538,11 @@ KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad 
   const bool nothing = ls == -INFINITY;
   const bool far = !(__builtin_fabsf(big) <= LM_FAR);   /* R is no part of the exponent then, as in the statistics */
   const float rest = (far ? 0.0f : __builtin_fmaf(p.by, m, -big)) + ls * 1.4426950408889634f;
-  const float a = -p.scale * (g + gh * h) + (ls - ls), b = -p.scale * gh * 0.6931471805599453f;   /* (NaN where ls is) */
-  const float own = p.scale * g;
+  /* a scale that would take A out of range, and 0 * A to NaN, is multiplied in at the end */
+  const bool steep = p.scale > 0x1p64f;
+  const float scale = steep ? p.scale * 0x1p-64f : p.scale;
+  const float a = -scale * (g + gh * h) + (ls - ls), b = -scale * gh * 0.6931471805599453f;   /* (NaN where ls is) */
+  const float own = scale * g;
 #pragma unroll
   for (int u = 0; u < LM_U; u++) {
     const ga_int c = at + u * 64 * LM_E;
@@ -1564,6 +1567,10 @@ KERNEL void __launch_bounds__(256) lm_logprobs_grad_rows(const lm_logprobs_grad 
       if (id >= from && id < from + LM_E) {
 #pragma unroll
         for (int e = 0; e < LM_E; e++) d[e] += from + e == id ? own : 0.0f;
+      }
+      if (steep) {
+#pragma unroll
+        for (int e = 0; e < LM_E; e++) d[e] *= 0x1p64f;
       }
     }
     if (from == c && v >= LM_E) {

@@ -171,14 +171,12 @@ def check_far_grad(ctx, x, kind, scale, rng):
     for stats, entropy, more in ((*exact, 0), (own.stats, own.entropy, joined)):
         limit = (bound + more) * (1 + 2.0 ** -7) + np.abs(want) * HALF_STEP[kind] + TINY[kind]
         got = decode(ga.token_logprobs_grad(dev(x), dev(ids), stats, dev(g), entropy=entropy, dentropy=dev(gh), scale=scale))
-        off = np.abs(got - want)
-        assert np.all(off <= limit), (np.argwhere(~(off <= limit))[:4], float(np.nanmax(off / limit)))
+        close(got, want, limit)          # (a gradient that no float holds is infinite)
         want_g, bound_g = grad64(x64, ids, g.astype(np.float64), np.zeros(t), scale)[:2]
         limit = (bound_g + scale * p * rest * np.abs(g)[:, None] + (more != 0) * scale * p * ls_err[:, None] * np.abs(g)[:, None])
         limit = limit * (1 + 2.0 ** -7) + np.abs(want_g) * HALF_STEP[kind] + TINY[kind]
         got = decode(ga.token_logprobs_grad(dev(x), dev(ids), stats, dev(g), scale=scale))
-        off = np.abs(got - want_g)
-        assert np.all(off <= limit), (np.argwhere(~(off <= limit))[:4], float(np.nanmax(off / limit)))
+        close(got, want_g, limit)
 
 
 @pytest.mark.parametrize("kind,low", CASES)
@@ -238,3 +236,15 @@ def test_scales_that_are_too_large_in_powers_of_two_are_refused(ctx):
                 call()
             assert e.value.code == _lib.GA_VALUE_ERROR
     assert ctx.last_launch_hash() == before
+
+
+@pytest.mark.parametrize("scale,size", [(2.3e38, 1e-38), (2.3e38, 1.0), (2.3e38, 1e30), (1e-30, 1e30), (1e-38, 3e38), (1e-38, 1.0)])
+def test_the_largest_and_smallest_scales(ctx, scale, size):
+    rng = np.random.default_rng(4)
+    scale = float(np.float32(scale))
+    x = (rng.uniform(-1, 1, (6, 900)) * size).astype(np.float32)
+    x[1, ::2] = x[1, 0]
+    x[2, 3] = -np.inf
+    x[3] = -size
+    check_far(ctx, x, scale, 5, rng)
+    check_far_grad(ctx, x, "float32", scale, rng)
